@@ -320,6 +320,134 @@ NIMBLE_API int nimble_adamw_step(float* weights, const void* grad, int grad_dtyp
                                  float weight_decay, void* weights_copy, int weights_copy_dtype,
                                  void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens, with entropy and top alternatives. The
+ * reference has a mean loss only; these serve policy gradients, preference
+ * losses and scoring.
+ * ------------------------------------------------------------------------- */
+
+/* Over logits that exist (n_rows x n_classes, rows row_pitch elements apart):
+ *   out_max[i], out_logsum[i]  row max m and log sum_j exp(x_ij - m); lse = their sum
+ *   out_logprob[i] = x_i,tokens[i] - lse_i
+ *   out_entropy[i] = -sum_j p_ij log p_ij            (p = exp(x - lse))
+ *   top_ids[i, :], top_logprobs[i, :]  the top_k classes of the row by logit,
+ *       best first, equal logits by the lowest class (0 <= top_k <= min(64,
+ *       n_classes); both null when top_k is 0).
+ * -inf logits are masked classes: probability zero, alternatives only when
+ * nothing else is left. A row of -inf only gives max and log probabilities
+ * -inf, logsum and entropy 0. A NaN or +inf logit makes the row's numbers NaN (NaN
+ * logits are no alternatives; missing ones are id -1, -inf). Rows whose token
+ * equals ignore_index are not read: log probability, entropy, max and logsum 0,
+ * alternatives id -1, -inf. A token outside [0, n_classes) that is not
+ * ignore_index sets NIMBLE_STATUS_BAD_LABEL and its log probability to NaN. */
+NIMBLE_API int nimble_token_logprobs_forward(const void* logits, int64_t row_pitch, const int64_t* tokens,
+                                             int64_t n_rows, int64_t n_classes, int dtype, int64_t ignore_index,
+                                             int top_k, float* out_logprob, float* out_entropy, float* out_max,
+                                             float* out_logsum, float* top_logprobs, int64_t* top_ids, int* status, void* stream);
+
+/* grad_logits_ij = a_i [j = tokens[i]] - p_ij (a_i + b_i (H_i + log p_ij)) with
+ * a = grad_logprob and b = grad_entropy (device, n_rows; a null one is zero).
+ * Zero rows for ignored and out-of-range tokens and for rows of -inf only. */
+NIMBLE_API int nimble_token_logprobs_backward(const float* grad_logprob, const float* grad_entropy,
+                                              const void* logits, int64_t row_pitch, const int64_t* tokens,
+                                              const float* row_max, const float* logsum, const float* entropy,
+                                              int64_t n_rows, int64_t n_classes, int dtype, int64_t ignore_index,
+                                              void* grad_logits, int64_t grad_row_pitch, void* stream);
+
+/* Bytes of workspace nimble_tied_logprobs_forward needs (f16 / bf16). */
+NIMBLE_API int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int64_t d_model, int64_t v_local,
+                                                           int dtype, size_t* bytes);
+
+/* The same two numbers from hidden states and the tied matrix, without an
+ * N x V buffer: statistics of one vocab shard, shard_stats (4, n_tokens) fp32 =
+ * row max m, sum 2^d, sum d 2^d with d = (s - m) log2 e, and the token's logit
+ * (0 where the shard does not hold it). f16 / bf16, fp32 accumulate. */
+NIMBLE_API int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
+                                            int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
+                                            int dtype, float* shard_stats, void* workspace, size_t workspace_bytes,
+                                            int* status, void* stream);
+
+/* Merges the statistics of n_shards shards ([n_shards][4][n_tokens]) in order
+ * into out_logprob, out_entropy and out_lse; ignored rows and bad tokens as in
+ * nimble_token_logprobs_forward. */
+NIMBLE_API int nimble_tied_logprobs_combine(const float* shard_stats, int n_shards, const int64_t* tokens,
+                                            int64_t n_tokens, int64_t vocab_size, int64_t ignore_index,
+                                            float* out_logprob, float* out_entropy, float* out_lse, int* status,
+                                            void* stream);
+
+/* Bytes of workspace nimble_tied_logprobs_backward needs; slab_bytes as in
+ * nimble_tied_ce_backward_workspace_size. */
+NIMBLE_API int nimble_tied_logprobs_backward_workspace_size(int64_t n_tokens, int64_t d_model, int64_t v_local,
+                                                            int dtype, size_t slab_bytes, size_t* bytes);
+
+/* Backward on one vocab shard: recomputes the logits slab by slab, forms the
+ * gradient of nimble_token_logprobs_backward in the compute dtype (fp16: times
+ * a power of two chosen from the largest row coefficient, undone in fp32) and
+ * computes grad_hidden (this shard's partial) and grad_weights as
+ * nimble_tied_ce_backward does. A null grad_hidden or grad_weights is not
+ * computed. hidden rows of ignored tokens must be finite: they are multiplied
+ * by zero gradients. */
+NIMBLE_API int nimble_tied_logprobs_backward(const float* grad_logprob, const float* grad_entropy,
+                                             const void* hidden, const void* weights, const int64_t* tokens,
+                                             const float* lse, const float* entropy, int64_t n_tokens,
+                                             int64_t d_model, int64_t v_local, int64_t v_offset, int64_t vocab_size,
+                                             int64_t ignore_index, int dtype, void* grad_hidden,
+                                             int grad_hidden_dtype, void* grad_weights, int grad_weights_dtype,
+                                             int accumulate_grad_weights, size_t slab_bytes, void* workspace,
+                                             size_t workspace_bytes, int* status, void* stream);
+
+/* Layer norm over the last dimension (d_model <= 8192):
+ *   y = (x - mean) * rstd * gamma + beta,  rstd = 1 / sqrt(var + eps)
+ * with the biased variance of centred values, fp32 statistics. x rows are
+ * x_row_pitch elements apart, y is contiguous; gamma and beta (null: none) are
+ * in param_dtype, the compute dtype or NIMBLE_DTYPE_F32. out_mean / out_rstd
+ * (both or neither) are what the backward needs. */
+NIMBLE_API int nimble_layernorm_forward(const void* x, int64_t x_row_pitch, const void* gamma, const void* beta,
+                                        int64_t n_rows, int64_t d_model, float eps, int dtype, int param_dtype,
+                                        void* y, float* out_mean, float* out_rstd, void* stream);
+
+/* Bytes of workspace nimble_layernorm_backward needs (16-byte aligned). */
+NIMBLE_API int nimble_layernorm_backward_workspace_size(int64_t n_rows, int64_t d_model, size_t* bytes);
+
+/* Layer norm backward: grad and grad_x are contiguous in the compute dtype,
+ * grad_gamma and grad_beta (null: not wanted) fp32, summed over the rows in a
+ * fixed order. */
+NIMBLE_API int nimble_layernorm_backward(const void* grad, const void* x, int64_t x_row_pitch, const void* gamma,
+                                         const float* mean, const float* rstd, int64_t n_rows, int64_t d_model,
+                                         int dtype, int param_dtype, void* grad_x, float* grad_gamma,
+                                         float* grad_beta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One tensor of nimble_adamw_step_many. weights are fp32 masters. With 32-bit
+ * moments exp_avg and exp_avg_sq are fp32 (n each) and the scales unused; with
+ * 8-bit moments they are e4m3 codes (n each) of the first moment and of the
+ * ROOT of the second, each run of 128 elements sharing one fp32 scale
+ * ((n + 127) / 128 each). weights_copy (null: none) receives the new weights. */
+typedef struct {
+  float* weights;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  void* weights_copy;
+  int64_t n;
+  int32_t grad_dtype;
+  int32_t weights_copy_dtype;
+} nimble_adamw_tensor;
+
+/* The update of nimble_adamw_step over n_tensors tensors (a HOST array, read
+ * before the call returns) in one launch per 400 tensors. Tensors must not
+ * overlap; any size and any alignment of whole elements. */
+NIMBLE_API int nimble_adamw_step_many(const nimble_adamw_tensor* tensors, int n_tensors, int moment_bits, double lr,
+                                      double beta1, double beta2, double bias_correction1, double bias_correction2,
+                                      double eps, double weight_decay, void* stream);
+
+/* 8-bit moments to and from fp32: out = code * scale, squared when root != 0
+ * (the second moment); quantize takes the root itself. */
+NIMBLE_API int nimble_adamw_dequantize(const void* codes, const float* scales, int64_t n, int root, float* out,
+                                       void* stream);
+NIMBLE_API int nimble_adamw_quantize(const float* x, int64_t n, int root, void* codes, float* scales, void* stream);
+
 /* Allocation-free variant of nimble_tied_ce_forward; no counterpart in the
  * reference. For callers that cannot allocate device memory (a runtime whose
  * GPU memory belongs to another framework's pool, or a binding that may only

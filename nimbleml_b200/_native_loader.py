@@ -94,6 +94,37 @@ SIGNATURES = {
     "nimble_adamw_step": (
         _c_int,
         [_c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_i64] + [ctypes.c_float] * 7 + [_c_vp, _c_int, _c_vp]),
+    "nimble_token_logprobs_forward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_int, _c_i64, _c_int] + [_c_vp] * 8),
+    "nimble_token_logprobs_backward": (
+        _c_int,
+        [_c_vp, _c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_int, _c_i64, _c_vp, _c_i64,
+         _c_vp]),
+    "nimble_tied_logprobs_forward_workspace_size": (
+        _c_int, [_c_i64, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_size)]),
+    "nimble_tied_logprobs_forward": (
+        _c_int,
+        [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_size, _c_vp, _c_vp]),
+    "nimble_tied_logprobs_combine": (
+        _c_int, [_c_vp, _c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "nimble_tied_logprobs_backward_workspace_size": (
+        _c_int, [_c_i64, _c_i64, _c_i64, _c_int, _c_size, ctypes.POINTER(_c_size)]),
+    "nimble_tied_logprobs_backward": (
+        _c_int,
+        [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_size, _c_vp, _c_size, _c_vp, _c_vp]),
+    "nimble_layernorm_forward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, ctypes.c_float, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp]),
+    "nimble_layernorm_backward_workspace_size": (_c_int, [_c_i64, _c_i64, ctypes.POINTER(_c_size)]),
+    "nimble_layernorm_backward": (
+        _c_int,
+        [_c_vp, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_int, _c_int, _c_vp, _c_vp, _c_vp, _c_vp,
+         _c_size, _c_vp]),
+    "nimble_adamw_step_many": (_c_int, [_c_vp, _c_int, _c_int] + [ctypes.c_double] * 7 + [_c_vp]),
+    "nimble_adamw_dequantize": (_c_int, [_c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_vp]),
+    "nimble_adamw_quantize": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_vp, _c_vp]),
     "nimble_tied_ce_backward": (
         _c_int,
         [_c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
@@ -149,6 +180,21 @@ class NativeLibrary:
     def rmsnorm_backward_workspace_size(self, n, d) -> int:
         out = _c_size(0)
         self.call("nimble_rmsnorm_backward_workspace_size", n, d, ctypes.byref(out))
+        return out.value
+
+    def tied_logprobs_forward_workspace_size(self, n, d, v_local, dtype) -> int:
+        out = _c_size(0)
+        self.call("nimble_tied_logprobs_forward_workspace_size", n, d, v_local, dtype, ctypes.byref(out))
+        return out.value
+
+    def tied_logprobs_backward_workspace_size(self, n, d, v_local, dtype, slab_bytes=0) -> int:
+        out = _c_size(0)
+        self.call("nimble_tied_logprobs_backward_workspace_size", n, d, v_local, dtype, slab_bytes, ctypes.byref(out))
+        return out.value
+
+    def layernorm_backward_workspace_size(self, n, d) -> int:
+        out = _c_size(0)
+        self.call("nimble_layernorm_backward_workspace_size", n, d, ctypes.byref(out))
         return out.value
 
 

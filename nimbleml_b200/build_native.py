@@ -24,15 +24,17 @@ REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libnimbleml_tied_ce.so"
-SOURCES = [CSRC / "tied_ce.cu", CSRC / "rowwise.cu"]
-HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "common.cuh", REPO_DIR / "include" / "nimbleml_tied_ce.h"]
+SOURCES = [CSRC / "tied_ce.cu", CSRC / "rowwise.cu", CSRC / "token_logprobs.cu", CSRC / "layernorm.cu",
+           CSRC / "adamw_many.cu"]
+HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "common.cuh", CSRC / "elementwise.cuh",
+           REPO_DIR / "include" / "nimbleml_tied_ce.h"]
 PYBIND_SOURCE = CSRC / "tied_ce_pybind.cpp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-    "-cudart", "static",
+    "-cudart", "static", "--threads", "0",
 ]
 
 

@@ -64,7 +64,12 @@ constexpr int kStagesWide = 3;
 constexpr int kSmemBytesPair = kStagesPair * (kABytes + kBBytes / 2) + kStoreBytes + 1024 + 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum Epi : int { EPI_CE_FWD = 0, EPI_CE_GRAD = 1, EPI_STORE = 2 };
+// EPI_LP_FWD / EPI_LP_GRAD are the cross-entropy epilogues of the per-token log
+// probabilities: the forward also sums d 2^d (d = (s - max) log2 e) for the
+// entropy, the gradient has coefficients of its own for every row.
+enum Epi : int { EPI_CE_FWD = 0, EPI_CE_GRAD = 1, EPI_STORE = 2, EPI_LP_FWD = 3, EPI_LP_GRAD = 4 };
+// Lower limit of d where it multiplies 2^d (zero long before).
+constexpr float kMinD = -1.0e4f;
 
 struct EpiParams {
   // Shared by the cross-entropy epilogues.
@@ -74,6 +79,10 @@ struct EpiParams {
   // EPI_CE_FWD
   float2* part;            // [n_tiles][M] per-tile (max, sum-exp)
   float* tgt;              // [M] target logit, written by the owning tile
+  // EPI_LP_FWD
+  float* part_u;           // [n_tiles][M] per-tile sum of d 2^d
+  // EPI_LP_GRAD
+  const float4* rowp;      // [M] (lse log2 e, onehot coefficient, c, b ln 2)
   // EPI_CE_GRAD
   const float* lse;        // [M]
   void* g;                 // [M][ldg]    G * gscale, compute dtype
@@ -379,11 +388,12 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       const int ncols = min(kBN, N - nb * kBN);
       const int64_t col0_tile = static_cast<int64_t>(nb) * kBN;
 
-      if constexpr (EPI == EPI_CE_FWD) {
+      if constexpr (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) {
         const int64_t lab = row_ok ? ep.labels[row] : INT64_MIN;
         const int64_t rel = (lab == INT64_MIN) ? -1 : lab - ep.col_origin - col0_tile;
         const int tcol = (rel >= 0 && rel < ncols) ? static_cast<int>(rel) : -1;
         float mrun = -INFINITY, srun = 0.0f, tval = 0.0f;
+        [[maybe_unused]] float urun = 0.0f;  // EPI_LP_FWD: sum of d 2^d
 #pragma unroll 1
         for (int c = c_begin; c < c_end; ++c) {
           if (c * 32 >= ncols) break;
@@ -407,12 +417,29 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           const float mnew = fmaxf(mrun, cm);
           const float ml2 = mnew * kLog2e;
           float s0 = 0.f, s1 = 0.f;
+          if constexpr (EPI == EPI_LP_FWD) {
+            float u0 = 0.f, u1 = 0.f;
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            s0 += ptx::ex2(fmaf(v[j], kLog2e, -ml2));
-            s1 += ptx::ex2(fmaf(v[j + 1], kLog2e, -ml2));
+            for (int j = 0; j < 32; j += 2) {
+              const float d0 = fmaf(v[j], kLog2e, -ml2), d1 = fmaf(v[j + 1], kLog2e, -ml2);
+              const float e0 = ptx::ex2(d0), e1 = ptx::ex2(d1);
+              s0 += e0;
+              s1 += e1;
+              u0 = fmaf(e0, fmaxf(d0, kMinD), u0);
+              u1 = fmaf(e1, fmaxf(d1, kMinD), u1);
+            }
+            const float dm = fmaxf((mrun - mnew) * kLog2e, kMinD);
+            const float f = ptx::ex2(dm);
+            urun = fmaf(urun + srun * dm, f, u0 + u1);
+            srun = fmaf(srun, f, s0 + s1);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              s0 += ptx::ex2(fmaf(v[j], kLog2e, -ml2));
+              s1 += ptx::ex2(fmaf(v[j + 1], kLog2e, -ml2));
+            }
+            srun = srun * ptx::ex2((mrun - mnew) * kLog2e) + (s0 + s1);
           }
-          srun = srun * ptx::ex2((mrun - mnew) * kLog2e) + (s0 + s1);
           mrun = mnew;
           const int jt = tcol - c * 32;
           if (static_cast<unsigned>(jt) < 32u) {
@@ -423,16 +450,24 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         }
         if (row_ok) {
           ep.part[(static_cast<int64_t>(nb) * kColHalves + ch) * M + row] = make_float2(mrun, srun);
+          if constexpr (EPI == EPI_LP_FWD) ep.part_u[(static_cast<int64_t>(nb) * kColHalves + ch) * M + row] = urun;
           // Only the warp whose column half holds the label writes the target.
           if (tcol >= c_begin * 32 && tcol < c_end * 32) ep.tgt[row] = tval;
         }
-      } else if constexpr (EPI == EPI_CE_GRAD) {
+      } else if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
         const int64_t lab = row_ok ? ep.labels[row] : ep.ignore_index;
         const bool live = row_ok && lab != ep.ignore_index;
         const int64_t rel = live ? lab - ep.col_origin - col0_tile : -1;
         const int tcol = (rel >= 0 && rel < ncols) ? static_cast<int>(rel) : -1;
-        const float lse_l2 = live ? ep.lse[row] * kLog2e : 0.0f;
-        const float gs = live ? ep.gscale : 0.0f;
+        float lse_l2, gs = 0.0f;
+        [[maybe_unused]] float4 rp = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if constexpr (EPI == EPI_LP_GRAD) {
+          if (live) rp = ep.rowp[row];
+          lse_l2 = rp.x;
+        } else {
+          lse_l2 = live ? ep.lse[row] * kLog2e : 0.0f;
+          gs = live ? ep.gscale : 0.0f;
+        }
         // The warp's 32 rows x 32 columns of G go through a swizzled staging
         // buffer and one TMA store (rows >= M / columns >= N are clipped by
         // the tensor map). Row bytes: 64 (16-bit, 64-byte swizzle) or 128
@@ -457,9 +492,16 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            float p = ptx::ex2(fmaf(__uint_as_float(r[j]), kLog2e, -lse_l2));
-            if (j == jt) p -= 1.0f;
-            v[j] = p * gs;
+            const float d = fmaf(__uint_as_float(r[j]), kLog2e, -lse_l2);
+            float p = ptx::ex2(d);
+            if constexpr (EPI == EPI_LP_GRAD) {
+              float w = -p * fmaf(rp.w, d, rp.z);
+              if (j == jt) w += rp.y;
+              v[j] = live ? w : 0.0f;
+            } else {
+              if (j == jt) p -= 1.0f;
+              v[j] = p * gs;
+            }
           }
           uint8_t* buf = wbuf + (store_seq % kBufs) * kBufBytes;
           if (store_seq >= kBufs && lane == 0) ptx::bulk_wait_read<kBufs - 1>();  // buffer's last store has read it
@@ -567,7 +609,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       release(acc);
     }
     // Every G store must have landed before the CTA exits.
-    if constexpr (EPI == EPI_CE_GRAD) {
+    if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
       if (lane == 0) ptx::bulk_wait<0>();
       __syncwarp();
     }
@@ -771,7 +813,7 @@ const int g_wide = [] {
 constexpr int kSmemBytesWide = kStagesWide * (2 * kABytes + kBBytes) + kStoreBytes + 1024 + 256;
 template <int EPI, bool kAMN>
 constexpr int gemm_kind_bit() {
-  return EPI == EPI_CE_FWD ? 1 : EPI == EPI_CE_GRAD ? 2 : kAMN ? 4 : 8;
+  return (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) ? 1 : (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) ? 2 : kAMN ? 4 : 8;
 }
 // Token blocks per rasterisation group (NIMBLEML_TIED_CE_GROUP_M, default 8: 2048 token rows with 256-row wide tiles).
 const int g_group_m = [] {
@@ -836,7 +878,7 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
   if (max_ctas > 0 && max_ctas < di.sms) di.sms = max_ctas;
   CUtensorMap ma, mb, mc;
   if (int rc = make_operand_map(&ma, A, dtype, kAMN, K, M, lda, kBM)) return rc;
-  if constexpr (EPI == EPI_CE_GRAD) {
+  if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
     if (int rc = make_store_map(&mc, ep.g, dtype, N, M, ep.ldg)) return rc;
   } else {
     mc = ma;  // unused by the other epilogues
@@ -895,7 +937,9 @@ int gemm_dispatch(int dtype, const void* A, int64_t lda, const void* B, int64_t 
     case NIMBLE_DTYPE_BF16:
       return launch_gemm<__nv_bfloat16, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
     case NIMBLE_DTYPE_F32:
-      return launch_gemm<float, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
+      // The log-probability epilogues serve 16-bit operands only.
+      if constexpr (EPI != EPI_LP_FWD && EPI != EPI_LP_GRAD)
+        return launch_gemm<float, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
   }
   return fail(NIMBLE_ERR_INVALID_ARG, "unknown dtype");
 }
@@ -1086,77 +1130,43 @@ extern "C" int nimble_round_tf32(const float* src, float* dst, int64_t n, void* 
 }
 
 namespace {
-int backward_impl(const float* grad_scale, const void* hidden, const void* weights, const int64_t* labels,
-                  const float* lse, const float* valid_count, int64_t n_tokens, int64_t d_model, int64_t v_local,
-                  int64_t v_offset, int64_t ignore_index, int dtype, void* grad_hidden, int grad_hidden_dtype,
-                  void* grad_weights, int grad_weights_dtype, int accumulate_grad_weights, size_t slab_bytes,
-                  void* workspace, size_t workspace_bytes, int* status, void* stream, void* dh_done_event,
-                  int last_de_max_ctas, float capped_fraction) {
-  if (int rc = check_common(hidden, weights, labels, n_tokens, d_model, v_local, dtype, true, true)) return rc;
-  if (!grad_weights || !grad_scale || !valid_count || (n_tokens > 0 && (!grad_hidden || !lse)))
-    return fail(NIMBLE_ERR_INVALID_ARG, "null pointer argument");
-  for (int dt : {grad_hidden_dtype, grad_weights_dtype})
-    if (dt != NIMBLE_DTYPE_F32 && dt != NIMBLE_DTYPE_F16 && dt != NIMBLE_DTYPE_BF16)
-      return fail(NIMBLE_ERR_INVALID_ARG, "bad output dtype");
-  if ((reinterpret_cast<uintptr_t>(grad_hidden) & 15) || (reinterpret_cast<uintptr_t>(grad_weights) & 15))
-    return fail(NIMBLE_ERR_INVALID_ARG, "gradient outputs must be 16-byte aligned");
-  if ((d_model * elem_size(grad_hidden_dtype)) % 16 || (d_model * elem_size(grad_weights_dtype)) % 16)
-    return fail(NIMBLE_ERR_INVALID_ARG, "d_model * output element size must be a multiple of 16 bytes");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (n_tokens == 0) {
-    if (!accumulate_grad_weights)
-      NIMBLE_CUDA_TRY(cudaMemsetAsync(grad_weights, 0, elem_size(grad_weights_dtype) * v_local * d_model, s));
-    return NIMBLE_OK;
-  }
-  const BwdLayout L = bwd_layout(n_tokens, d_model, v_local, dtype, slab_bytes, /*whole_vocab=*/!dh_done_event);
-  if (!workspace || workspace_bytes < L.total) return fail(NIMBLE_ERR_WORKSPACE, "backward workspace too small");
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
+// Walks the vocabulary slabs of a backward pass: the gradient epilogue EPI
+// (base parameters `eg`) recomputes a slab's logits and writes its G, then two
+// GEMMs add the slab's share of grad_hidden and write its grad_weights rows, both
+// times alpha = alpha_num / alpha_den * alpha_mult (device scalars, null = 1).
+// A null grad_hidden or grad_weights leaves that GEMM out.
+template <int EPI>
+int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, const float* alpha_num,
+                  const float* alpha_den, float alpha_mult, const void* h, const void* E, int64_t n_tokens,
+                  int64_t d_model, int64_t v_local, int64_t v_offset, int dtype, void* grad_hidden,
+                  int grad_hidden_dtype, void* grad_weights, int grad_weights_dtype, int accumulate_grad_weights,
+                  int* status, cudaStream_t s, void* dh_done_event, int last_de_max_ctas, float capped_fraction) {
   const int64_t es = elem_size(dtype);
-  const void* h = hidden;
-  const void* E = weights;
-  if (dtype == NIMBLE_DTYPE_F32) {
-    float* hr = reinterpret_cast<float*>(ws + L.hr);
-    float* er = reinterpret_cast<float*>(ws + L.er);
-    if (int rc = launch_round(static_cast<const float*>(hidden), hr, n_tokens * d_model, s)) return rc;
-    if (int rc = launch_round(static_cast<const float*>(weights), er, v_local * d_model, s)) return rc;
-    h = hr;
-    E = er;
-  }
-  if (dtype == NIMBLE_DTYPE_TF32) dtype = NIMBLE_DTYPE_F32;  // already rounded: read in place
   void* g = ws + L.g;
   float* dh_acc = L.n_slabs > 1 ? reinterpret_cast<float*>(ws + L.dh) : nullptr;
-
-  // G is stored scaled by 2^15 in fp16 so that softmax probabilities of order
-  // 1/V stay in the normal range; the scale is undone in the dE / dh epilogue.
-  const float gscale = dtype == NIMBLE_DTYPE_F16 ? 32768.0f : 1.0f;
   for (int64_t sl = 0; sl < L.n_slabs; ++sl) {
     const int64_t c0 = sl * L.slab;
     const int64_t vc = std::min<int64_t>(L.slab, v_local - c0);
     const void* E_sl = static_cast<const uint8_t*>(E) + es * c0 * d_model;
     // 1) recompute the slab's logits, write G [N x vc] (row pitch L.slab).
-    EpiParams eg{};
-    eg.labels = labels;
+    EpiParams eg = eg_base;
     eg.col_origin = v_offset + c0;
-    eg.ignore_index = ignore_index;
-    eg.lse = lse;
     eg.g = g;
     eg.ldg = L.slab;
-    eg.gscale = gscale;
-    eg.status = status;
-    if (int rc = gemm_dispatch<EPI_CE_GRAD>(dtype, h, d_model, E_sl, d_model, n_tokens, vc, d_model, eg, s)) return rc;
+    if (int rc = gemm_dispatch<EPI>(dtype, h, d_model, E_sl, d_model, n_tokens, vc, d_model, eg, s)) return rc;
     const bool last = sl == L.n_slabs - 1;
     // 2) dE[c0:c0+vc] = G^T h: A = G read MN-major ([tokens x vc]), B = h
     //    read MN-major ([tokens x d]); K = tokens.
     // dE rows [r0, r1) of the slab on at most max_ctas SMs (0 = all).
     auto run_de = [&](int max_ctas, int64_t r0, int64_t r1) -> int {
-      if (r1 <= r0) return NIMBLE_OK;
+      if (r1 <= r0 || !grad_weights) return NIMBLE_OK;
       EpiParams ee{};
       ee.out = static_cast<uint8_t*>(grad_weights) + elem_size(grad_weights_dtype) * (c0 + r0) * d_model;
       ee.ld_out = d_model;
       ee.out_dtype = grad_weights_dtype;
-      ee.alpha_num = grad_scale;
-      ee.alpha_den = valid_count;
-      ee.alpha_mult = 1.0f / gscale;
+      ee.alpha_num = alpha_num;
+      ee.alpha_den = alpha_den;
+      ee.alpha_mult = alpha_mult;
       ee.accum_out = accumulate_grad_weights ? 1 : 0;
       ee.status = status;
       return gemm_dispatch<EPI_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
@@ -1165,14 +1175,15 @@ int backward_impl(const float* grad_scale, const void* hidden, const void* weigh
     // 3) dh (+)= G E[c0:c0+vc]: A = G K-major, B = E slab read MN-major
     //    ([vc x d]); K = slab columns.
     auto run_dh = [&]() -> int {
+      if (!grad_hidden) return NIMBLE_OK;
       EpiParams eh{};
       eh.status = status;
       if (last) {
         eh.out = grad_hidden;
         eh.out_dtype = grad_hidden_dtype;
-        eh.alpha_num = grad_scale;
-        eh.alpha_den = valid_count;
-        eh.alpha_mult = 1.0f / gscale;
+        eh.alpha_num = alpha_num;
+        eh.alpha_den = alpha_den;
+        eh.alpha_mult = alpha_mult;
       } else {
         eh.out = dh_acc;
         eh.out_dtype = NIMBLE_DTYPE_F32;
@@ -1202,6 +1213,58 @@ int backward_impl(const float* grad_scale, const void* hidden, const void* weigh
     }
   }
   return NIMBLE_OK;
+}
+
+int backward_impl(const float* grad_scale, const void* hidden, const void* weights, const int64_t* labels,
+                  const float* lse, const float* valid_count, int64_t n_tokens, int64_t d_model, int64_t v_local,
+                  int64_t v_offset, int64_t ignore_index, int dtype, void* grad_hidden, int grad_hidden_dtype,
+                  void* grad_weights, int grad_weights_dtype, int accumulate_grad_weights, size_t slab_bytes,
+                  void* workspace, size_t workspace_bytes, int* status, void* stream, void* dh_done_event,
+                  int last_de_max_ctas, float capped_fraction) {
+  if (int rc = check_common(hidden, weights, labels, n_tokens, d_model, v_local, dtype, true, true)) return rc;
+  if (!grad_weights || !grad_scale || !valid_count || (n_tokens > 0 && (!grad_hidden || !lse)))
+    return fail(NIMBLE_ERR_INVALID_ARG, "null pointer argument");
+  for (int dt : {grad_hidden_dtype, grad_weights_dtype})
+    if (dt != NIMBLE_DTYPE_F32 && dt != NIMBLE_DTYPE_F16 && dt != NIMBLE_DTYPE_BF16)
+      return fail(NIMBLE_ERR_INVALID_ARG, "bad output dtype");
+  if ((reinterpret_cast<uintptr_t>(grad_hidden) & 15) || (reinterpret_cast<uintptr_t>(grad_weights) & 15))
+    return fail(NIMBLE_ERR_INVALID_ARG, "gradient outputs must be 16-byte aligned");
+  if ((d_model * elem_size(grad_hidden_dtype)) % 16 || (d_model * elem_size(grad_weights_dtype)) % 16)
+    return fail(NIMBLE_ERR_INVALID_ARG, "d_model * output element size must be a multiple of 16 bytes");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n_tokens == 0) {
+    if (!accumulate_grad_weights)
+      NIMBLE_CUDA_TRY(cudaMemsetAsync(grad_weights, 0, elem_size(grad_weights_dtype) * v_local * d_model, s));
+    return NIMBLE_OK;
+  }
+  const BwdLayout L = bwd_layout(n_tokens, d_model, v_local, dtype, slab_bytes, /*whole_vocab=*/!dh_done_event);
+  if (!workspace || workspace_bytes < L.total) return fail(NIMBLE_ERR_WORKSPACE, "backward workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const void* h = hidden;
+  const void* E = weights;
+  if (dtype == NIMBLE_DTYPE_F32) {
+    float* hr = reinterpret_cast<float*>(ws + L.hr);
+    float* er = reinterpret_cast<float*>(ws + L.er);
+    if (int rc = launch_round(static_cast<const float*>(hidden), hr, n_tokens * d_model, s)) return rc;
+    if (int rc = launch_round(static_cast<const float*>(weights), er, v_local * d_model, s)) return rc;
+    h = hr;
+    E = er;
+  }
+  if (dtype == NIMBLE_DTYPE_TF32) dtype = NIMBLE_DTYPE_F32;  // already rounded: read in place
+
+  // G is stored scaled by 2^15 in fp16 so that softmax probabilities of order
+  // 1/V stay in the normal range; the scale is undone in the dE / dh epilogue.
+  const float gscale = dtype == NIMBLE_DTYPE_F16 ? 32768.0f : 1.0f;
+  EpiParams eg{};
+  eg.labels = labels;
+  eg.ignore_index = ignore_index;
+  eg.lse = lse;
+  eg.gscale = gscale;
+  eg.status = status;
+  return slab_backward<EPI_CE_GRAD>(L, ws, eg, grad_scale, valid_count, 1.0f / gscale, h, E, n_tokens, d_model,
+                                    v_local, v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
+                                    grad_weights_dtype, accumulate_grad_weights, status, s, dh_done_event,
+                                    last_de_max_ctas, capped_fraction);
 }
 }  // namespace
 
@@ -1341,6 +1404,230 @@ extern "C" int nimble_tied_logits_backward(const void* grad_logits, int64_t grad
       return rc;
   }
   return NIMBLE_OK;
+}
+
+// =============================================== per-token log probabilities
+// logp_i = s_i,t - lse_i and H_i = -sum_j p_ij log p_ij for every token, from
+// the hidden states and the tied matrix: the forward GEMM with an epilogue that
+// also sums d 2^d, and the slab backward with a gradient of its own per row,
+//   G_ij = a_i [j = t_i] - p_ij (a_i + b_i H_i + b_i log p_ij),
+// a = d loss / d logp, b = d loss / d H. No N x V buffer exists in either pass.
+
+namespace nimble {
+namespace {
+
+// Merges the per-tile (max, sum 2^d, sum d 2^d) of each token into the shard's
+// statistics (4, M); the fourth row is the token's logit if the shard owns it.
+// Threads of a column of the block take every kReduceGroups-th tile of 32
+// neighbouring tokens (coalesced), then a fixed-order merge in shared memory.
+constexpr int kReduceGroups = 16;
+__global__ void __launch_bounds__(32 * kReduceGroups)
+lp_row_reduce_kernel(const float2* __restrict__ part, const float* __restrict__ part_u, int n_parts,
+                     const float* __restrict__ tgt, const int64_t* __restrict__ tokens, int64_t M, int64_t v_offset,
+                     int64_t v_local, float* __restrict__ stats) {
+  __shared__ float sm[3][kReduceGroups][32];
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  float m = -INFINITY, s = 0.0f, u = 0.0f;
+  auto merge = [&](float m2, float s2, float u2) {
+    const float mn = fmaxf(m, m2);
+    const float d1 = m == mn ? 0.0f : fmaxf((m - mn) * kLog2e, kMinD);
+    const float d2 = m2 == mn ? 0.0f : fmaxf((m2 - mn) * kLog2e, kMinD);
+    const float f1 = ptx::ex2(d1), f2 = ptx::ex2(d2);
+    u = (u + s * d1) * f1 + (u2 + s2 * d2) * f2;
+    s = s * f1 + s2 * f2;
+    m = mn;
+  };
+  if (row < M)
+    for (int t = grp; t < n_parts; t += kReduceGroups) {
+      const float2 p = part[static_cast<int64_t>(t) * M + row];
+      merge(p.x, p.y, part_u[static_cast<int64_t>(t) * M + row]);
+    }
+  sm[0][grp][lane] = m;
+  sm[1][grp][lane] = s;
+  sm[2][grp][lane] = u;
+  __syncthreads();
+  if (grp != 0 || row >= M) return;
+  for (int g = 1; g < kReduceGroups; ++g) merge(sm[0][g][lane], sm[1][g][lane], sm[2][g][lane]);
+  stats[row] = m;
+  stats[M + row] = s;
+  stats[2 * M + row] = u;
+  const int64_t tok = tokens[row];
+  stats[3 * M + row] = (tok >= v_offset && tok < v_offset + v_local) ? tgt[row] : 0.0f;
+}
+
+// Row coefficients of the gradient epilogue, scaled by a power of two that
+// fp16 G needs: |G_ij| <= |a_i| + |b_i| (H_i + 1/e), and the largest such bound
+// is brought to (2^14, 2^15], so that probabilities of order 1/V stay normal
+// numbers whatever the upstream gradients' size. bf16 has fp32's exponents and
+// is not scaled. scale[0] = 1 / factor goes to the dE / dh epilogues. One block.
+constexpr int kPrepThreads = 1024;
+__global__ void __launch_bounds__(kPrepThreads)
+lp_row_prep_kernel(const float* __restrict__ g_logp, const float* __restrict__ g_ent, const float* __restrict__ lse,
+                   const float* __restrict__ entropy, const int64_t* __restrict__ tokens, int64_t M, int64_t V,
+                   int64_t ignore_index, bool scaled, float4* __restrict__ rowp, float* __restrict__ scale) {
+  __shared__ float red[kPrepThreads / 32];
+  auto is_live = [&](int64_t i) {
+    const int64_t t = tokens[i];
+    return t != ignore_index && t >= 0 && t < V;
+  };
+  float factor = 1.0f;
+  if (scaled) {
+    float top = 0.0f;
+    for (int64_t i = threadIdx.x; i < M; i += kPrepThreads)
+      if (is_live(i))
+        top = fmaxf(top, (g_logp ? fabsf(g_logp[i]) : 0.0f) + (g_ent ? fabsf(g_ent[i]) * (entropy[i] + 0.37f) : 0.0f));
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int w = 0; w < kPrepThreads / 32; ++w) top = fmaxf(top, red[w]);
+    // 2^-100 < top < 2^100, else (all zero, infinite, NaN) no scale.
+    if (top > 7.9e-31f && top < 1.2e30f) {
+      int e;
+      frexpf(top, &e);  // top in [2^(e-1), 2^e)
+      factor = ldexpf(1.0f, 15 - e);
+    }
+  }
+  if (threadIdx.x == 0) scale[0] = 1.0f / factor;
+  for (int64_t i = threadIdx.x; i < M; i += kPrepThreads) {
+    float4 p = make_float4(1.0e30f, 0.0f, 0.0f, 0.0f);  // p = 2^-1e30 = 0
+    if (is_live(i)) {
+      const float a = g_logp ? g_logp[i] * factor : 0.0f;
+      const float b = g_ent ? g_ent[i] * factor : 0.0f;
+      p = make_float4(lse[i] * kLog2e, a, fmaf(b, entropy[i], a), b * 0.6931471805599453f);
+    }
+    rowp[i] = p;
+  }
+}
+
+int check_half(int dtype) {
+  if (dtype != NIMBLE_DTYPE_F16 && dtype != NIMBLE_DTYPE_BF16)
+    return fail(NIMBLE_ERR_INVALID_ARG, "tied log probabilities support f16 / bf16 compute");
+  return NIMBLE_OK;
+}
+
+struct LpFwdLayout {
+  size_t part = 0, part_u = 0, tgt = 0, total = 0;
+};
+LpFwdLayout lp_fwd_layout(int64_t N, int64_t V) {
+  LpFwdLayout L;
+  const int64_t n_parts = (V + kBN - 1) / kBN * kColHalves;
+  size_t off = 0;
+  L.part = off; off = align_up(off + sizeof(float2) * n_parts * N);
+  L.part_u = off; off = align_up(off + sizeof(float) * n_parts * N);
+  L.tgt = off; off = align_up(off + sizeof(float) * N);
+  L.total = off;
+  return L;
+}
+
+// The slab backward's workspace, then the row coefficients and the scale.
+struct LpBwdLayout {
+  BwdLayout slabs;
+  size_t rowp = 0, scale = 0, total = 0;
+};
+LpBwdLayout lp_bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t slab_bytes) {
+  LpBwdLayout L;
+  L.slabs = bwd_layout(N, d, V, dtype, slab_bytes);
+  size_t off = L.slabs.total;
+  L.rowp = off; off = align_up(off + sizeof(float4) * N);
+  L.scale = off; off = align_up(off + sizeof(float));
+  L.total = off;
+  return L;
+}
+
+}  // namespace
+}  // namespace nimble
+
+extern "C" int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int64_t d_model, int64_t v_local,
+                                                           int dtype, size_t* bytes) {
+  if (!bytes) return fail(NIMBLE_ERR_INVALID_ARG, "bytes is null");
+  if (int rc = check_half(dtype)) return rc;
+  if (n_tokens < 0 || d_model <= 0 || v_local <= 0) return fail(NIMBLE_ERR_INVALID_ARG, "sizes must be positive");
+  *bytes = lp_fwd_layout(n_tokens, v_local).total;
+  return NIMBLE_OK;
+}
+
+extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
+                                            int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
+                                            int dtype, float* shard_stats, void* workspace, size_t workspace_bytes,
+                                            int* status, void* stream) {
+  if (int rc = check_half(dtype)) return rc;
+  if (int rc = check_common(hidden, weights, tokens, n_tokens, d_model, v_local, dtype)) return rc;
+  if (v_offset < 0) return fail(NIMBLE_ERR_INVALID_ARG, "v_offset must be >= 0");
+  if (n_tokens == 0) return NIMBLE_OK;
+  if (!shard_stats) return fail(NIMBLE_ERR_INVALID_ARG, "null output pointer");
+  const LpFwdLayout L = lp_fwd_layout(n_tokens, v_local);
+  if (!workspace || workspace_bytes < L.total)
+    return fail(NIMBLE_ERR_WORKSPACE, "log probability forward workspace too small");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  EpiParams ep{};
+  ep.labels = tokens;
+  ep.col_origin = v_offset;
+  ep.part = reinterpret_cast<float2*>(ws + L.part);
+  ep.part_u = reinterpret_cast<float*>(ws + L.part_u);
+  ep.tgt = reinterpret_cast<float*>(ws + L.tgt);
+  ep.status = status;
+  if (int rc = gemm_dispatch<EPI_LP_FWD>(dtype, hidden, d_model, weights, d_model, n_tokens, v_local, d_model, ep, s))
+    return rc;
+  const int n_parts = static_cast<int>((v_local + kBN - 1) / kBN * kColHalves);
+  lp_row_reduce_kernel<<<static_cast<unsigned>((n_tokens + 31) / 32), 32 * kReduceGroups, 0, s>>>(
+      ep.part, ep.part_u, n_parts, ep.tgt, tokens, n_tokens, v_offset, v_local, shard_stats);
+  NIMBLE_CUDA_TRY(cudaGetLastError());
+  return NIMBLE_OK;
+}
+
+extern "C" int nimble_tied_logprobs_backward_workspace_size(int64_t n_tokens, int64_t d_model, int64_t v_local,
+                                                            int dtype, size_t slab_bytes, size_t* bytes) {
+  if (!bytes) return fail(NIMBLE_ERR_INVALID_ARG, "bytes is null");
+  if (int rc = check_half(dtype)) return rc;
+  if (n_tokens < 0 || d_model <= 0 || v_local <= 0) return fail(NIMBLE_ERR_INVALID_ARG, "sizes must be positive");
+  *bytes = lp_bwd_layout(n_tokens, d_model, v_local, dtype, slab_bytes).total;
+  return NIMBLE_OK;
+}
+
+extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const float* grad_entropy, const void* hidden,
+                                             const void* weights, const int64_t* tokens, const float* lse,
+                                             const float* entropy, int64_t n_tokens, int64_t d_model, int64_t v_local,
+                                             int64_t v_offset, int64_t vocab_size, int64_t ignore_index, int dtype,
+                                             void* grad_hidden, int grad_hidden_dtype, void* grad_weights,
+                                             int grad_weights_dtype, int accumulate_grad_weights, size_t slab_bytes,
+                                             void* workspace, size_t workspace_bytes, int* status, void* stream) {
+  if (int rc = check_half(dtype)) return rc;
+  if (int rc = check_common(hidden, weights, tokens, n_tokens, d_model, v_local, dtype)) return rc;
+  if (v_offset < 0 || v_offset + v_local > vocab_size)
+    return fail(NIMBLE_ERR_INVALID_ARG, "the shard must lie inside the vocabulary");
+  for (int dt : {grad_hidden_dtype, grad_weights_dtype})
+    if (!valid_dtype(dt)) return fail(NIMBLE_ERR_INVALID_ARG, "bad output dtype");
+  if ((reinterpret_cast<uintptr_t>(grad_hidden) & 15) || (reinterpret_cast<uintptr_t>(grad_weights) & 15))
+    return fail(NIMBLE_ERR_INVALID_ARG, "gradient outputs must be 16-byte aligned");
+  if ((d_model * elem_size(grad_hidden_dtype)) % 16 || (d_model * elem_size(grad_weights_dtype)) % 16)
+    return fail(NIMBLE_ERR_INVALID_ARG, "d_model * output element size must be a multiple of 16 bytes");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n_tokens == 0) {
+    if (grad_weights && !accumulate_grad_weights)
+      NIMBLE_CUDA_TRY(cudaMemsetAsync(grad_weights, 0, elem_size(grad_weights_dtype) * v_local * d_model, s));
+    return NIMBLE_OK;
+  }
+  if (!lse || !entropy) return fail(NIMBLE_ERR_INVALID_ARG, "null pointer argument");
+  const LpBwdLayout L = lp_bwd_layout(n_tokens, d_model, v_local, dtype, slab_bytes);
+  if (!workspace || workspace_bytes < L.total)
+    return fail(NIMBLE_ERR_WORKSPACE, "log probability backward workspace too small");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float4* rowp = reinterpret_cast<float4*>(ws + L.rowp);
+  float* scale = reinterpret_cast<float*>(ws + L.scale);
+  lp_row_prep_kernel<<<1, kPrepThreads, 0, s>>>(grad_logprob, grad_entropy, lse, entropy, tokens, n_tokens, vocab_size,
+                                                ignore_index, dtype == NIMBLE_DTYPE_F16, rowp, scale);
+  NIMBLE_CUDA_TRY(cudaGetLastError());
+  EpiParams eg{};
+  eg.labels = tokens;
+  eg.ignore_index = ignore_index;
+  eg.rowp = rowp;
+  eg.status = status;
+  return slab_backward<EPI_LP_GRAD>(L.slabs, ws, eg, scale, nullptr, 1.0f, hidden, weights, n_tokens, d_model, v_local,
+                                    v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
+                                    grad_weights_dtype, accumulate_grad_weights, status, s, nullptr, 0, 1.0f);
 }
 
 // ============================================ allocation-free forward variant

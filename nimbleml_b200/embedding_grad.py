@@ -6,11 +6,15 @@
   deterministically and for one vocab shard.
 * ``AdamW`` — the reference's fused AdamW update (NimbleML/optimizers/adam.py:20-43,
   85-131, 295-312) over fp32 master weights, e.g. one rank's vocab shard of E,
-  with an optional low-precision copy written in the same pass.
+  with an optional low-precision copy written in the same pass. A step
+  updates all tensors in one launch, with the moments in 32 or in 8 bits.
+* ``adamw_step_many`` — that step as a function over lists of tensors.
 """
 from __future__ import annotations
 
-from typing import Iterable, Optional
+import contextlib
+from array import array
+from typing import Iterable, NamedTuple, Optional, Sequence, Union
 
 import torch
 
@@ -46,41 +50,220 @@ def embedding_scatter_add(grad_weights: torch.Tensor, ids: torch.Tensor, grad_ou
     return grad_weights
 
 
+QUANT_BLOCK = 128  # elements that share a scale
+
+
+class QuantizedMoment(NamedTuple):
+    """An AdamW moment in 8 bits: e4m3 codes of the tensor's shape and one fp32
+    scale for each run of 128 elements. The second moment holds its root."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for the native calls when it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _check_quantized(codes: torch.Tensor, scales: torch.Tensor) -> None:
+    if codes.dtype != torch.float8_e4m3fn or not codes.is_contiguous():
+        raise ValueError("8-bit moments are contiguous float8_e4m3fn codes")
+    if (scales.dtype != torch.float32 or not scales.is_contiguous() or
+            scales.numel() != -(-codes.numel() // QUANT_BLOCK)):
+        raise ValueError(f"8-bit moments need one contiguous float32 scale per {QUANT_BLOCK} elements")
+    if not codes.is_cuda or scales.device != codes.device:
+        raise ValueError("8-bit moments live on one CUDA device")
+
+
+def quantize_moment(x: torch.Tensor, *, root: bool = False) -> QuantizedMoment:
+    """An fp32 moment in 8 bits; ``root`` for the second moment, which is held as its root."""
+    if x.dtype != torch.float32 or not x.is_cuda:
+        raise ValueError("moments are float32 CUDA tensors")
+    x = x.contiguous()
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(-(-x.numel() // QUANT_BLOCK), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        native.call("nimble_adamw_quantize", x.data_ptr(), x.numel(), int(root), codes.data_ptr(), scales.data_ptr(),
+                    _stream_ptr(x.device))
+    return QuantizedMoment(codes, scales)
+
+
+def dequantize_moment(codes: torch.Tensor, scales: torch.Tensor, *, root: bool = False) -> torch.Tensor:
+    """The fp32 values that 8-bit codes stand for (``root``: their squares, the second moment)."""
+    _check_quantized(codes, scales)
+    out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
+    with _on(codes.device):
+        native.call("nimble_adamw_dequantize", codes.data_ptr(), scales.data_ptr(), codes.numel(), int(root),
+                    out.data_ptr(), _stream_ptr(codes.device))
+    return out
+
+
+Moment = Union[torch.Tensor, QuantizedMoment]
+
+
+@torch.no_grad()
+def adamw_step_many(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]],
+                    exp_avgs: Sequence[Moment], exp_avg_sqs: Sequence[Moment], *, step: int,
+                    learning_rate: float = 0.001, beta1: float = 0.9, beta2: float = 0.999, epsilon: float = 1e-8,
+                    weight_decay: float = 0.01, copies: Optional[Sequence[Optional[torch.Tensor]]] = None) -> None:
+    """One in-place AdamW step over many tensors, in one launch for up to 400 of them.
+
+    Args:
+        params: contiguous fp32 master weights of any sizes. Two that overlap in part must
+            not be in one step; one that is listed twice is updated twice, in order.
+        grads: gradients of the same sizes (float32, float16 or bfloat16);
+            tensors whose gradient is None are left as they are.
+        exp_avgs, exp_avg_sqs: all fp32 tensors, or all 8-bit pairs (codes,
+            scales) as :class:`QuantizedMoment` describes them.
+        step: the step's number, from 1 (bias correction).
+        copies: tensors (or None) that receive the new weights in their dtype.
+
+    The update is that of the reference's AdamW (NimbleML/optimizers/adam.py:20-43).
+    With 8-bit moments the weights are updated from the new moments before
+    these are rounded. A gradient that is not finite spoils its own weight and,
+    with 8-bit moments, the block of 128 it lies in. A captured step keeps the
+    scalars it was captured with.
+    """
+    n = len(params)
+    copies = copies if copies is not None else [None] * n
+    if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(copies) == n:
+        raise ValueError("params, grads, exp_avgs, exp_avg_sqs and copies must have one entry per tensor")
+    if step < 1:
+        raise ValueError("step counts from 1")
+    eight: Optional[bool] = None
+    dev = -1
+    rows, keep, seen = array("q"), [], set()
+    dtypes = _TORCH_TO_NIMBLE
+    f32 = torch.float32
+
+    def launch() -> None:
+        if not seen:
+            return
+        device = torch.device("cuda", dev)
+        with _on(device):
+            native.call("nimble_adamw_step_many", rows.buffer_info()[0], len(seen), 8 if eight else 32, learning_rate,
+                        beta1, beta2, 1.0 - beta1 ** step, 1.0 - beta2 ** step, epsilon, weight_decay,
+                        _stream_ptr(device))
+
+    for p, g, m, v, c in zip(params, grads, exp_avgs, exp_avg_sqs, copies):
+        if g is None:
+            continue
+        size = p.numel()
+        at = p.get_device()
+        if dev < 0:
+            dev, eight = at, not isinstance(m, torch.Tensor)
+            if dev < 0:
+                raise ValueError("adamw_step_many needs CUDA tensors; there is no CPU path")
+        if p.dtype is not f32 or not p.is_contiguous():
+            raise ValueError("AdamW master weights must be contiguous float32 tensors")
+        if g.dtype not in dtypes or g.numel() != size:
+            raise ValueError(f"a gradient of {g.numel()} elements in {g.dtype} for {size} weights")
+        if not g.is_contiguous():
+            g = g.contiguous()
+            keep.append(g)
+        if at != dev or g.get_device() != dev:
+            raise ValueError("all tensors of a step must be on one device")
+        ms = vs = 0
+        if eight:
+            if isinstance(m, torch.Tensor) or isinstance(v, torch.Tensor):
+                raise ValueError("moments are all fp32 tensors or all (codes, scales) pairs")
+            (m, m_scales), (v, v_scales) = m, v
+            _check_quantized(m, m_scales)
+            _check_quantized(v, v_scales)
+            ms, vs = m_scales.data_ptr(), v_scales.data_ptr()
+        elif not isinstance(m, torch.Tensor) or not isinstance(v, torch.Tensor):
+            raise ValueError("moments are all fp32 tensors or all (codes, scales) pairs")
+        elif m.dtype is not f32 or v.dtype is not f32 or not m.is_contiguous() or not v.is_contiguous():
+            raise ValueError("fp32 moments must be contiguous float32 tensors")
+        if m.numel() != size or v.numel() != size or m.get_device() != dev or v.get_device() != dev:
+            raise ValueError("moments must have the sizes and the device of their weights")
+        c_ptr = c_dt = 0
+        if c is not None:
+            if c.dtype not in dtypes or c.numel() != size or not c.is_contiguous() or c.get_device() != dev:
+                raise ValueError("a copy must be contiguous, on the device and of the size of its weights")
+            c_ptr, c_dt = c.data_ptr(), dtypes[c.dtype]
+        if size == 0:
+            continue
+        ptr = p.data_ptr()
+        if ptr in seen:  # listed twice: its second update follows the first
+            launch()
+            rows, seen = array("q"), set()
+        seen.add(ptr)
+        # One nimble_adamw_tensor: seven pointers, the size, two 32-bit dtypes.
+        rows.extend((ptr, g.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, c_ptr, size, dtypes[g.dtype] | c_dt << 32))
+    launch()
+
+
 class AdamW:
     """AdamW over fp32 master tensors (learning_rate, beta1, beta2, epsilon, weight_decay
     as in the reference's ``AdamW``); ``copies`` optionally receive the updated
-    weights in their own dtype (e.g. the fp16 E used by the GEMMs)."""
+    weights in their own dtype (e.g. the fp16 E used by the GEMMs).
+
+    ``state_bits``: 32 keeps the moments ``m`` and ``v`` as fp32 tensors (8
+    bytes a weight), 8 as :class:`QuantizedMoment` pairs (2.06 bytes); ``v``
+    then holds the second moment's root, and ``moments()`` gives both in fp32.
+    """
 
     def __init__(self, params: Iterable[torch.Tensor], learning_rate=0.001, beta1=0.9, beta2=0.999,
-                 epsilon=1e-8, weight_decay=0.01, copies: Optional[Iterable[Optional[torch.Tensor]]] = None):
+                 epsilon=1e-8, weight_decay=0.01, copies: Optional[Iterable[Optional[torch.Tensor]]] = None,
+                 state_bits: int = 32):
         self.params = list(params)
         for p in self.params:
             if p.dtype != torch.float32 or not p.is_contiguous():
                 raise ValueError("AdamW master weights must be contiguous float32 tensors")
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8")
+        self.state_bits = int(state_bits)
         self.copies = list(copies) if copies is not None else [None] * len(self.params)
         self.lr, self.beta1, self.beta2 = float(learning_rate), float(beta1), float(beta2)
         self.epsilon, self.weight_decay = float(epsilon), float(weight_decay)
-        self.m = [torch.zeros_like(p) for p in self.params]
-        self.v = [torch.zeros_like(p) for p in self.params]
+        self.m = [self._zero_moment(p) for p in self.params]
+        self.v = [self._zero_moment(p) for p in self.params]
         self.t = 0
+
+    def _zero_moment(self, p: torch.Tensor) -> Moment:
+        if self.state_bits == 32:
+            return torch.zeros_like(p)
+        return QuantizedMoment(torch.zeros(p.shape, dtype=torch.uint8, device=p.device).view(torch.float8_e4m3fn),
+                               torch.zeros(-(-p.numel() // QUANT_BLOCK), dtype=torch.float32, device=p.device))
+
+    def moments(self):
+        """(first moments, second moments) as lists of fp32 tensors: the state itself in 32 bits, else its values."""
+        if self.state_bits == 32:
+            return self.m, self.v
+        return [dequantize_moment(*q) for q in self.m], [dequantize_moment(*q, root=True) for q in self.v]
 
     @torch.no_grad()
     def step(self):
         self.t += 1
-        bc1 = 1.0 - self.beta1 ** self.t
-        bc2 = 1.0 - self.beta2 ** self.t
-        for p, m, v, c in zip(self.params, self.m, self.v, self.copies):
-            if p.grad is None:
-                continue
-            g = p.grad.contiguous()
-            native.call("nimble_adamw_step", p.data_ptr(), g.data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
-                        v.data_ptr(), p.numel(), self.lr, self.beta1, self.beta2, bc1, bc2, self.epsilon,
-                        self.weight_decay, c.data_ptr() if c is not None else None,
-                        _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0, _stream_ptr(p.device))
+        grads = [p.grad for p in self.params]
+        if self.state_bits == 32:
+            # Tensors that are not whole eights on 16-byte boundaries keep a
+            # step of their own, whose scalar kernel rounds in another order.
+            for i, (p, g) in enumerate(zip(self.params, grads)):
+                if g is not None and not self._whole(p, g, self.m[i], self.v[i], self.copies[i]):
+                    self._step_alone(i, g.contiguous())
+                    grads[i] = None
+        adamw_step_many(self.params, grads, self.m, self.v, step=self.t, learning_rate=self.lr, beta1=self.beta1,
+                        beta2=self.beta2, epsilon=self.epsilon, weight_decay=self.weight_decay, copies=self.copies)
+
+    @staticmethod
+    def _whole(p, *others) -> bool:
+        return p.numel() % 8 == 0 and not any(t is not None and t.data_ptr() & 15 for t in (p, *others))
+
+    def _step_alone(self, i: int, g: torch.Tensor) -> None:
+        p, m, v, c = self.params[i], self.m[i], self.v[i], self.copies[i]
+        native.call("nimble_adamw_step", p.data_ptr(), g.data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
+                    v.data_ptr(), p.numel(), self.lr, self.beta1, self.beta2, 1.0 - self.beta1 ** self.t,
+                    1.0 - self.beta2 ** self.t, self.epsilon, self.weight_decay,
+                    c.data_ptr() if c is not None else None, _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0,
+                    _stream_ptr(p.device))
 
     def zero_grad(self, set_to_none: bool = True):
         for p in self.params:
             p.grad = None if set_to_none else (torch.zeros_like(p) if p.grad is None else p.grad.zero_())
 
 
-__all__ = ["embedding_scatter_add", "AdamW"]
+__all__ = ["embedding_scatter_add", "AdamW", "QuantizedMoment", "adamw_step_many", "quantize_moment",
+           "dequantize_moment"]

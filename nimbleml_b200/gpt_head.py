@@ -41,6 +41,7 @@ from nimbleml_b200.kernels.fused_tied_crossentropy import (
     native,
 )
 from nimbleml_b200.losses.cross_entropy import tied_backward_core, tied_cross_entropy, tied_forward_core
+from nimbleml_b200.losses.logprobs import TokenLogProbs, tied_token_logprobs
 from nimbleml_b200.norm import rmsnorm_backward, rmsnorm_forward
 
 
@@ -170,6 +171,13 @@ class TiedEmbedding:
         h2d = hidden.reshape(-1, d)
         y = as_label_indices(labels, batch_size=h2d.shape[0], device=hidden.device)
         return tied_cross_entropy(h2d, self.weight, y, ignore_index, **kw)
+
+    def token_logprobs(self, hidden: torch.Tensor, tokens, ignore_index: Optional[int] = None) -> TokenLogProbs:
+        """Log probability of every token and entropy of every row of the tied head
+        over ``hidden`` (..., d), 16-bit; the head's dE is added into ``grad``."""
+        return tied_token_logprobs(hidden, self.weight, tokens, ignore_index, vocab_offset=self.vocab_offset,
+                                   vocab_size=self.vocab_size, group=self.group if self.world > 1 else None,
+                                   grad_weights_buffer=self.grad)
 
     def zero_grad(self) -> None:
         self.grad.zero_()

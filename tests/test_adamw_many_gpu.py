@@ -1,0 +1,312 @@
+"""AdamW over many tensors: 32-bit moments bit for bit as the single-tensor step, 8-bit moments bit for bit as
+their definition, and both against 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [0, 1, 3, 7, 8, 127, 128, 129, 255, 1000, 8191, 8192, 8193, 20011]
+HYPER = dict(learning_rate=2e-2, beta1=0.9, beta2=0.99, epsilon=1e-8, weight_decay=0.1)
+MAX, TINY = 448.0, 2.0**-9
+
+
+def views(sizes, dtype, gap, fill=0.0):
+    """Tensors cut from one buffer, `gap` elements apart, and the buffer."""
+    at, out = gap, []
+    buf = torch.full((sum(sizes) + gap * (len(sizes) + 1),), fill, device="cuda").to(dtype)
+    for n in sizes:
+        out.append(buf[at:at + n])
+        at += n + gap
+    return out, buf
+
+
+def make(sizes, gdtype, cdtype, gap, seed):
+    g = torch.Generator().manual_seed(seed)
+    ps, pbuf = views(sizes, torch.float32, gap, 7.0)
+    gs, _ = views(sizes, gdtype, gap)
+    cs, cbuf = views(sizes, cdtype, gap, 7.0) if cdtype else ([None] * len(sizes), None)
+    for p, gr in zip(ps, gs):
+        p.copy_(torch.randn(p.shape, generator=g))
+        gr.copy_(torch.randn(gr.shape, generator=g) * 10 ** float(torch.empty(()).uniform_(-4, 0, generator=g)))
+    return ps, gs, cs, pbuf, cbuf, g
+
+
+def gaps_untouched(buf, sizes, gap):
+    keep = torch.ones(buf.numel(), dtype=torch.bool)
+    at = gap
+    for n in sizes:
+        keep[at:at + n] = False
+        at += n + gap
+    return (buf.cpu()[keep] == 7).all()
+
+
+@pytest.mark.parametrize("gdtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cdtype", [None, torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gap", [16, 1])
+def test_32_bits_as_the_single_step(gdtype, cdtype, gap):
+    from nimbleml_b200.embedding_grad import _TORCH_TO_NIMBLE, _stream_ptr, adamw_step_many, native
+
+    sizes = [16 * ((n + 15) // 16) if gap == 16 else n for n in SIZES]
+    ps, gs, cs, pbuf, cbuf, _ = make(sizes, gdtype, cdtype, gap, 5)
+    ms, vs = [torch.zeros_like(p) for p in ps], [torch.zeros_like(p) for p in ps]
+    ref = [(p.clone(), torch.zeros_like(p), torch.zeros_like(p), None if c is None else torch.zeros_like(c))
+           for p, c in zip(ps, cs)]
+    start = [p.double() for p in ps]
+    m64, v64 = [torch.zeros_like(p) for p in start], [torch.zeros_like(p) for p in start]
+    for step in (1, 2, 3):
+        adamw_step_many(ps, gs, ms, vs, step=step, copies=cs, **HYPER)
+        for (p, m, v, c), g in zip(ref, gs):
+            h = HYPER
+            native.call("nimble_adamw_step", p.data_ptr(), g.contiguous().data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
+                        v.data_ptr(), p.numel(), h["learning_rate"], h["beta1"], h["beta2"], 1 - h["beta1"]**step,
+                        1 - h["beta2"]**step, h["epsilon"], h["weight_decay"], c.data_ptr() if c is not None else None,
+                        _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0, _stream_ptr(p.device))
+        for i, g in enumerate(gs):
+            g64 = g.double()
+            m64[i] = 0.9 * m64[i] + 0.1 * g64
+            v64[i] = 0.99 * v64[i] + 0.01 * g64 * g64
+            start[i] = start[i] * (1 - 2e-3) - 2e-2 * (m64[i] / (1 - 0.9**step)) / ((v64[i] / (1 - 0.99**step)).sqrt() + 1e-8)
+    for p, m, v, c, (rp, rm, rv, rc), w64 in zip(ps, ms, vs, cs, ref, start):
+        if gap == 16:  # whole eights on 16-byte boundaries: the single step's vector kernel
+            assert p.equal(rp) and m.equal(rm) and v.equal(rv)
+            assert c is None or c.equal(rc)
+        else:  # its scalar kernel rounds a moment's two products in another order
+            assert c is None or c.equal(p.to(c.dtype))
+        # Three steps of about 12 roundings each: 40 2^-24 of the weight and of the steps taken (< 0.1).
+        assert ((p.double() - w64).abs() <= 40 * 2.0**-24 * (w64.abs() + 0.2)).all()
+    assert gaps_untouched(pbuf, sizes, gap)
+    assert cbuf is None or gaps_untouched(cbuf, sizes, gap)
+
+
+# The definition of the 8-bit step in fp32 operations, each rounded on its own.
+def encode(x, root):
+    n = x.numel()
+    b = torch.zeros(-(-n // 128) * 128)
+    b[:n] = x
+    b = b.view(-1, 128)
+    top = b.abs().amax(1, keepdim=True)
+    live = top >= 2.0**-100
+    up = torch.where(live, torch.div(torch.full_like(top, MAX), top), torch.zeros_like(top))
+    y = b * up
+    if root:
+        y = torch.where((b > 0) & (y < TINY), torch.full_like(y, TINY), y)
+    scale = torch.where(live, top * (1.0 / MAX), torch.zeros_like(top))
+    return y.clamp(-MAX, MAX).to(torch.float8_e4m3fn).flatten()[:n], scale.flatten()
+
+
+def decode(codes, scales):
+    n = codes.numel()
+    return codes.float() * scales.repeat_interleave(128)[:n]
+
+
+def step8(w, g, mq, vq, step, h):
+    f = torch.float32
+    sc = {k: torch.tensor(v, dtype=torch.float64).to(f) for k, v in dict(
+        b1=h["beta1"], omb1=1 - h["beta1"], b2=h["beta2"], omb2=1 - h["beta2"],
+        decay=1 - h["learning_rate"] * h["weight_decay"], c1=h["learning_rate"] / (1 - h["beta1"]**step),
+        c2=1 / math.sqrt(1 - h["beta2"]**step), eps=h["epsilon"]).items()}
+    m, r = decode(*mq), decode(*vq)
+    m = m * sc["b1"] + g * sc["omb1"]
+    r = ((r * r) * sc["b2"] + (g * g) * sc["omb2"]).sqrt()
+    w = w * sc["decay"] - (m * sc["c1"]) / (r * sc["c2"] + sc["eps"])
+    return w, encode(m, False), encode(r, True)
+
+
+def same_codes(a, b):
+    return a.view(torch.uint8).equal(b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("gdtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("cdtype", [None, torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gap", [16, 1])
+def test_8_bits_as_defined(gdtype, cdtype, gap):
+    from nimbleml_b200.embedding_grad import QuantizedMoment, adamw_step_many, dequantize_moment
+
+    sizes = [16 * ((n + 15) // 16) if gap == 16 else n for n in SIZES]
+    ps, gs, cs, pbuf, cbuf, g = make(sizes, gdtype, cdtype, gap, 6)
+    cut, codebuf = views(sizes, torch.float32, gap)
+    code = [torch.zeros(codebuf.numel(), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2)]
+    place, at = [], gap
+    for n in sizes:
+        place.append(slice(at, at + n))
+        at += n + gap
+    blocks = [-(-n // 128) for n in sizes]
+    ms = [QuantizedMoment(code[0][s], torch.zeros(b, device="cuda")) for s, b in zip(place, blocks)]
+    vs = [QuantizedMoment(code[1][s], torch.zeros(b, device="cuda")) for s, b in zip(place, blocks)]
+    ref = [(p.cpu(), (m.codes.cpu(), m.scales.cpu()), (v.codes.cpu(), v.scales.cpu())) for p, m, v in zip(ps, ms, vs)]
+    for step in (1, 2, 3, 4):
+        for gr in gs:  # small entries, and some that are zero
+            gr.mul_(torch.rand(gr.shape, generator=g).cuda().round() * 0.7)
+        adamw_step_many(ps, gs, ms, vs, step=step, copies=cs, **HYPER)
+        ref = [step8(w, gr.float().cpu(), m, v, step, HYPER) for (w, m, v), gr in zip(ref, gs)]
+        for p, m, v, c, (w, rm, rv) in zip(ps, ms, vs, cs, ref):
+            assert same_codes(m.codes.cpu(), rm[0]) and m.scales.cpu().equal(rm[1])
+            assert same_codes(v.codes.cpu(), rv[0]) and v.scales.cpu().equal(rv[1])
+            assert p.cpu().equal(w)
+            assert c is None or c.cpu().equal(w.to(c.dtype))
+            assert dequantize_moment(*m).cpu().equal(decode(*rm))
+            assert dequantize_moment(*v, root=True).cpu().equal(decode(*rv) * decode(*rv))
+    assert gaps_untouched(pbuf, sizes, gap)
+    assert cbuf is None or gaps_untouched(cbuf, sizes, gap)
+    inside = torch.zeros(code[0].numel(), dtype=torch.bool)
+    for s in place:
+        inside[s] = True
+    for c in code:
+        assert (c.view(torch.uint8).cpu()[~inside] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 127, 128, 129, 5000])
+def test_quantised_values(n):
+    """A code is off by at most half a step of e4m3, 2^-4 of the value, or 2^-10 of the block's scale below 2^-6 of
+    it; a positive root never becomes zero; blocks of zeros stay zeros."""
+    from nimbleml_b200.embedding_grad import dequantize_moment, quantize_moment
+
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, generator=g) * torch.exp(4 * torch.randn(n, generator=g))
+    x[: n // 3] = 0.0
+    q = quantize_moment(x.cuda())
+    assert same_codes(q.codes.cpu(), encode(x, False)[0])
+    back = dequantize_moment(*q).cpu()
+    scale = q.scales.cpu().repeat_interleave(128)[:n]
+    assert ((back - x).abs() <= torch.maximum(x.abs() * 2.0**-4, scale * 2.0**-10) * (1 + 2.0**-20)).all()
+    v = x.abs()
+    q = quantize_moment(v.cuda(), root=True)
+    r = dequantize_moment(*q).cpu()
+    assert (r[v > 0] > 0).all() and (r[v == 0] == 0).all()
+    z = quantize_moment(torch.zeros(n, device="cuda"))
+    assert (dequantize_moment(*z) == 0).all() and (z.scales == 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_many_tensors_none_and_twice(bits):
+    """Over 400 tensors go in two launches; None leaves a tensor; one listed twice is updated twice in order."""
+    from nimbleml_b200.embedding_grad import AdamW
+
+    ps = [torch.full((5 + i % 3,), 1.0 + i, device="cuda") for i in range(405)]
+    opt = AdamW(ps, learning_rate=0.5, state_bits=bits)
+    for i, p in enumerate(ps):
+        p.grad = None if i == 403 else torch.full_like(p, 0.25)
+    before = ps[403].clone()
+    opt.step()
+    assert ps[403].equal(before)
+    lone = AdamW([torch.full((5,), 1.0, device="cuda")], learning_rate=0.5, state_bits=bits)
+    lone.params[0].grad = torch.full((5,), 0.25, device="cuda")
+    lone.step()
+    assert ps[0].equal(lone.params[0])
+    assert all(torch.isfinite(p).all() for p in ps) and not ps[404].eq(405.0).any()
+    p = torch.ones(300, device="cuda")
+    p.grad = torch.ones(300, device="cuda")
+    twice = AdamW([p, p], state_bits=bits, learning_rate=0.1, weight_decay=0.0)
+    twice.step()
+    # m / (sqrt v + eps) is 1 in each of the two updates, to the rounding of the 8-bit path's 1 / 448 scales.
+    assert ((p - 0.8).abs() <= 1e-6).all()
+    m, v = twice.moments()
+    assert ((m[0] - 0.1).abs() <= 0.1 * 2.0**-4).all() and ((v[0] - 0.001).abs() <= 0.001 * 2.0**-2).all()
+
+
+def test_8_bit_root_follows_its_gradients():
+    """With a constant gradient the root of the second moment decays and grows as the exact one (block scales)."""
+    from nimbleml_b200.embedding_grad import AdamW
+
+    p = torch.zeros(256, device="cuda")
+    opt = AdamW([p], learning_rate=1e-3, beta2=0.99, state_bits=8)
+    want = 0.0
+    for size, steps in ((1.0, 50), (1e-3, 200)):
+        for _ in range(steps):
+            p.grad = torch.full((256,), size, device="cuda")
+            opt.step()
+            want = 0.99 * want + 0.01 * size * size
+        v = opt.moments()[1][0]
+        # Equal elements share the block's maximum: 448 exactly, so only fp32 roundings add up (steps x 8).
+        assert ((v.double() / want - 1).abs() <= 250 * 8 * 2.0**-24).all()
+
+
+def test_non_finite_gradients_stay_in_their_block():
+    from nimbleml_b200.embedding_grad import AdamW
+
+    for bits in (32, 8):
+        p, q = torch.ones(512, device="cuda"), torch.ones(512, device="cuda")
+        opt = AdamW([p, q], state_bits=bits)
+        p.grad, q.grad = torch.full((512,), 0.5, device="cuda"), torch.full((512,), 0.5, device="cuda")
+        p.grad[200] = torch.nan
+        opt.step()
+        p.grad[200] = 0.5
+        opt.step()
+        bad = torch.isnan(p)
+        assert bad[200] and not bad[:128].any() and not bad[256:].any() and not torch.isnan(q).any()
+        if bits == 32:
+            assert int(bad.sum()) == 1
+
+
+def test_optimizer_step_keeps_the_bits_of_single_steps():
+    """AdamW.step equals a loop of nimble_adamw_step over its tensors bit for bit, odd sizes and offsets included."""
+    from nimbleml_b200.embedding_grad import _TORCH_TO_NIMBLE, AdamW, _stream_ptr, native
+
+    for cdtype in (None, torch.float16, torch.bfloat16):
+        for gap in (16, 1):
+            ps, gs, cs, _, _, _ = make(SIZES[1:], torch.bfloat16, cdtype, gap, 3)
+            ps2, _, cs2, _, _, _ = make(SIZES[1:], torch.bfloat16, cdtype, gap, 3)
+            ref = [(p, torch.zeros_like(p), torch.zeros_like(p), c) for p, c in zip(ps2, cs2)]
+            opt = AdamW(ps, learning_rate=1e-2, copies=cs)
+            for step in (1, 2):
+                for p, g in zip(ps, gs):
+                    p.grad = g.float() if step == 1 else g.float() * 0.3
+                opt.step()
+                for (p, m, v, c), q in zip(ref, ps):
+                    native.call("nimble_adamw_step", p.data_ptr(), q.grad.data_ptr(), _TORCH_TO_NIMBLE[q.grad.dtype],
+                                m.data_ptr(), v.data_ptr(), p.numel(), 1e-2, 0.9, 0.999, 1 - 0.9**step,
+                                1 - 0.999**step, 1e-8, 0.01, c.data_ptr() if c is not None else None,
+                                _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0, _stream_ptr(p.device))
+            for (p, m, v, c), q, mm, vv, cc in zip(ref, ps, opt.m, opt.v, cs):
+                assert p.equal(q) and m.equal(mm) and v.equal(vv) and (c is None or c.equal(cc))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_and_on_another_stream(bits):
+    from nimbleml_b200.embedding_grad import adamw_step_many, quantize_moment
+
+    sizes = [300, 9000]
+    ps, gs, cs, _, _, _ = make(sizes, torch.float16, torch.bfloat16, 1, 9)
+
+    def state():
+        p = [x.clone() for x in ps]
+        z = [torch.zeros_like(x) for x in ps]
+        if bits == 8:
+            return p, [quantize_moment(x) for x in z], [quantize_moment(x) for x in z]
+        return p, z, [x.clone() for x in z]
+
+    a, b = state(), state()
+    for _ in range(2):
+        adamw_step_many(a[0], gs, a[1], a[2], step=7, **HYPER)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adamw_step_many(b[0], gs, b[1], b[2], step=7, **HYPER)
+    graph.replay()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    for x, y in zip(a[0], b[0]):
+        assert x.equal(y)
+
+
+def test_gradients_with_strides():
+    from nimbleml_b200.embedding_grad import adamw_step_many
+
+    w = torch.ones(64, 48, device="cuda")
+    g = torch.randn(48, 64, device="cuda").t()
+    one = [x.clone() for x in (w, torch.zeros_like(w), torch.zeros_like(w))]
+    two = [x.clone() for x in one]
+    adamw_step_many([one[0]], [g], [one[1]], [one[2]], step=1)
+    adamw_step_many([two[0]], [g.contiguous()], [two[1]], [two[2]], step=1)
+    assert one[0].equal(two[0])
+    with pytest.raises(ValueError, match="contiguous float32"):
+        adamw_step_many([w.t()], [g], [one[1]], [one[2]], step=1)
+    with pytest.raises(ValueError, match="elements"):
+        adamw_step_many([w], [g[:3]], [one[1]], [one[2]], step=1)
+    with pytest.raises(ValueError, match="moments"):
+        adamw_step_many([w], [g], [one[1]], [one[2][:3]], step=1)

@@ -1,0 +1,494 @@
+"""Token log probabilities over logits and from the tied matrix, against 64-bit definitions.
+
+Tolerances are bounds, element by element, with u = 2^-24. Let d = x - m (m the row's
+max), D1 = sum p |d| and D2 = sum p d^2. An exponential is off by 2^-22 of itself and by
+2 u |d| from its argument; a lane adds at most n = V / 256 + 48 terms in a row (the rest
+is a tree), each addition off by u of the sum. So the sum is off by
+e_s = n u + 2^-22 + 2 u D1 relative, ln s by e_s + u |ln s|; a log probability by that and
+u (|x - m| + |logp|); the entropy ln s - sum(2^d d) / s by e_s + (n u + 2^-22 + e_s) D1 +
+2 u D2 and roundings of its two terms (``row_bounds``).
+"""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+HALF = [torch.float16, torch.bfloat16]
+IGN = -100
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def exact_rows(x, tokens):
+    """(logp, entropy, p, logq, d) in 64 bits; a row of -inf only: -inf, 0, 0, -inf, 0.
+
+    log p is (x - m) - ln sum exp(x - m): next to an m of -3.4e38 even 64 bits lose the logarithm."""
+    x = x.double()
+    m = x.amax(1, keepdim=True)
+    d = x - torch.where(torch.isneginf(m), torch.zeros_like(m), m)
+    total = d.exp().sum(1, keepdim=True)
+    logq = torch.where(total > 0, d - total.log(), torch.full_like(d, -torch.inf))
+    p = logq.exp()
+    h = -(p * torch.where(p > 0, logq, torch.zeros_like(logq))).sum(1)
+    return logq.gather(1, tokens.clamp(min=0).unsqueeze(1)).squeeze(1), h, p, logq, torch.where(p > 0, d, torch.zeros_like(d))
+
+
+def row_bounds(p, d, h):
+    """(of the sum's logarithm, of the entropy), each (rows,)."""
+    u, v = 2.0**-24, p.shape[1]
+    d1, d2 = (p * d.abs()).sum(1), (p * d * d).sum(1)
+    n = v / 256 + 48
+    e_s = n * u + 2.0**-22 + 2 * u * d1
+    ls = h + d1  # ln s = H + ln 2 u / s
+    return e_s + u * ls, e_s + u * ls + (n * u + 2.0**-22 + e_s) * d1 + 2 * u * d2 + 2 * u * (ls + d1 + h)
+
+
+def make_logits(rows, v, dtype, seed, scale=2.5, pitch=None, offset=0):
+    g = torch.Generator().manual_seed(seed)
+    pitch = pitch or v
+    flat = torch.zeros(rows * pitch + offset + 16, dtype=dtype, device="cuda")
+    view = flat[offset:offset + rows * pitch].view(rows, pitch)[:, :v]
+    view.copy_((torch.randn(rows, v, generator=g) * scale).to(dtype))
+    tokens = torch.randint(0, v, (rows,), generator=g).cuda()
+    return view, tokens, g
+
+
+def check_rows(r, x, tokens, ignored=None):
+    lp, h, p, logq, d = exact_rows(x, tokens)
+    t_ls, t_h = row_bounds(p, d, h)
+    used = tokens != IGN
+    assert torch.isneginf(r.logprobs[used]).equal(torch.isneginf(lp[used]))
+    fin = used & torch.isfinite(lp)
+    # x - m and the result are rounded: 2^-24 of each, |x - m| <= |logp| + ln s.
+    tol = t_ls + 2.0**-24 * (2 * lp.abs() + h + (p * d.abs()).sum(1))
+    assert ((r.logprobs.double() - lp).abs() <= tol)[fin].all()
+    assert ((r.entropy.double() - h).abs() <= t_h)[used].all()
+    assert (r.logprobs[~used] == 0).all() and (r.entropy[~used] == 0).all()
+    if r.top_ids is not None:
+        k = r.top_ids.shape[1]
+        ids = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :k]
+        assert r.top_ids[used].equal(ids[used])
+        want = logq.gather(1, ids)
+        off = (r.top_logprobs.double() - want).abs()
+        same = torch.isneginf(want) & torch.isneginf(r.top_logprobs)
+        tol = t_ls.unsqueeze(1) + 2.0**-24 * (2 * want.abs() + (h + (p * d.abs()).sum(1)).unsqueeze(1))
+        assert (same | (off <= tol))[used].all()
+        assert (r.top_ids[~used] == -1).all() and torch.isneginf(r.top_logprobs[~used]).all()
+
+
+def check_grad(got, x, tokens, a, b):
+    """Rounded once, from a p off by the sum's error, 2^-22 and 4 u (|x - m| + ln s) relative."""
+    _, h, p, logq, d = exact_rows(x, tokens)
+    zero = torch.zeros_like(p)
+    lq = torch.where(p > 0, logq, zero)
+    a, b = a.double().unsqueeze(1), b.double().unsqueeze(1)
+    onehot = zero.scatter(1, tokens.clamp(min=0).unsqueeze(1), 1.0)
+    dead = (tokens == IGN).unsqueeze(1) | torch.isneginf(x).all(1, keepdim=True)
+    want = torch.where(dead, zero, a * onehot - p * (a + b * (h.unsqueeze(1) + lq)))
+    t_ls, t_h = (t.unsqueeze(1) for t in row_bounds(p, d, h))
+    h = h.unsqueeze(1)
+    e_lp = t_ls + 2.0**-22 * (d.abs() + lq.abs())  # of log p
+    coef = a.abs() + b.abs() * (h + lq.abs())
+    slack = p * (coef * (e_lp + 2.0**-21) + b.abs() * (t_h + e_lp))
+    fin = torch.finfo(got.dtype)
+    tol = half_step(got.dtype) * want.abs() + (1 + 2.0**-7) * slack + 2.0**-23 * a.abs() * onehot
+    assert ((got.double() - want).abs() <= tol * (1 + 2.0**-7) + fin.smallest_normal * fin.eps).all()
+    assert (got[dead.squeeze(1)] == 0).all()
+
+
+SHAPES = [(1, 1), (3, 2), (2, 7), (5, 100), (33, 1001), (4, 2047), (3, 2304), (300, 4099), (6, 50257), (2, 128259),
+          (700, 8200)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rows_and_gradient(dtype, shape):
+    from nimbleml_b200.losses import token_logprobs
+
+    rows, v = shape
+    x, tokens, g = make_logits(rows, v, dtype, rows * 31 + v)
+    if rows > 2:
+        tokens[2::5] = IGN
+    a, b = torch.randn(rows, generator=g).cuda(), torch.randn(rows, generator=g).cuda()
+    for k in sorted({0, 1, min(5, v), min(64, v)}):
+        leaf = x.detach().requires_grad_()
+        r = token_logprobs(leaf, tokens, IGN, top_k=k)
+        check_rows(r, x, tokens)
+        (gx,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (a, b))
+        check_grad(gx, x, tokens, a, b)
+    # One gradient alone; the same call gives the same bits.
+    leaf = x.detach().requires_grad_()
+    r2 = token_logprobs(leaf, tokens, IGN)
+    (g1,) = torch.autograd.grad(r2.entropy, leaf, b, retain_graph=True)
+    check_grad(g1, x, tokens, torch.zeros_like(a), b)
+    (g2,) = torch.autograd.grad(r2.logprobs, leaf, a)
+    check_grad(g2, x, tokens, a, torch.zeros_like(b))
+    assert r2.logprobs.equal(r.logprobs) and r2.entropy.equal(r.entropy)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["pitch", "offset", "odd_pitch", "transposed", "broadcast", "three_d"])
+def test_strides(dtype, layout):
+    from nimbleml_b200.losses import token_logprobs
+
+    rows, v = 12, 1003
+    es = torch.empty(0, dtype=dtype).element_size()
+    if layout == "pitch":
+        x, tokens, g = make_logits(rows, v, dtype, 1, pitch=1008)
+    elif layout == "offset":
+        x, tokens, g = make_logits(rows, v, dtype, 2, pitch=1008, offset=3)
+    elif layout == "odd_pitch":
+        x, tokens, g = make_logits(rows, v, dtype, 3, pitch=1037, offset=1)
+    elif layout == "transposed":
+        x, tokens, g = make_logits(v, rows, dtype, 4)
+        x, tokens = x.t(), torch.arange(rows, device="cuda")
+    elif layout == "broadcast":
+        x, tokens, g = make_logits(1, v, dtype, 5)
+        x, tokens = x.expand(rows, v), torch.arange(rows, device="cuda")
+    else:
+        x, tokens, g = make_logits(rows, v, dtype, 6, pitch=1000 + 16 // es)
+        x3, t3 = x.view(3, 4, v), tokens.view(3, 4)
+        r = token_logprobs(x3, t3, top_k=3)
+        assert r.logprobs.shape == (3, 4) and r.top_ids.shape == (3, 4, 3)
+    a, b = torch.randn(rows, generator=g).cuda(), torch.randn(rows, generator=g).cuda()
+    leaf = x.detach().requires_grad_()
+    r = token_logprobs(leaf, tokens, top_k=7)
+    check_rows(r, x, tokens)
+    (gx,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (a, b))
+    check_grad(gx, x, tokens, a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,v", [(3, 300), (2, 9000), (400, 9000)])
+def test_masks_ties_and_orders(dtype, rows, v):
+    """-inf masks, a row of -inf only, the type's lowest value, ties, and rows that rise or fall to their end."""
+    from nimbleml_b200.losses import token_logprobs
+
+    kinds = {}
+    x, tokens, g = make_logits(rows, v, dtype, v + rows)
+    low = torch.finfo(dtype).min
+    masked = x.clone()
+    masked[:, torch.rand(v, generator=g).cuda() < 0.5] = -torch.inf
+    masked[0] = -torch.inf
+    masked[1] = -torch.inf
+    masked[1, v - 2] = 1.5
+    kinds["masked"] = masked
+    lowest = x.clone()
+    lowest[:, ::2] = low
+    lowest[0] = low
+    kinds["lowest"] = lowest
+    kinds["constant"] = torch.zeros_like(x)
+    ties = (x * 1.0).round()
+    ties[:, 5] = -0.0
+    kinds["ties"] = ties
+    kinds["rising"] = x.sort(dim=1).values
+    kinds["falling"] = x.sort(dim=1, descending=True).values
+    # Strictly rising bits, so that every logit beats all before it.
+    step = torch.arange(v, device="cuda", dtype=torch.float64)
+    kinds["ramp"] = (step / v * 8 - 4).to(dtype).expand(rows, v).contiguous()
+    a, b = torch.randn(rows, generator=g).cuda(), torch.randn(rows, generator=g).cuda()
+    for name, y in kinds.items():
+        leaf = y.detach().requires_grad_()
+        r = token_logprobs(leaf, tokens, top_k=min(64, v))
+        check_rows(r, y, tokens)
+        (gx,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (a, b))
+        check_grad(gx, y, tokens, a, b)
+
+
+def test_nan_inf_ignored_and_bad_tokens():
+    from nimbleml_b200.kernels.fused_tied_crossentropy import check_status
+    from nimbleml_b200.losses import token_logprobs
+
+    x, tokens, _ = make_logits(6, 5000, torch.float32, 9)
+    x[0] = torch.nan  # ignored: not read
+    tokens[0] = IGN
+    x[1, 17] = torch.inf
+    x[2, 4999] = torch.nan
+    x[3, :4000] = -torch.inf
+    x[3, 4500] = torch.nan
+    leaf = x.detach().requires_grad_()
+    r = token_logprobs(leaf, tokens, IGN, top_k=5)
+    assert r.logprobs[0] == 0 and r.entropy[0] == 0
+    assert torch.isnan(r.logprobs[1:4]).all() and torch.isnan(r.entropy[1:4]).all()
+    assert torch.isfinite(r.logprobs[4:]).all()
+    assert r.top_ids[1, 0] == 17
+    (gx,) = torch.autograd.grad(r.logprobs.sum(), leaf)
+    assert (gx[0] == 0).all() and torch.isfinite(gx[4:]).all()
+    check_status(x.device)
+    tokens[5] = 5000
+    leaf = x.detach().requires_grad_()
+    r = token_logprobs(leaf, tokens, IGN)
+    assert torch.isnan(r.logprobs[5]) and torch.isfinite(r.logprobs[4])
+    (gx,) = torch.autograd.grad(r.logprobs[4:].sum(), leaf)
+    assert (gx[5] == 0).all()
+    with pytest.raises(ValueError):
+        check_status(x.device)
+    # No rows at all.
+    r = token_logprobs(x[:0], tokens[:0], top_k=3)
+    assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
+
+
+def test_gradient_against_differences():
+    """Central differences of the log probability and the entropy in x: off by h^2 / 6 |f'''| <= h^2 and by the values' own
+    error (below 2e-6 for these rows) over h."""
+    from nimbleml_b200.losses import token_logprobs
+
+    x, tokens, g = make_logits(2, 19, torch.float32, 11, scale=1.0)
+    a, b = torch.tensor([0.7, -1.1]).cuda(), torch.tensor([0.4, 0.9]).cuda()
+    leaf = x.detach().requires_grad_()
+    r = token_logprobs(leaf, tokens)
+    (gx,) = torch.autograd.grad((r.logprobs, r.entropy), leaf, (a, b))
+    h = 2.0**-6
+    for j in range(19):
+        f = []
+        for s in (1, -1):
+            y = x.clone()
+            y[:, j] += s * h
+            q = token_logprobs(y, tokens)
+            f.append((a * q.logprobs + b * q.entropy).double())
+        num = (f[0] - f[1]) / (2 * h)
+        assert ((num - gx[:, j].double()).abs() <= 2 * h * h * 2 + 4e-6 / h).all()
+
+
+def test_refusals_on_the_gpu():
+    from nimbleml_b200.losses import tied_token_logprobs, token_logprobs
+
+    x, tokens, _ = make_logits(3, 70, torch.float32, 1)
+    for k in (-1, 65, 71):
+        with pytest.raises(ValueError, match="top_k"):
+            token_logprobs(x, tokens, top_k=k)
+    with pytest.raises(ValueError, match="label count"):
+        token_logprobs(x, tokens[:2])
+    with pytest.raises(ValueError, match="dtype"):
+        token_logprobs(x.double(), tokens)
+    h, w = torch.zeros(3, 16, device="cuda").half(), torch.zeros(5, 16, device="cuda").half()
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        tied_token_logprobs(h.float(), w, tokens)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        tied_token_logprobs(h[:, :12], w[:, :12], tokens)
+    with pytest.raises(ValueError, match="d_model"):
+        tied_token_logprobs(h, w[:, :8], tokens)
+    with pytest.raises(ValueError, match="inside the vocabulary"):
+        tied_token_logprobs(h, w, tokens, vocab_offset=3, vocab_size=7)
+    with pytest.raises(ValueError, match="grad_weights_buffer"):
+        tied_token_logprobs(h, w, tokens, grad_weights_buffer=torch.zeros(5, 16).half().cuda())
+
+
+# ------------------------------------------------------------------- the tied form
+def make_tied(n, d, v, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, d, generator=g).to(dtype).cuda()
+    w = (torch.randn(v, d, generator=g) / d**0.5).to(dtype).cuda()
+    tokens = torch.randint(0, v, (n,), generator=g).cuda()
+    return h, w, tokens, g
+
+
+def logit_error(h, w):
+    """The logits are fp32 sums of d products: off by at most d 2^-23 of the sum of magnitudes, in any order."""
+    return (h.double().abs() @ w.double().abs().t()).amax(1) * (h.shape[1] + 16) * 2.0**-23
+
+
+def check_tied(r, h, w, tokens):
+    used = tokens != IGN
+    x = h.double() @ w.double().t()
+    mag = logit_error(h, w)
+    lp, ent, p, logq, d = exact_rows(x, tokens)
+    t_ls, t_h = row_bounds(p, d, ent)
+    # The epilogue's d is x log2 e - m log2 e: 2^-23 of the logits' size more.
+    big = 2.0**-22 * x.abs().amax(1)
+    assert ((r.logprobs.double() - lp).abs() <= t_ls + 2 * mag + 2 * big + 2.0**-23 * lp.abs())[used].all()
+    spread = (p * (logq.abs() + ent.unsqueeze(1))).sum(1)  # |dH / dx| summed
+    assert ((r.entropy.double() - ent).abs() <= t_h + 2 * (mag + big) * (1 + spread))[used].all()
+
+
+def check_tied_grads(gh, gw, h, w, tokens, a, b, base=None):
+    """G is rounded to 16 bits once (fp16: scaled by a power of two so that its largest bound lies in (2^14, 2^15], its
+    smallest step is then at most 2^-24 2^-14 of that bound), then summed in fp32 and rounded to the result's type."""
+    x = h.double() @ w.double().t()
+    _, ent, p, logq, d = exact_rows(x, tokens)
+    live = (tokens != IGN).unsqueeze(1)
+    a, b = a.double().unsqueeze(1), b.double().unsqueeze(1)
+    zero = torch.zeros_like(p)
+    onehot = zero.scatter(1, tokens.clamp(min=0).unsqueeze(1), 1.0)
+    t_ls, t_h = (t.unsqueeze(1) for t in row_bounds(p, d, ent))
+    ent = ent.unsqueeze(1)
+    big_g = torch.where(live, a * onehot - p * (a + b * (ent + logq)), zero)
+    mag = logit_error(h, w).unsqueeze(1) + 2.0**-22 * x.abs().amax(1, keepdim=True)
+    e_lp = t_ls + 4 * mag + 2.0**-22 * (d.abs() + logq.abs())
+    spread = (p * (logq.abs() + ent)).sum(1, keepdim=True)
+    slack = p * ((a.abs() + b.abs() * (ent + logq.abs())) * (e_lp + 2.0**-21) + b.abs() * (t_h + 2 * mag * (1 + spread) + e_lp))
+    under = 0.0
+    if h.dtype == torch.float16:
+        under = 2.0**-24 * 2.0**-14 * torch.where(live, a.abs() + b.abs() * (ent + 0.37), zero[:, :1]).amax()
+    err = torch.where(live, half_step(h.dtype) * big_g.abs() + (1 + 2.0**-6) * slack + under + 2.0**-22 * a.abs() * onehot, zero)
+    for got, g, other, e in ((gh, big_g, w.double(), err), (gw, big_g.t(), h.double(), err.t())):
+        if got is None:
+            continue
+        want = g @ other
+        if got is gw and base is not None:
+            want = want + base.double()
+        fin = torch.finfo(got.dtype)
+        tol = half_step(got.dtype) * want.abs() + e @ other.abs() + (g.shape[1] + 16) * 2.0**-23 * (g.abs() @ other.abs())
+        off = (got.double() - want).abs()
+        assert (off <= tol * (1 + 2.0**-6) + fin.smallest_normal * fin.eps).all(), float((off / (tol + 1e-300)).max())
+
+
+TIED = [(1, 8, 1), (1, 8, 3), (2, 64, 5), (7, 64, 257), (129, 136, 1000), (300, 72, 5003), (513, 256, 256), (1, 1024, 20011)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape", TIED)
+def test_tied(dtype, shape):
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    n, d, v = shape
+    h, w, tokens, g = make_tied(n, d, v, dtype, n * 7 + v)
+    if n > 2:
+        tokens[1::4] = IGN
+    a, b = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    hl, wl = h.requires_grad_(), w.requires_grad_()
+    r = tied_token_logprobs(hl, wl, tokens, IGN)
+    check_tied(r, h.detach(), w.detach(), tokens)
+    assert (r.logprobs[tokens == IGN] == 0).all() and (r.entropy[tokens == IGN] == 0).all()
+    gh, gw = torch.autograd.grad((r.logprobs, r.entropy), (hl, wl), (a, b), retain_graph=True)
+    check_tied_grads(gh, gw, h.detach(), w.detach(), tokens, a, b)
+    assert (gh[tokens == IGN] == 0).all()
+    # The same again, bit for bit, and each gradient alone.
+    gh2, gw2 = torch.autograd.grad((r.logprobs, r.entropy), (hl, wl), (a, b), retain_graph=True)
+    assert gh2.equal(gh) and gw2.equal(gw)
+    (gh3,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), (a, b), retain_graph=True)
+    assert gh3.equal(gh)
+    (gh4,) = torch.autograd.grad(r.entropy, (hl,), b, retain_graph=True)
+    check_tied_grads(gh4, None, h.detach(), w.detach(), tokens, torch.zeros_like(a), b)
+    (gw4,) = torch.autograd.grad(r.logprobs, (wl,), a)
+    check_tied_grads(None, gw4, h.detach(), w.detach(), tokens, a, torch.zeros_like(b))
+
+
+@pytest.mark.parametrize("size", [1e-12, 1e-6, 1.0, 1e6])
+def test_tied_fp16_upstream_sizes(size):
+    """Upstream gradients of any size keep the 16-bit G in range; the fp32 weight grad shows it."""
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    h, w, tokens, g = make_tied(64, 64, 3001, torch.float16, 3)
+    a, b = (size * torch.randn(64, generator=g)).cuda(), (size * torch.randn(64, generator=g)).cuda()
+    w32 = w.float().requires_grad_()
+    r = tied_token_logprobs(h, w32, tokens)
+    (gw,) = torch.autograd.grad((r.logprobs, r.entropy), (w32,), (a, b))
+    assert gw.dtype == torch.float32
+    check_tied_grads(None, gw, h, w, tokens, a, b)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_tied_slabs_buffer_and_layouts(dtype, monkeypatch):
+    from nimbleml_b200.losses import tied_token_logprobs
+    import nimbleml_b200.losses.logprobs as mod
+
+    monkeypatch.setattr(mod, "SLAB_BYTES", 1)  # 256 columns a slab
+    h, w, tokens, g = make_tied(70, 64, 1500, dtype, 21)
+    a, b = torch.randn(70, generator=g).cuda(), torch.randn(70, generator=g).cuda()
+    buf = torch.randn(1500, 64, generator=g).cuda()
+    base = buf.clone()
+    # Hidden rows in (7, 10) with a storage offset off the 16-byte grid.
+    store = torch.zeros(70 * 64 + 1, dtype=dtype, device="cuda")
+    hv = store[1:].view(7, 10, 64)
+    hv.copy_(h.view(7, 10, 64))
+    hl = hv.detach().requires_grad_()
+    r = tied_token_logprobs(hl, w, tokens.view(7, 10), grad_weights_buffer=buf)
+    assert r.logprobs.shape == (7, 10)
+    (gh,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), (a.view(7, 10), b.view(7, 10)))
+    check_tied_grads(gh.view(70, 64), buf, h, w, tokens, a, b, base=base)
+
+
+def test_tied_shards_and_all_ignored():
+    """Two vocabulary shards merge into the whole; partial hidden grads add up."""
+    import nimbleml_b200.losses.logprobs as mod
+
+    h, w, tokens, g = make_tied(50, 64, 1001, torch.bfloat16, 5)
+    tokens[7] = IGN
+    cut = 600
+    s0 = mod.shard_logprob_stats(h, w[:cut].contiguous(), tokens, 0)
+    s1 = mod.shard_logprob_stats(h, w[cut:].contiguous(), tokens, cut)
+    lp, ent, lse = mod.combine_logprob_stats(torch.stack([s0, s1]), tokens, 1001, IGN)
+    check_tied(mod.TokenLogProbs(lp, ent), h, w, tokens)
+    a, b = torch.randn(50, generator=g).cuda(), torch.randn(50, generator=g).cuda()
+    parts, rows = [], []
+    for lo, hi in ((0, cut), (cut, 1001)):
+        gh = torch.empty(50, 64, device="cuda")
+        gw = torch.empty(hi - lo, 64, dtype=torch.bfloat16, device="cuda")
+        mod.shard_logprob_backward(a, b, h, w[lo:hi].contiguous(), tokens, lse, ent, vocab_offset=lo, vocab_size=1001,
+                                   ignore_index=IGN, grad_hidden=gh, grad_weights=gw)
+        parts.append(gh)
+        rows.append(gw)
+    check_tied_grads(parts[0] + parts[1], torch.cat(rows), h, w, tokens, a, b)
+    tokens[:] = IGN
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    hl, wl = h.requires_grad_(), w.requires_grad_()
+    r = tied_token_logprobs(hl, wl, tokens, IGN)
+    gh, gw = torch.autograd.grad((r.logprobs, r.entropy), (hl, wl), (a, b))
+    assert (r.logprobs == 0).all() and (gh == 0).all() and (gw == 0).all()
+    r = tied_token_logprobs(hl[:0], wl, tokens[:0])
+    (gw,) = torch.autograd.grad(r.logprobs.sum(), (wl,))
+    assert r.logprobs.shape == (0,) and (gw == 0).all()
+
+
+def test_tied_bad_token():
+    from nimbleml_b200.kernels.fused_tied_crossentropy import check_status
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    h, w, tokens, g = make_tied(40, 64, 300, torch.float16, 8)
+    check_status(h.device)
+    tokens[3] = 300
+    tokens[4] = -7
+    hl = h.requires_grad_()
+    r = tied_token_logprobs(hl, w, tokens)
+    assert torch.isnan(r.logprobs[3:5]).all() and torch.isfinite(r.logprobs[5:]).all()
+    with pytest.raises(ValueError):  # at the latest a later call of the path raises by itself
+        check_status(h.device)
+    (gh,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), (torch.ones(40).cuda(), torch.ones(40).cuda()))
+    assert (gh[3:5] == 0).all() and torch.isfinite(gh).all()
+    check_status(h.device)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_captured_and_on_another_stream(tied):
+    """Forward and backward in a CUDA graph, replayed on new values, equal the eager calls bit for bit."""
+    from nimbleml_b200.losses import tied_token_logprobs, token_logprobs
+
+    h, w, tokens, g = make_tied(33, 64, 700, torch.bfloat16, 2)
+    up = (torch.randn(33, generator=g).cuda(), torch.randn(33, generator=g).cuda())
+
+    def work(h, w):
+        if tied:
+            r = tied_token_logprobs(h, w, tokens)
+        else:
+            r = token_logprobs(h @ w.t(), tokens)
+        return (r.logprobs.detach(), r.entropy.detach(), *torch.autograd.grad((r.logprobs, r.entropy), (h, w), up))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hs, ws = h.clone().requires_grad_(), w.clone().requires_grad_()
+        on_side = work(hs, ws)
+    torch.cuda.current_stream().wait_stream(side)
+    del hs, ws
+    hc, wc = h.clone().requires_grad_(), w.clone().requires_grad_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(hc, wc)
+    for turn in range(2):
+        if turn:
+            with torch.no_grad():
+                hc.copy_(-h)
+                wc.mul_(0.5)
+        graph.replay()
+        want = work(hc.detach().clone().requires_grad_(), wc.detach().clone().requires_grad_())
+        for x, y in zip(got, want):
+            assert x.equal(y)
+        if not turn:
+            for x, y in zip(on_side, want):
+                assert x.equal(y)
