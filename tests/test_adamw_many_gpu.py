@@ -2,6 +2,7 @@
 their definition, and both against 64 bits."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -109,7 +110,8 @@ def step8(w, g, mq, vq, step, h):
         c2=1 / math.sqrt(1 - h["beta2"]**step), eps=h["epsilon"]).items()}
     m, r = decode(*mq), decode(*vq)
     m = m * sc["b1"] + g * sc["omb1"]
-    r = ((r * r) * sc["b2"] + (g * g) * sc["omb2"]).sqrt()
+    # NumPy's root is the rounded one; torch's on the CPU may be a last bit off.
+    r = torch.from_numpy(np.sqrt(((r * r) * sc["b2"] + (g * g) * sc["omb2"]).numpy()))
     w = w * sc["decay"] - (m * sc["c1"]) / (r * sc["c2"] + sc["eps"])
     return w, encode(m, False), encode(r, True)
 
@@ -200,8 +202,10 @@ def test_optimizer_many_tensors_none_and_twice(bits):
     p.grad = torch.ones(300, device="cuda")
     twice = AdamW([p, p], state_bits=bits, learning_rate=0.1, weight_decay=0.0)
     twice.step()
-    # m / (sqrt v + eps) is 1 in each of the two updates, to the rounding of the 8-bit path's 1 / 448 scales.
-    assert ((p - 0.8).abs() <= 1e-6).all()
+    # m / (sqrt v + eps) is 1 in each of the two updates, to roundings of 2^-24 and, with fp32 moments, to that of
+    # 1 - 0.999 taken in fp32 as the single step takes it: 0.00099998713 for 0.001, whose root is 6.5e-6 less than one,
+    # so 2 x 0.1 x 6.5e-6 = 1.3e-6 and a few 2^-24.
+    assert ((p - 0.8).abs() <= 1.3e-6 + 8 * 2.0**-24).all()
     m, v = twice.moments()
     assert ((m[0] - 0.1).abs() <= 0.1 * 2.0**-4).all() and ((v[0] - 0.001).abs() <= 0.001 * 2.0**-2).all()
 
