@@ -360,7 +360,7 @@ NIMBLE_API int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int
 
 /* The same two numbers from hidden states and the tied matrix, without an
  * N x V buffer: statistics of one vocab shard, shard_stats (4, n_tokens) fp32 =
- * row max m, sum 2^d, sum d 2^d with d = (s - m) log2 e, and the token's logit
+ * row max m, sum 2^d, sum d 2^d with d = s log2 e - fl(m log2 e), and the token's logit
  * (0 where the shard does not hold it). f16 / bf16, fp32 accumulate. */
 NIMBLE_API int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
                                             int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,

@@ -428,7 +428,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
               u0 = fmaf(e0, fmaxf(d0, kMinD), u0);
               u1 = fmaf(e1, fmaxf(d1, kMinD), u1);
             }
-            const float dm = fmaxf((mrun - mnew) * kLog2e, kMinD);
+            const float dm = fmaxf(__fmul_rn(mrun, kLog2e) - ml2, kMinD);
             const float f = ptx::ex2(dm);
             urun = fmaf(urun + srun * dm, f, u0 + u1);
             srun = fmaf(srun, f, s0 + s1);
@@ -1431,8 +1431,9 @@ lp_row_reduce_kernel(const float2* __restrict__ part, const float* __restrict__ 
   float m = -INFINITY, s = 0.0f, u = 0.0f;
   auto merge = [&](float m2, float s2, float u2) {
     const float mn = fmaxf(m, m2);
-    const float d1 = m == mn ? 0.0f : fmaxf((m - mn) * kLog2e, kMinD);
-    const float d2 = m2 == mn ? 0.0f : fmaxf((m2 - mn) * kLog2e, kMinD);
+    // The reference points are m log2 e rounded to fp32, as in the epilogue.
+    const float d1 = m == mn ? 0.0f : fmaxf(__fmul_rn(m, kLog2e) - __fmul_rn(mn, kLog2e), kMinD);
+    const float d2 = m2 == mn ? 0.0f : fmaxf(__fmul_rn(m2, kLog2e) - __fmul_rn(mn, kLog2e), kMinD);
     const float f1 = ptx::ex2(d1), f2 = ptx::ex2(d2);
     u = (u + s * d1) * f1 + (u2 + s2 * d2) * f2;
     s = s * f1 + s2 * f2;

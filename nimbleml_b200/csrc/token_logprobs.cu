@@ -6,11 +6,16 @@
 // For a row x with token t:
 //   lse = log sum_j exp(x_j),  logp = x_t - lse,
 //   H   = -sum_j p_j log p_j   with p_j = exp(x_j - lse)
-// One pass keeps the running (m, s, u) = (max, sum 2^d, sum d 2^d) with
-// d = (x - m) log2 e; then lse = m + ln s, logp = (x_t - m) - ln s and
-// H = ln s - ln 2 * u / s, which subtract nothing large from anything large:
-// m and ln s are kept apart, since a row of a type's lowest value has an m next
-// to which ln s is lost. With upstream gradients a (of logp) and b (of H):
+// One pass keeps a reference logit f near the running max and, with
+// r = f log2 e rounded to fp32, s = sum 2^d and u = sum d 2^d, d = x log2 e - r
+// (one rounding). f is raised only when a logit lies 2^16 above it: a thread then
+// rescales a few times a row, not at each new max (a warp had rescaled in nearly
+// every vector, since any of its lanes makes all wait: 11 instructions a logit).
+// With c = ln 2 (f log2 e - r), what r left of f:
+//   lse = f + (ln s - c),  logp = (x_t - f) - (ln s - c),  H = ln s - ln 2 * u / s,
+// which subtract nothing large from anything large. The max m and lse - m are kept
+// apart: next to the m of a row of a type's lowest value the logarithm is lost.
+// With upstream gradients a (of logp) and b (of H):
 //   dx_j = a [j = t] - p_j (a + b H + b log p_j).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -19,6 +24,7 @@
 #include <cmath>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "elementwise.cuh"
@@ -34,59 +40,196 @@ constexpr float kLn2 = 0.6931471805599453f;
 // before (fp32 ends at 2^-149), and 0 * -inf must not become NaN.
 constexpr float kMinD = -1.0e4f;
 
-// Running (m, s, u) of a set of logits. A NaN makes s and u NaN; a set of
-// -inf only (or the empty set) is (-inf, 0, 0).
-struct SoftStats {
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
+// Beyond this size two different logits are so far apart that the smaller one's
+// weight is zero, and products with log2 e may overflow: weights are 1 or 0.
+constexpr float kHuge = 1.0e30f;
 
-  __device__ __forceinline__ void raise(float m2) {  // m2 > m
-    const float d = fmaxf((m - m2) * kLog2e, kMinD);
-    const float f = ex2(d);
-    u = (u + s * d) * f;
-    s *= f;
-    m = m2;
+// Packed pairs: one instruction for two fp32 operations.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+
+// Max of n vectors' logits, NaN left aside. 16-bit logits are compared in pairs
+// before they are widened.
+template <typename T, int n>
+__device__ __forceinline__ float vec_max(const uint4 (&raw)[n]) {
+  if constexpr (sizeof(T) == 4) {
+    float hi = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < n; ++i)
+      hi = fmaxf(hi, fmaxf(fmaxf(__uint_as_float(raw[i].x), __uint_as_float(raw[i].y)),
+                           fmaxf(__uint_as_float(raw[i].z), __uint_as_float(raw[i].w))));
+    return hi;
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+    const T2* p = reinterpret_cast<const T2*>(raw);
+    T2 h = p[0];
+#pragma unroll
+    for (int i = 1; i < 4 * n; ++i) h = __hmax2(h, p[i]);
+    float2 f;
+    if constexpr (std::is_same_v<T, __half>) f = __half22float2(h);
+    else f = __bfloat1622float2(h);
+    return fmaxf(f.x, f.y);
   }
-  template <int n>
-  __device__ __forceinline__ float add_n(const float* v) {
-    float vm = v[0];
+}
+// A vector of -inf: what a thread without a vector sums.
+template <typename T> __device__ __forceinline__ uint4 no_vec() {
+  constexpr uint32_t w = sizeof(T) == 4 ? 0xFF800000u : (std::is_same_v<T, __half> ? 0xFC00FC00u : 0xFF80FF80u);
+  return make_uint4(w, w, w, w);
+}
+template <typename T>
+__device__ __forceinline__ void widen(const uint4& raw, float2 (&v)[8 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = make_float2(__uint_as_float(raw.x), __uint_as_float(raw.y));
+    v[1] = make_float2(__uint_as_float(raw.z), __uint_as_float(raw.w));
+  } else {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int k = 1; k < n; ++k) vm = fmaxf(vm, v[k]);
-    if (vm > m) raise(vm);
-    const float at = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int k = 0; k < n; ++k) {
-      // Not v log2 e - m log2 e: that product overflows for a mask of the
-      // lowest fp32 value.
-      const float d = (v[k] - at) * kLog2e;
-      const float e = ex2(d);
-      s += e;
-      u = fmaf(e, fmaxf(d, kMinD), u);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __half>)
+        v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      else
+        v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     }
-    return vm;
   }
-  __device__ __forceinline__ void merge(float m2, float s2, float u2) {
-    if (m2 > m) {
-      // Take the other set's maximum; `this` is scaled down to it.
-      raise(m2);
+}
+
+// Logit j of a vector in registers, j not known at compile time.
+template <typename T>
+__device__ __forceinline__ float vec_elem(const uint4& v, int j) {
+  constexpr int kPer = 4 / sizeof(T);
+  const int q = j / kPer;
+  const uint32_t w = q < 2 ? (q == 0 ? v.x : v.y) : (q == 2 ? v.z : v.w);
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+  const uint16_t h = static_cast<uint16_t>(w >> (16 * (j & 1)));
+  if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half(h));
+  else return __uint_as_float(static_cast<uint32_t>(h) << 16);
+}
+// Bits of the logits of a vector that are >= t.
+template <typename T>
+__device__ __forceinline__ uint32_t vec_at_least(const uint4& raw, float t) {
+  float2 v[8 / sizeof(T)];
+  widen<T>(raw, v);
+  uint32_t mask = 0;
+#pragma unroll
+  for (int k = 0; k < 8 / static_cast<int>(sizeof(T)); ++k) {
+    if (v[k].x >= t) mask |= 1u << (2 * k);
+    if (v[k].y >= t) mask |= 2u << (2 * k);
+  }
+  return mask;
+}
+// Running statistics of a set of logits: max m, reference f (r = f log2 e), s, u. A
+// NaN makes s and u NaN; a set of -inf only (or the empty set) has m = f = -inf and
+// s = u = 0.
+struct SoftStats {
+  static constexpr float kLag = 16.0f;  // most that a logit's d may exceed zero
+  float f = -INFINITY, r = -INFINITY, s = 0.0f, u = 0.0f, m = -INFINITY;
+
+  // d of one reference in terms of another that is not below it.
+  __device__ __forceinline__ static float shift(float f_low, float r_low, float f_high, float r_high) {
+    const float d = r_low - r_high;
+    return f_low == f_high ? 0.0f : (d > kMinD ? d : kMinD);  // NaN (both overflowed): far apart
+  }
+  __device__ __forceinline__ void raise(float f2) {
+    const float r2 = f2 * kLog2e;
+    const float d = shift(f, r, f2, r2);
+    const float w = ex2(d);
+    u = (u + s * d) * w;
+    s *= w;
+    f = f2;
+    r = r2;
+  }
+  __device__ __forceinline__ bool too_low(float v) const {
+    return v > f && (fmaf(v, kLog2e, -r) > kLag || !(fabsf(f) < kHuge));
+  }
+  // Any logit.
+  __device__ __forceinline__ void add(float v) {
+    m = fmaxf(m, v);
+    if (too_low(v)) raise(v);
+    float d = 0.0f, e;
+    if (fabsf(f) < kHuge) {
+      d = fmaf(v, kLog2e, -r);
+      e = ex2(d);
+    } else if (v == f) {  // huge: weight 1; -inf: 0; +inf: NaN
+      e = f == -INFINITY ? 0.0f : 1.0f + (f - f);
+    } else {  // far below, or NaN
+      e = v != v ? v : 0.0f;
+    }
+    s += e;
+    u = fmaf(e, fmaxf(d, kMinD), u);
+  }
+  // n vectors of logits whose max is hi; false (and nothing done) where weights
+  // are not to be taken as exponentials (huge logits).
+  template <typename T, int n>
+  __device__ __forceinline__ bool add_vecs(const uint4 (&raw)[n], float hi) {
+    constexpr int kPairs = 8 / sizeof(T);
+    if (hi >= kHuge) return false;
+    m = fmaxf(m, hi);
+    if (too_low(hi)) raise(hi);
+    if (fabsf(f) >= kHuge && f != -INFINITY) return false;
+    const float2 l2 = make_float2(kLog2e, kLog2e);
+    const float nr1 = f == -INFINITY ? 0.0f : -r;  // nothing but -inf and NaN so far
+    const float2 nr = make_float2(nr1, nr1);
+    float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      float2 v[kPairs];
+      widen<T>(raw[i], v);
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const float2 d = fma2(v[k], l2, nr);
+        const float2 e = make_float2(ex2(d.x), ex2(d.y));
+        s2 = add2(s2, e);
+        // -inf: weight zero, and 0 * -inf must not become NaN.
+        u2 = fma2(e, make_float2(fmaxf(d.x, kMinD), fmaxf(d.y, kMinD)), u2);
+      }
+    }
+    s += s2.x + s2.y;
+    u += u2.x + u2.y;
+    return true;
+  }
+  __device__ __forceinline__ void merge(float f2, float s2, float u2, float m2) {
+    m = fmaxf(m, m2);
+    if (f2 > f) {
+      raise(f2);
       s += s2;
       u += u2;
     } else {
-      const float d = m2 == m ? 0.0f : fmaxf((m2 - m) * kLog2e, kMinD);
-      const float f = ex2(d);
-      u += (u2 + s2 * d) * f;
-      s += s2 * f;
+      const float d = shift(f2, f2 * kLog2e, f, r);
+      const float w = ex2(d);
+      u += (u2 + s2 * d) * w;
+      s += s2 * w;
     }
   }
 };
 
-// max and ln sum: the lse is their sum. A row of -inf only has (-inf, 0).
+// Statistics of `lanes` lanes (a power of two) that have them, in every lane: the
+// highest reference first, then each lane rescales once and two sums are taken.
+__device__ __forceinline__ void lanes_merge(SoftStats& a, int lanes) {
+  float f = a.f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+    if (off < lanes) {
+      f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, off));
+      a.m = fmaxf(a.m, __shfl_xor_sync(0xffffffffu, a.m, off));
+    }
+  if (f > a.f) a.raise(f);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+    if (off < lanes) {
+      a.s += __shfl_xor_sync(0xffffffffu, a.s, off);
+      a.u += __shfl_xor_sync(0xffffffffu, a.u, off);
+    }
+}
+
+// max and ln sum exp(x - max): the lse is their sum. A row of -inf only has (-inf, 0).
 struct RowResult {
   float max, logsum, entropy;
 };
-__device__ __forceinline__ RowResult row_result(float m, float s, float u) {
-  if (m == -INFINITY && s == 0.0f) return {-INFINITY, 0.0f, 0.0f};
-  const float ls = logf(s);
-  return {m, ls, ls - kLn2 * (u / s)};
+__device__ __forceinline__ RowResult row_result(const SoftStats& a) {
+  if (a.m == -INFINITY && a.s == 0.0f) return {-INFINITY, 0.0f, 0.0f};
+  const float ls = logf(a.s);
+  const float c = fabsf(a.f) < kHuge ? kLn2 * fmaf(a.f, kLog2e, -a.r) : 0.0f;
+  return {a.m, (a.f == a.m ? 0.0f : a.f - a.m) + (ls - c), ls - kLn2 * (a.u / a.s)};
 }
 // A row of -inf only gives every token -inf instead of NaN.
 __device__ __forceinline__ float token_logprob(float x, float max, float logsum) {
@@ -97,24 +240,35 @@ __device__ __forceinline__ float token_logprob(float x, float max, float logsum)
 // A logit and its column as one key that orders like (value, lowest column):
 // the value's bits made monotonic (+0 and -0 are one value), then the column's
 // complement. No two columns of a row have the same key, and 0 is below all.
-__device__ __forceinline__ uint64_t make_key(float v, uint32_t col) {
+__device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
-  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return (static_cast<uint64_t>(o) << 32) | static_cast<uint32_t>(~col);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t o = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float unordered(uint32_t o) {
   return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
+__device__ __forceinline__ uint64_t make_key(float v, uint32_t col) {
+  return (static_cast<uint64_t>(ordered(v)) << 32) | static_cast<uint32_t>(~col);
+}
+__device__ __forceinline__ float key_value(uint64_t key) { return unordered(static_cast<uint32_t>(key >> 32)); }
 __device__ __forceinline__ uint32_t key_col(uint64_t key) { return ~static_cast<uint32_t>(key); }
 
+// The top k of a row in one pass over it. While the logits are summed, each
+// thread notes the maxima of up to kSegs segments of its share. The k-th best of
+// the threads' maxima, found by bisection over counts, is no better than the k-th
+// best logit; only segments that reach it are read again (from L2: k of 16 x 256
+// and a few more), and what reaches it there is sorted. Keeping a list of
+// candidates against a rising threshold inside the pass was measured first: its
+// rare, divergent insertions took 150 to 900 us of a 4096 x 128256 bf16 pass for
+// k = 5 to 64, which takes 150 us by itself.
 constexpr int kMaxTopK = 64;
 constexpr int kRowThreads = 256;
-// More candidates than this after a step are cut back to the best k, so a
-// step of one vector a thread (256 x 8 logits at most) always finds room.
-constexpr int kKeyWater = 256;
-constexpr int kKeyCap = kKeyWater + kRowThreads * 8;
-constexpr int kSortCap = 4096;  // the power of two that a sort of kKeyCap keys fills up to
+constexpr int kSegs = 16;
+constexpr int kKeyCap = 2048;  // candidates a block holds
+// The second scan below: candidates beyond kKeyWater are cut back to the best k
+// after each of its steps, which offer at most 4 logits a thread.
+constexpr int kKeyWater = 512;
+static_assert(kKeyWater + 4 * kRowThreads <= kKeyCap, "a step of the second scan must find room");
 
 // Sorts keys[0, n) in descending order (bitonic, whole block); keys must have
 // room for the next power of two of n. Starts and ends with a barrier.
@@ -142,21 +296,36 @@ __device__ void block_sort_desc(uint64_t* keys, int n) {
 }
 
 struct TopKShared {
-  uint64_t keys[kSortCap];
+  uint64_t keys[kKeyCap];
+  uint64_t best[kMaxTopK];  // the best k, sorted
+  float seg_max[kSegs][kRowThreads];
   uint64_t tau;  // keys above it are candidates
   int count;
 };
 
-// Cuts the first n candidates back to the best k (sorted) and raises the
-// threshold to the k-th. Returns how many are left. Whole block; starts and
-// ends with a barrier.
+// The best k of the first n candidates, sorted, to sh.best and to the front of
+// sh.keys; the threshold becomes the k-th. Returns how many there are. Whole
+// block; starts and ends with a barrier.
 __device__ int topk_prune(TopKShared& sh, int n, int k) {
-  block_sort_desc(sh.keys, n);
   const int left = min(n, k);
-  if (threadIdx.x == 0) {
-    sh.count = left;
-    if (n >= k) sh.tau = sh.keys[k - 1];
+  if (n <= kRowThreads) {
+    // Few: each takes the place that the number of greater ones gives it.
+    __syncthreads();
+    if (threadIdx.x < n) {
+      const uint64_t key = sh.keys[threadIdx.x];
+      int rank = 0;
+      for (int i = 0; i < n; ++i) rank += sh.keys[i] > key;
+      if (rank < k) sh.best[rank] = key;
+    }
+    __syncthreads();
+    if (threadIdx.x < left) sh.keys[threadIdx.x] = sh.best[threadIdx.x];
+  } else {
+    block_sort_desc(sh.keys, n);
+    if (threadIdx.x < left) sh.best[threadIdx.x] = sh.keys[threadIdx.x];
   }
+  if (threadIdx.x == 0) sh.count = left;
+  __syncthreads();
+  if (threadIdx.x == 0 && n >= k) sh.tau = sh.best[k - 1];
   __syncthreads();
   return left;
 }
@@ -165,7 +334,7 @@ __device__ int topk_prune(TopKShared& sh, int n, int k) {
 // A cluster of `parts` blocks per row, each block on one contiguous part of
 // the columns; its first block merges the parts over distributed shared memory.
 template <typename T, bool kTopK>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, kTopK ? 5 : 6)
 logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens, int64_t V,
                      int64_t ignore_index, int k, int parts, float* __restrict__ out_logp,
                      float* __restrict__ out_ent, float* __restrict__ out_max, float* __restrict__ out_logsum,
@@ -174,8 +343,8 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kU = 4;  // 16-byte loads in flight per thread
   constexpr int kWarps = kRowThreads / 32;
-  __shared__ float sm_warp[3][kWarps];
-  __shared__ float sm_part[3];
+  __shared__ float sm_warp[4][kWarps];
+  __shared__ float sm_part[4];
   extern __shared__ __align__(16) uint8_t dyn[];
   TopKShared& sh = *reinterpret_cast<TopKShared*>(dyn);  // dereferenced only with kTopK
 
@@ -202,153 +371,157 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   const int64_t per = ((V + parts - 1) / parts + 63) / 64 * 64;
   const int64_t c0 = min(V, part * per), c1 = min(V, c0 + per);
   const T* r = x + row * ld + c0;
-  const int64_t n = c1 - c0;
+  const int n = static_cast<int>(c1 - c0);  // V < 2^31
   // The elements up to the 16-byte grid and behind the last vector go one by one.
-  const int64_t head = min(n, static_cast<int64_t>(((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / sizeof(T)));
-  const int64_t nvec = (n - head) / kVec;
-  const int64_t tail0 = head + nvec * kVec;
+  const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / sizeof(T)));
+  const int nvec = (n - head) / kVec;
+  const int tail0 = head + nvec * kVec;
   const uint4* r4 = reinterpret_cast<const uint4*>(r + head);
 
   SoftStats acc;
   float tau_v = -INFINITY;
   uint64_t tau = 0;
-  int kept = 0;  // candidates in place, the same in every thread
-  if constexpr (kTopK) {
-    if (threadIdx.x == 0) {
-      sh.tau = 0;
-      sh.count = 0;
-    }
-    __syncthreads();
-  }
-  // Offers one logit as a candidate.
-  auto offer = [&](float v, int64_t col) -> bool {
-    if (!(v >= tau_v)) return false;
-    const uint64_t key = make_key(v, static_cast<uint32_t>(col));
-    if (key <= tau) return false;
+  // Offers one logit as a candidate. The counter goes on where there is no room.
+  auto offer = [&](float v, uint32_t col) {
+    if (!(v >= tau_v)) return;
+    const uint64_t key = make_key(v, col);
+    if (key <= tau) return;
     const int slot = atomicAdd(&sh.count, 1);
     if (slot < kKeyCap) sh.keys[slot] = key;
-    return true;
   };
   auto take_threshold = [&] {
     tau = sh.tau;
     tau_v = tau ? key_value(tau) : -INFINITY;
   };
+  const uint32_t col0 = static_cast<uint32_t>(c0);
 
-  if (threadIdx.x < head + (n - tail0)) {  // fewer than 2 * kVec <= 16 elements
-    const int64_t j = threadIdx.x < head ? threadIdx.x : tail0 + (threadIdx.x - head);
-    const float v = to_f<T>(r[j]);
-    acc.add_n<1>(&v);
-    if constexpr (kTopK) offer(v, c0 + j);
+  const int steps = (nvec + kU * kRowThreads - 1) / (kU * kRowThreads);
+  const int per_seg = (steps + kSegs - 1) / kSegs;  // steps a segment
+  auto vec_at = [&](int p, int i) { return (p * kU + i) * kRowThreads + static_cast<int>(threadIdx.x); };
+  float seg_hi = -INFINITY;
+  int seg = 0, seg_left = per_seg;
+  for (int p = 0; p < steps; ++p) {
+    uint4 raw[kU];
+#pragma unroll
+    for (int i = 0; i < kU; ++i) raw[i] = vec_at(p, i) < nvec ? __ldg(r4 + vec_at(p, i)) : no_vec<T>();
+    const float hi = vec_max<T, kU>(raw);
+    if (!acc.template add_vecs<T, kU>(raw, hi)) {
+#pragma unroll 1
+      for (int i = 0; i < kU; ++i)
+#pragma unroll 1
+        for (int j = 0; j < kVec && vec_at(p, i) < nvec; ++j) acc.add(to_f<T>(r[head + vec_at(p, i) * kVec + j]));
+    }
+    if constexpr (kTopK) {
+      seg_hi = fmaxf(seg_hi, hi);
+      if (--seg_left == 0) {
+        sh.seg_max[seg++][threadIdx.x] = seg_hi;  // read by this thread only
+        seg_hi = -INFINITY;
+        seg_left = per_seg;
+      }
+    }
   }
+  // The fewer than 2 * kVec <= 16 elements before and behind the vectors.
+  const bool ragged = static_cast<int>(threadIdx.x) < head + (n - tail0);
+  const int ragged_j = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail0 + (threadIdx.x - head);
+  float ragged_v = -INFINITY;
+  if (ragged) {
+    ragged_v = to_f<T>(r[ragged_j]);
+    acc.add(ragged_v);
+  }
+  if constexpr (kTopK) {
+    if (seg_left != per_seg) sh.seg_max[seg++][threadIdx.x] = seg_hi;
+    if (threadIdx.x == 0) {
+      sh.tau = 0;
+      sh.count = 0;
+    }
+    // Largest 16-bit prefix of an ordered value that k threads' maxima reach; 0
+    // where fewer than k threads have any logit.
+    const uint32_t mine = nvec > static_cast<int>(threadIdx.x) || ragged ? ordered(acc.m) : 0u;
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t t = prefix | (1u << bit);
+      if (__syncthreads_count(mine >= (t << 16)) >= k) prefix = t;
+    }
+    tau_v = prefix <= 0x007Fu ? -INFINITY : unordered(prefix << 16);
+    if (ragged) offer(ragged_v, col0 + ragged_j);
+#pragma unroll 1
+    for (int g = 0; g < seg; ++g) {
+      if (!(sh.seg_max[g][threadIdx.x] >= tau_v)) continue;
+#pragma unroll 1
+      for (int p = g * per_seg; p < min(steps, (g + 1) * per_seg); ++p) {
+        uint4 raw[kU];
+#pragma unroll
+        for (int i = 0; i < kU; ++i) raw[i] = vec_at(p, i) < nvec ? __ldg(r4 + vec_at(p, i)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kU; ++i) {
+          if (vec_at(p, i) >= nvec) continue;
+#pragma unroll 1
+          for (uint32_t mask = vec_at_least<T>(raw[i], tau_v); mask != 0; mask &= mask - 1) {
+            const int j = __ffs(mask) - 1;
+            offer(vec_elem<T>(raw[i], j), col0 + head + vec_at(p, i) * kVec + j);
+          }
+        }
+      }
+    }
+  }
+  int kept = 0;
   if constexpr (kTopK) {
     __syncthreads();
     kept = sh.count;
     __syncthreads();
-  }
-
-  for (int64_t q0 = 0; q0 < nvec; q0 += kU * kRowThreads) {
-    uint4 raw[kU];
-    float vmax[kU];
-#pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      const int64_t q = q0 + i * kRowThreads + threadIdx.x;
-      if (q < nvec) raw[i] = __ldg(r4 + q);
-    }
-#pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      const int64_t q = q0 + i * kRowThreads + threadIdx.x;
-      vmax[i] = -INFINITY;
-      if (q < nvec) {
-        const T* e = reinterpret_cast<const T*>(&raw[i]);
-        float v[kVec];
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) v[j] = to_f<T>(e[j]);
-        vmax[i] = acc.add_n<kVec>(v);
+    if (kept <= kKeyCap) {
+      kept = topk_prune(sh, kept, k);
+    } else {
+      // More candidates than room (a row that rises with its columns): scan the
+      // part again, from the threshold that the candidates at hand give, and cut
+      // the candidates back between steps. The candidates themselves come again.
+      topk_prune(sh, kKeyCap, k);
+      if (threadIdx.x == 0) {
+        sh.tau = sh.best[k - 1] - 1;
+        sh.count = 0;
       }
-    }
-    if constexpr (kTopK) {
-      auto has = [&](int i) { return q0 + i * kRowThreads + threadIdx.x < nvec; };
-      auto col_of = [&](int i) { return c0 + head + (q0 + i * kRowThreads + threadIdx.x) * kVec; };
-      auto offer_vec = [&](int i) -> bool {
-        bool any = false;
-        if (has(i) && vmax[i] >= tau_v) {
-          const T* e = reinterpret_cast<const T*>(&raw[i]);
+      __syncthreads();
+      take_threshold();
+      kept = 0;
+      for (int j0 = 0; j0 < n; j0 += 4 * kRowThreads) {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) any |= offer(to_f<T>(e[j]), col_of(i) + j);
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + e * kRowThreads + threadIdx.x;
+          if (j < n) offer(to_f<T>(r[j]), col0 + j);
         }
-        return any;
-      };
-      if (q0 == 0 && nvec >= kRowThreads) {
-        // A first threshold: the k-th best of the threads' own best logits
-        // is no better than the k-th best of the part.
-        uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < kU; ++i) {
-          if (!has(i)) continue;
-          const T* e = reinterpret_cast<const T*>(&raw[i]);
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) {
-            const float v = to_f<T>(e[j]);
-            if (v >= vmax[i]) best = max(best, make_key(v, static_cast<uint32_t>(col_of(i) + j)));
-          }
-        }
-        uint64_t* own = sh.keys + kept;  // kept < 16 here
-        own[threadIdx.x] = best;
-        block_sort_desc(own, kRowThreads);
-        if (threadIdx.x == 0 && own[k - 1] != 0) sh.tau = own[k - 1] - 1;  // k <= kMaxTopK <= kRowThreads
         __syncthreads();
-        take_threshold();
-      }
-      bool any = false;
-#pragma unroll
-      for (int i = 0; i < kU; ++i) any |= offer_vec(i);
-      if (__syncthreads_or(any)) {
-        const int count = sh.count;
+        kept = sh.count;
         __syncthreads();
-        if (count > kKeyCap) {
-          // More candidates than there is room for (a row that rises towards
-          // its end): take this step's back and offer it one vector a thread
-          // at a time, which fits.
-          if (threadIdx.x == 0) sh.count = kept;
-#pragma unroll
-          for (int i = 0; i < kU; ++i) {
-            __syncthreads();
-            offer_vec(i);
-            __syncthreads();
-            kept = topk_prune(sh, sh.count, k);
-            take_threshold();
-          }
-        } else if (count > kKeyWater) {
-          kept = topk_prune(sh, count, k);
+        if (kept > kKeyWater) {
+          kept = topk_prune(sh, kept, k);
           take_threshold();
-        } else {
-          kept = count;
         }
       }
+      kept = topk_prune(sh, kept, k);
     }
   }
-  if constexpr (kTopK) kept = topk_prune(sh, kept, k);
 
   // The block's statistics: lanes, then warps, in a fixed order.
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, acc.m, off);
-    const float s2 = __shfl_xor_sync(0xffffffffu, acc.s, off);
-    const float u2 = __shfl_xor_sync(0xffffffffu, acc.u, off);
-    acc.merge(m2, s2, u2);
-  }
+  lanes_merge(acc, 32);
   if ((threadIdx.x & 31) == 0) {
-    sm_warp[0][threadIdx.x >> 5] = acc.m;
+    sm_warp[0][threadIdx.x >> 5] = acc.f;
     sm_warp[1][threadIdx.x >> 5] = acc.s;
     sm_warp[2][threadIdx.x >> 5] = acc.u;
+    sm_warp[3][threadIdx.x >> 5] = acc.m;
   }
   __syncthreads();
   SoftStats all;
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < kWarps; ++w) all.merge(sm_warp[0][w], sm_warp[1][w], sm_warp[2][w]);
-    sm_part[0] = all.m;
-    sm_part[1] = all.s;
-    sm_part[2] = all.u;
+  if (threadIdx.x < 32) {
+    const int w = threadIdx.x & (kWarps - 1);
+    all.merge(sm_warp[0][w], sm_warp[1][w], sm_warp[2][w], sm_warp[3][w]);
+    lanes_merge(all, kWarps);
+    if (threadIdx.x == 0) {
+      sm_part[0] = all.f;
+      sm_part[1] = all.s;
+      sm_part[2] = all.u;
+      sm_part[3] = all.m;
+    }
   }
   if (parts > 1) {
     cg::cluster_group cluster = cg::this_cluster();
@@ -357,7 +530,7 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
       if (threadIdx.x == 0)
         for (int p = 1; p < parts; ++p) {
           const float* o = cluster.map_shared_rank(&sm_part[0], p);
-          all.merge(o[0], o[1], o[2]);
+          all.merge(o[0], o[1], o[2], o[3]);
         }
       if constexpr (kTopK) {
         // parts * k <= 8 * 64 keys.
@@ -374,7 +547,7 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
     if (part != 0) return;
   }
   if (threadIdx.x == 0) {
-    const RowResult res = row_result(all.m, all.s, all.u);
+    const RowResult res = row_result(all);
     const bool bad = tok < 0 || tok >= V;
     if (bad && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
     out_logp[row] =
@@ -483,10 +656,10 @@ __global__ void logprobs_combine_kernel(const float* __restrict__ stats, int sha
   float target = 0.0f;
   for (int p = 0; p < shards; ++p) {
     const float* s = stats + static_cast<int64_t>(p) * 4 * N + i;
-    acc.merge(s[0], s[N], s[2 * N]);
+    acc.merge(s[0], s[N], s[2 * N], s[0]);
     target += s[3 * N];
   }
-  const RowResult res = row_result(acc.m, acc.s, acc.u);
+  const RowResult res = row_result(acc);
   const bool bad = tok < 0 || tok >= V;
   if (bad && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
   out_logp[i] = bad ? __int_as_float(0x7fc00000) : token_logprob(target, res.max, res.logsum);

@@ -166,7 +166,8 @@ def round_tf32(x: torch.Tensor) -> torch.Tensor:
 
 
 def _stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def compute_dtype_of(t: torch.Tensor) -> int:

@@ -18,11 +18,10 @@ d/dx_j (a logp_t + b H) = a [j = t] - p_j (a + b (H + log p_j)).
 """
 from __future__ import annotations
 
-import contextlib
+import math
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from nimbleml_b200.kernels.fused_tied_crossentropy import (
     _NO_IGNORE,
@@ -55,62 +54,92 @@ class TokenLogProbs(NamedTuple):
     top_ids: Optional[torch.Tensor] = None
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current for the native calls when it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
 def _grad_rows(grad: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if grad is None else grad.reshape(-1).float().contiguous()
+    if grad is None:
+        return None
+    if grad.dtype != torch.float32:
+        grad = grad.float()
+    return grad if grad.is_contiguous() else grad.contiguous()
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _token_ids(tokens, n: int, device: torch.device) -> torch.Tensor:
+    if (isinstance(tokens, torch.Tensor) and tokens.dtype == torch.int64 and tokens.device == device and
+            tokens.numel() == n and tokens.is_contiguous()):
+        return tokens  # the kernels read n ids in order, whatever the shape
+    return as_label_indices(tokens, batch_size=n, device=device)
+
+
+def _refuse_double_backward() -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError("the log probabilities' backward is not differentiable itself")
+
+
+def _rows_forward(x2d, tokens, ignore_index, top_k):
+    """(x2d as the kernel read it, (4, n) log probability, entropy, max, ln sum; alternatives)."""
+    dev = x2d.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _rows_forward(x2d, tokens, ignore_index, top_k)
+    n, v = x2d.shape
+    # Rows may be a view of wider ones; a broadcast or a transposed matrix is copied.
+    if x2d.stride(1) != 1 or (n > 1 and x2d.stride(0) < v):
+        x2d = x2d.contiguous()
+    out = torch.empty((4, n), dtype=torch.float32, device=dev)
+    top_lp = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
+    top_id = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
+    at = out.data_ptr()
+    native.call("nimble_token_logprobs_forward", x2d.data_ptr(), max(x2d.stride(0), v), tokens.data_ptr(), n, v,
+                _TORCH_TO_NIMBLE[x2d.dtype], ignore_index, top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
+                _ptr(top_lp), _ptr(top_id), status_word(dev).data_ptr(), _stream_ptr(dev))
+    if CHECK_BOUNDS:
+        check_status(dev)
+    return x2d, out, top_lp, top_id
+
+
+def _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index):
+    dev = x2d.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index)
+    n, v = x2d.shape
+    ld = max(x2d.stride(0), v)
+    # Rows of whole 16 bytes where the logits have them, so that both sides use vectors.
+    per16 = 16 // x2d.element_size()
+    pitch = -(-v // per16) * per16 if ld % per16 == 0 else v
+    g = torch.empty((n, pitch), dtype=x2d.dtype, device=dev)
+    a, b, at = _grad_rows(g_lp), _grad_rows(g_ent), out.data_ptr()
+    native.call("nimble_token_logprobs_backward", _ptr(a), _ptr(b), x2d.data_ptr(), ld, tokens.data_ptr(),
+                at + 8 * n, at + 12 * n, at + 4 * n, n, v, _TORCH_TO_NIMBLE[x2d.dtype], ignore_index, g.data_ptr(),
+                pitch, _stream_ptr(dev))
+    return g if pitch == v else g[:, :v]
+
+
 class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x2d, tokens, ignore_index, top_k):
-        n, v = x2d.shape
-        dev = x2d.device
-        # Rows may be a view of wider ones; a broadcast or a transposed matrix is copied.
-        if x2d.stride(1) != 1 or (n > 1 and x2d.stride(0) < v):
-            x2d = x2d.contiguous()
-        out = torch.empty((4, n), dtype=torch.float32, device=dev)
-        top_lp = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
-        top_id = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
-        with _on(dev):
-            native.call("nimble_token_logprobs_forward", x2d.data_ptr(), max(x2d.stride(0), v), tokens.data_ptr(), n,
-                        v, _TORCH_TO_NIMBLE[x2d.dtype], ignore_index, top_k, out[0].data_ptr(), out[1].data_ptr(),
-                        out[2].data_ptr(), out[3].data_ptr(), _ptr(top_lp), _ptr(top_id), status_word(dev).data_ptr(), _stream_ptr(dev))
-        if CHECK_BOUNDS:
-            check_status(dev)
-        lp, ent, row_max, logsum = out.unbind(0)
+    def forward(ctx, logits, tokens, ignore_index, top_k):
+        v = logits.shape[-1]
+        x2d, out, top_lp, top_id = _rows_forward(logits if logits.ndim == 2 else logits.reshape(-1, v), tokens,
+                                                 ignore_index, top_k)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x2d, tokens, row_max, logsum, ent)
-        ctx.ignore_index = ignore_index
+        ctx.save_for_backward(x2d, tokens, out)
+        ctx.meta = (ignore_index, logits.shape)
         if top_k:
             ctx.mark_non_differentiable(top_lp, top_id)
-        return lp, ent, top_lp, top_id
+        return out[0], out[1], top_lp, top_id
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent, *_):
-        x2d, tokens, row_max, logsum, ent = ctx.saved_tensors
+        _refuse_double_backward()
         if g_lp is None and g_ent is None:
             return None, None, None, None
-        n, v = x2d.shape
-        ld = max(x2d.stride(0), v)
-        # Rows of whole 16 bytes where the logits have them, so that both sides use vectors.
-        per16 = 16 // x2d.element_size()
-        pitch = -(-v // per16) * per16 if ld % per16 == 0 else v
-        g = torch.empty((n, pitch), dtype=x2d.dtype, device=x2d.device)
-        a, b = _grad_rows(g_lp), _grad_rows(g_ent)
-        with _on(x2d.device):
-            native.call("nimble_token_logprobs_backward", _ptr(a), _ptr(b), x2d.data_ptr(), ld, tokens.data_ptr(),
-                        row_max.data_ptr(), logsum.data_ptr(), ent.data_ptr(), n, v, _TORCH_TO_NIMBLE[x2d.dtype], ctx.ignore_index,
-                        g.data_ptr(), pitch, _stream_ptr(x2d.device))
-        return g[:, :v], None, None, None
+        x2d, tokens, out = ctx.saved_tensors
+        ignore_index, shape = ctx.meta
+        g = _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index)
+        return g if len(shape) == 2 else g.reshape(shape), None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = None, *, top_k: int = 0) -> TokenLogProbs:
@@ -132,21 +161,26 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs on B200 needs CUDA tensors; there is no CPU path")
     compute_dtype_of(logits)
-    if logits.ndim == 0 or logits.shape[-1] == 0:
+    shape = logits.shape
+    if not shape or shape[-1] == 0:
         raise ValueError("logits must be (..., classes) with at least one class")
-    v = logits.shape[-1]
+    v = shape[-1]
     top_k = int(top_k)
     if not 0 <= top_k <= min(MAX_TOP_K, v):
         raise ValueError(f"top_k must lie in [0, {min(MAX_TOP_K, v)}], got {top_k}")
-    shape = logits.shape[:-1]
-    x2d = logits.reshape(-1, v)
-    ids = as_label_indices(tokens, batch_size=x2d.shape[0], device=logits.device)
+    shape = shape[:-1]
+    ids = _token_ids(tokens, math.prod(shape), logits.device)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
-    lp, ent, top_lp, top_id = _TokenLogProbs.apply(x2d, ids, ign, top_k)
-    if not top_k:
-        return TokenLogProbs(lp.reshape(shape), ent.reshape(shape))
-    return TokenLogProbs(lp.reshape(shape), ent.reshape(shape), top_lp.reshape(*shape, top_k),
-                         top_id.reshape(*shape, top_k))
+    if logits.requires_grad and torch.is_grad_enabled():
+        lp, ent, top_lp, top_id = _TokenLogProbs.apply(logits, ids, ign, top_k)
+    else:
+        _, out, top_lp, top_id = _rows_forward(logits if len(shape) == 1 else logits.reshape(-1, v), ids, ign, top_k)
+        lp, ent = out[0], out[1]
+    if len(shape) != 1:
+        lp, ent = lp.view(shape), ent.view(shape)
+        if top_k:
+            top_lp, top_id = top_lp.view(*shape, top_k), top_id.view(*shape, top_k)
+    return TokenLogProbs(lp, ent, top_lp, top_id)
 
 
 def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0) -> torch.Tensor:
@@ -165,19 +199,19 @@ def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, 
 
 
 def combine_logprob_stats(stats: torch.Tensor, tokens: torch.Tensor, vocab_size: int, ignore_index: int):
-    """Merges (P, 4, N) shard statistics into (logprobs, entropy, lse), each (N,)."""
+    """Merges (P, 4, N) shard statistics into (3, N): log probabilities, entropies, lse."""
     p, _, n = stats.shape
     dev = stats.device
     out = torch.empty((3, n), dtype=torch.float32, device=dev)
+    at = out.data_ptr()
     native.call("nimble_tied_logprobs_combine", stats.data_ptr(), p, tokens.data_ptr(), n, vocab_size, ignore_index,
-                out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), status_word(dev).data_ptr(),
-                _stream_ptr(dev))
-    return out.unbind(0)
+                at, at + 4 * n, at + 8 * n, status_word(dev).data_ptr(), _stream_ptr(dev))
+    return out
 
 
 def shard_logprob_backward(g_lp, g_ent, h, w, tokens, lse, ent, *, vocab_offset=0, vocab_size=None, ignore_index,
                            grad_hidden=None, grad_weights=None, accumulate=False):
-    """Adds nothing to None: fills ``grad_hidden`` (this shard's partial) and ``grad_weights`` where given."""
+    """Fills ``grad_hidden`` (this shard's partial) and fills or adds to ``grad_weights``, those that are given."""
     n, d = h.shape
     v_local = w.shape[0]
     dt = compute_dtype_of(h)
@@ -197,62 +231,70 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group):
+    """(h, w as the kernels read them, (3, n) log probability, entropy, lse)."""
+    from nimbleml_b200 import vocab_parallel
+
+    dev = hidden.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
+    # 16-bit operands for the tensor cores; fp32 master weights still get an fp32 grad.
+    w = _aligned(weights if weights.dtype == hidden.dtype else weights.to(hidden.dtype))
+    h = _aligned(hidden if hidden.ndim == 2 else hidden.reshape(-1, hidden.shape[-1]))
+    # A captured launch must not be joined by event queries and host copies.
+    watch = not torch.cuda.is_current_stream_capturing()
+    if watch:
+        poll_status(dev)
+    part = shard_logprob_stats(h, w, tokens, vocab_offset)
+    if vocab_parallel.world_size(group) > 1:
+        part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
+    else:
+        part = part.unsqueeze(0)
+    out = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
+    if watch:
+        snapshot_status(dev)
+    if CHECK_BOUNDS:
+        check_status(dev)
+    return h, w, out
+
+
 class _TiedTokenLogProbs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, h2d, weights, tokens, ignore_index, vocab_offset, vocab_size, group, grad_buffer):
-        from nimbleml_b200 import vocab_parallel
-
-        dev = h2d.device
-        # 16-bit operands for the tensor cores; fp32 master weights still get an fp32 grad.
-        w = _aligned(weights if weights.dtype == h2d.dtype else weights.to(h2d.dtype))
-        h = _aligned(h2d)
-        # A captured launch must not be joined by event queries and host copies.
-        watch = not torch.cuda.is_current_stream_capturing()
-        with _on(dev):
-            if watch:
-                poll_status(dev)
-            part = shard_logprob_stats(h, w, tokens, vocab_offset)
-            if vocab_parallel.world_size(group) > 1:
-                part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
-            else:
-                part = part.unsqueeze(0)
-            lp, ent, lse = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
-            if watch:
-                snapshot_status(dev)
-        if CHECK_BOUNDS:
-            check_status(dev)
+    def forward(ctx, hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group, grad_buffer):
+        h, w, out = _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(h, w, tokens, lse, ent)
-        ctx.meta = (ignore_index, vocab_offset, vocab_size, group, weights.dtype)
+        ctx.save_for_backward(h, w, tokens, out)
+        ctx.meta = (ignore_index, vocab_offset, vocab_size, group, weights.dtype, hidden.shape)
         ctx.grad_buffer = grad_buffer
-        return lp, ent
+        return out[0], out[1]
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_lp, g_ent):
         from nimbleml_b200 import vocab_parallel
 
+        _refuse_double_backward()
         none = (None,) * 6
         if g_lp is None and g_ent is None:
             return (None, None, *none)
-        h, w, tokens, lse, ent = ctx.saved_tensors
-        ignore_index, vocab_offset, vocab_size, group, w_dtype = ctx.meta
+        h, w, tokens, out = ctx.saved_tensors
+        ignore_index, vocab_offset, vocab_size, group, w_dtype, shape = ctx.meta
         buf = ctx.grad_buffer
         dev = h.device
         world = vocab_parallel.world_size(group)
-        gh = gw = None
-        if ctx.needs_input_grad[0]:
-            gh = torch.empty(h.shape, dtype=vocab_parallel.dh_reduce_dtype(h.dtype) if world > 1 else h.dtype,
-                             device=dev)
-        if buf is not None:
-            gw = buf
-        elif ctx.needs_input_grad[1]:
-            gw = torch.empty(w.shape, dtype=w_dtype, device=dev)
-        watch = not torch.cuda.is_current_stream_capturing()
-        with _on(dev):
+        with torch.cuda.device(dev):
+            gh = gw = None
+            if ctx.needs_input_grad[0]:
+                gh = torch.empty(h.shape, dtype=vocab_parallel.dh_reduce_dtype(h.dtype) if world > 1 else h.dtype,
+                                 device=dev)
+            if buf is not None:
+                gw = buf
+            elif ctx.needs_input_grad[1]:
+                gw = torch.empty(w.shape, dtype=w_dtype, device=dev)
+            watch = not torch.cuda.is_current_stream_capturing()
             if watch:
                 poll_status(dev)
-            shard_logprob_backward(_grad_rows(g_lp), _grad_rows(g_ent), h, w, tokens, lse, ent,
+            shard_logprob_backward(_grad_rows(g_lp), _grad_rows(g_ent), h, w, tokens, out[2], out[1],
                                    vocab_offset=vocab_offset, vocab_size=vocab_size, ignore_index=ignore_index,
                                    grad_hidden=gh, grad_weights=gw, accumulate=buf is not None)
             if watch:
@@ -261,6 +303,8 @@ class _TiedTokenLogProbs(torch.autograd.Function):
                 gh = vocab_parallel.reduce_grad_hidden(gh, group).to(h.dtype)
         if CHECK_BOUNDS:
             check_status(dev)
+        if gh is not None and len(shape) != 2:
+            gh = gh.view(shape)
         return (gh, None if buf is not None else gw, *none)
 
 
@@ -304,12 +348,17 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
                                             not grad_weights_buffer.is_contiguous()):
         raise ValueError("grad_weights_buffer must be a contiguous float32 tensor of the weights' shape")
     shape = hidden.shape[:-1]
-    h2d = hidden.reshape(-1, d)
-    ids = as_label_indices(tokens, batch_size=h2d.shape[0], device=hidden.device)
+    ids = _token_ids(tokens, math.prod(shape), hidden.device)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
-    lp, ent = _TiedTokenLogProbs.apply(h2d, weights, ids, ign, int(vocab_offset), vocab_size, group,
-                                       grad_weights_buffer)
-    return TokenLogProbs(lp.reshape(shape), ent.reshape(shape))
+    args = (hidden, weights, ids, ign, int(vocab_offset), vocab_size, group)
+    if (hidden.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
+        lp, ent = _TiedTokenLogProbs.apply(*args, grad_weights_buffer)
+    else:
+        out = _tied_forward(*args)[2]
+        lp, ent = out[0], out[1]
+    if len(shape) != 1:
+        lp, ent = lp.view(shape), ent.view(shape)
+    return TokenLogProbs(lp, ent)
 
 
 __all__ = ["TokenLogProbs", "token_logprobs", "tied_token_logprobs", "MAX_TOP_K"]

@@ -1,8 +1,9 @@
 """Token log probabilities over logits and from the tied matrix, against 64-bit definitions.
 
-Tolerances are bounds, element by element, with u = 2^-24. Let d = x - m (m the row's
-max), D1 = sum p |d| and D2 = sum p d^2. An exponential is off by 2^-22 of itself and by
-2 u |d| from its argument; a lane adds at most n = V / 256 + 48 terms in a row (the rest
+Tolerances are bounds, element by element, with u = 2^-24. Exponentials are taken of
+d = x - f, f a logit within L = 16 ln 2 below the row's max or at it. Let D1 = sum p |x - m| + L
+and D2 = sum p (|x - m| + L)^2. An exponential is off by 2^-22 of itself and by 2 u |d|
+from its argument; a lane adds at most n = V / 256 + 48 terms in a row (the rest
 is a tree), each addition off by u of the sum. So the sum is off by
 e_s = n u + 2^-22 + 2 u D1 relative, ln s by e_s + u |ln s|; a log probability by that and
 u (|x - m| + |logp|); the entropy ln s - sum(2^d d) / s by e_s + (n u + 2^-22 + e_s) D1 +
@@ -40,7 +41,8 @@ def exact_rows(x, tokens):
 def row_bounds(p, d, h):
     """(of the sum's logarithm, of the entropy), each (rows,)."""
     u, v = 2.0**-24, p.shape[1]
-    d1, d2 = (p * d.abs()).sum(1), (p * d * d).sum(1)
+    lag = 16 * np.log(2)
+    d1, d2 = (p * d.abs()).sum(1) + lag, (p * (d.abs() + lag) ** 2).sum(1)
     n = v / 256 + 48
     e_s = n * u + 2.0**-22 + 2 * u * d1
     ls = h + d1  # ln s = H + ln 2 u / s
@@ -412,7 +414,7 @@ def test_tied_shards_and_all_ignored():
     cut = 600
     s0 = mod.shard_logprob_stats(h, w[:cut].contiguous(), tokens, 0)
     s1 = mod.shard_logprob_stats(h, w[cut:].contiguous(), tokens, cut)
-    lp, ent, lse = mod.combine_logprob_stats(torch.stack([s0, s1]), tokens, 1001, IGN)
+    lp, ent, lse = mod.combine_logprob_stats(torch.stack([s0, s1]), tokens, 1001, IGN).unbind(0)
     check_tied(mod.TokenLogProbs(lp, ent), h, w, tokens)
     a, b = torch.randn(50, generator=g).cuda(), torch.randn(50, generator=g).cuda()
     parts, rows = [], []
