@@ -31,6 +31,12 @@ template <> __device__ __forceinline__ float from_f<float>(float v) { return v; 
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Packed pairs: one instruction for two fp32 operations.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
 // Eight consecutive elements as fp32 (16-byte vector loads / stores; the
 // pointer must be 16-byte aligned for 16-bit types, 32-byte for fp32).
 template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);

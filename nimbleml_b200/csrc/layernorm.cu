@@ -25,190 +25,347 @@ namespace {
 
 constexpr int64_t kLnMaxD = 8192;
 
-// A row's elements over the kW * 32 threads of its group, kV eights a thread:
-// eight q of thread t holds elements 8 (t + q T) .. + 7 (kVec: 16-byte
-// accesses), else elements t + (8 q + e) T for e = 0..7.
-template <int kW, bool kVec>
-struct RowMap {
-  static constexpr int T = 32 * kW;
-  __device__ static __forceinline__ int at(int t, int q, int e) {
-    return kVec ? 8 * (t + q * T) + e : t + (8 * q + e) * T;
+// Eight elements of a row as they come from memory.
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void set(int e, T x) { reinterpret_cast<T*>(v)[e] = x; }  // e known at compile time
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {
+    const T* p = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = make_float2(to_f<T>(p[2 * e]), to_f<T>(p[2 * e + 1]));
   }
 };
 
-template <typename E, int kW, int kV, bool kVec>
-__device__ __forceinline__ void load_row(const E* p, int t, int d, float (&v)[kV][8]) {
+// A row's elements over the T = kW * 32 threads of its group, eights a thread:
+// eight q of thread t holds elements 8 (t + q T) .. + 7 (kVec: 16-byte accesses),
+// else elements t + (8 q + e) T for e = 0..7.
+template <int kW, bool kVec>
+__device__ __forceinline__ int elem_at(int t, int q, int e) {
+  return kVec ? 8 * (t + q * 32 * kW) + e : t + (8 * q + e) * 32 * kW;
+}
+
+template <typename T, int kW, bool kVec>
+__device__ __forceinline__ void load_eight(const T* p, int t, int q, int d, Eight<T>& o) {
+  if constexpr (kVec) {
+    const int j = elem_at<kW, true>(t, q, 0);
+    if (j < d) o.load(p + j);
+    else o.zero();
+  } else {
 #pragma unroll
-  for (int q = 0; q < kV; ++q) {
-    if constexpr (kVec) {
-      const int j = RowMap<kW, true>::at(t, q, 0);
-      if (j < d) {
-        load8<E>(p + j, v[q]);
-      } else {
+    for (int e = 0; e < 8; ++e) {
+      const int j = elem_at<kW, false>(t, q, e);
+      o.set(e, j < d ? p[j] : from_f<T>(0.0f));
+    }
+  }
+}
+template <typename T, int kW, bool kVec>
+__device__ __forceinline__ void load_floats(const T* p, int t, int q, int d, float2 (&o)[4]) {
+  Eight<T> x;
+  load_eight<T, kW, kVec>(p, t, q, d, x);
+  x.get(o);
+}
+template <typename T, int kW, bool kVec>
+__device__ __forceinline__ void store_eight(T* p, int t, int q, int d, const float2 (&f)[4]) {
+  const float v[8] = {f[0].x, f[0].y, f[1].x, f[1].y, f[2].x, f[2].y, f[3].x, f[3].y};
+  if constexpr (kVec) {
+    const int j = elem_at<kW, true>(t, q, 0);
+    if (j < d) store8<T>(p + j, v);
+  } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[q][e] = 0.0f;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = RowMap<kW, false>::at(t, q, e);
-        v[q][e] = j < d ? to_f<E>(p[j]) : 0.0f;
-      }
+    for (int e = 0; e < 8; ++e) {
+      const int j = elem_at<kW, false>(t, q, e);
+      if (j < d) p[j] = from_f<T>(v[e]);
     }
   }
 }
 
-template <typename E, int kW, int kV, bool kVec>
-__device__ __forceinline__ void store_row(E* p, int t, int d, const float (&v)[kV][8]) {
-#pragma unroll
-  for (int q = 0; q < kV; ++q) {
-    if constexpr (kVec) {
-      const int j = RowMap<kW, true>::at(t, q, 0);
-      if (j < d) store8<E>(p + j, v[q]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = RowMap<kW, false>::at(t, q, e);
-        if (j < d) p[j] = from_f<E>(v[q][e]);
-      }
-    }
-  }
+// Barrier of the warps of one group (ids 1..15; id 0 is __syncthreads).
+__device__ __forceinline__ void group_barrier(int group, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
 }
 
-// Sum over the row's group of warps, the same bits in every thread. `red` holds
-// kW floats of this group; two buffers in turn need one barrier a sum.
+// Two sums over the row's group of kW warps, the same bits in every thread. `red`
+// holds kW pairs of this group; two buffers in turn need one barrier a sum.
 template <int kW>
-__device__ __forceinline__ float group_sum(float v, float* red) {
+__device__ __forceinline__ float2 group_sum(float2 v, float2* red, int group) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  for (int off = 16; off > 0; off >>= 1)
+    v = add2(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, off), __shfl_xor_sync(0xffffffffu, v.y, off)));
   if constexpr (kW > 1) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kW; ++w) v += red[w];
-  }
-  return v;
-}
-template <int kW>
-__device__ __forceinline__ float2 group_sum2(float2 v, float2* red) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, off);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, off);
-  }
-  if constexpr (kW > 1) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[(threadIdx.x >> 5) % kW] = v;
+    group_barrier(group, 32 * kW);
     v = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kW; ++w) {
-      v.x += red[w].x;
-      v.y += red[w].y;
+    for (int w = 0; w < kW; w += 2) {
+      const float4 two = *reinterpret_cast<const float4*>(red + w);
+      v = add2(v, add2(make_float2(two.x, two.y), make_float2(two.z, two.w)));
     }
   }
   return v;
 }
 
-// Rows per block: four one-warp rows, else one row of kW warps.
-__host__ __device__ constexpr int rows_per_block(int kW) { return kW == 1 ? 4 : 1; }
-__host__ __device__ constexpr int block_threads(int kW) { return 32 * kW * rows_per_block(kW); }
-
+// ------------------------------------------------------------------- forward
+// A group of kW warps has two rows, up to 32 elements of each a thread, which stay
+// in registers in their own type: rows of up to 1024 need one warp and no barrier.
+// Two rows share the loads of gamma and beta: one row a group was bound by the
+// L1 cache (fp32 parameters are twice the row's bytes; 115 us for 32768 x 4096
+// bf16 against 0.54 GB).
+__host__ __device__ constexpr int fwd_warps(int kW) { return kW > 8 ? kW : 8; }
 template <typename T, typename P, int kW, int kV, bool kVec>
-__global__ void __launch_bounds__(block_threads(kW))
+__global__ void __launch_bounds__(32 * fwd_warps(kW))
 layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma, const P* __restrict__ beta,
                      int64_t N, int d, float eps, T* __restrict__ y, float* __restrict__ out_mean,
                      float* __restrict__ out_rstd) {
-  constexpr int kRows = rows_per_block(kW);
-  __shared__ float red[2][kW];
-  const int t = threadIdx.x % (32 * kW);
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (32 * kW);
-  if (row >= N) return;  // whole warps; with kW > 1 a block has one row and never returns here
-  float v[kV][8];
-  load_row<T, kW, kV, kVec>(x + row * ldx, t, d, v);
-  float sum = 0.0f;
+  constexpr int kGroups = fwd_warps(kW) / kW;
+  __shared__ __align__(16) float2 red[2][fwd_warps(kW)];
+  const int t = threadIdx.x % (32 * kW), group = threadIdx.x / (32 * kW);
+  const int64_t row = 2 * (static_cast<int64_t>(blockIdx.x) * kGroups + group);
+  if (row >= N) return;  // whole groups
+  const bool two = row + 1 < N;
+  Eight<T> raw[2][kV];
 #pragma unroll
-  for (int q = 0; q < kV; ++q)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += v[q][e];
-  const float inv_d = 1.0f / static_cast<float>(d);
-  const float mean = group_sum<kW>(sum, red[0]) * inv_d;
-  float sq = 0.0f;
-#pragma unroll
-  for (int q = 0; q < kV; ++q)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[q][e] -= mean;
-      if (RowMap<kW, kVec>::at(t, q, e) < d) sq = fmaf(v[q][e], v[q][e], sq);
-    }
-  const float rstd = 1.0f / sqrtf(group_sum<kW>(sq, red[1]) * inv_d + eps);
-  float w[kV][8];
-  load_row<P, kW, kV, kVec>(gamma, t, d, w);
-#pragma unroll
-  for (int q = 0; q < kV; ++q)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[q][e] *= rstd * w[q][e];
-  if (beta) {
-    load_row<P, kW, kV, kVec>(beta, t, d, w);
-#pragma unroll
-    for (int q = 0; q < kV; ++q)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[q][e] += w[q][e];
+  for (int q = 0; q < kV; ++q) {
+    load_eight<T, kW, kVec>(x + row * ldx, t, q, d, raw[0][q]);
+    if (two) load_eight<T, kW, kVec>(x + (row + 1) * ldx, t, q, d, raw[1][q]);
+    else raw[1][q].zero();
   }
-  store_row<T, kW, kV, kVec>(y + row * d, t, d, v);
+  const float inv_d = 1.0f / static_cast<float>(d);
+  float2 sum[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int q = 0; q < kV; ++q) {
+      float2 v[4];
+      raw[k][q].get(v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[k] = add2(sum[k], v[e]);
+    }
+  float2 mean = group_sum<kW>(make_float2(sum[0].x + sum[0].y, sum[1].x + sum[1].y), red[0] + group * kW, group);
+  mean = mul2(mean, both(inv_d));
+  float2 sq[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float2 m = both(k ? -mean.y : -mean.x);
+#pragma unroll
+    for (int q = 0; q < kV; ++q) {
+      float2 v[4];
+      raw[k][q].get(v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 c = add2(v[e], m);
+        if (elem_at<kW, kVec>(t, q, 2 * e) >= d) c.x = 0.0f;
+        if (elem_at<kW, kVec>(t, q, 2 * e + 1) >= d) c.y = 0.0f;
+        sq[k] = fma2(c, c, sq[k]);
+      }
+    }
+  }
+  const float2 var =
+      mul2(group_sum<kW>(make_float2(sq[0].x + sq[0].y, sq[1].x + sq[1].y), red[1] + group * kW, group), both(inv_d));
+  const float2 rstd = make_float2(1.0f / sqrtf(var.x + eps), 1.0f / sqrtf(var.y + eps));
+#pragma unroll
+  for (int q = 0; q < kV; ++q) {
+    float2 w[4], b[4] = {both(0.0f), both(0.0f), both(0.0f), both(0.0f)};
+    load_floats<P, kW, kVec>(gamma, t, q, d, w);
+    if (beta) load_floats<P, kW, kVec>(beta, t, q, d, b);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && !two) break;
+      const float2 m = both(k ? -mean.y : -mean.x), r = both(k ? rstd.y : rstd.x);
+      float2 v[4];
+      raw[k][q].get(v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fma2(mul2(add2(v[e], m), r), w[e], b[e]);
+      store_eight<T, kW, kVec>(y + (row + k) * d, t, q, d, v);
+    }
+  }
   if (t == 0 && out_mean) {
-    out_mean[row] = mean;
-    out_rstd[row] = rstd;
+    out_mean[row] = mean.x;
+    out_rstd[row] = rstd.x;
+    if (two) {
+      out_mean[row + 1] = mean.y;
+      out_rstd[row + 1] = rstd.y;
+    }
   }
 }
 
-// grad_x, and per row group the sums over its rows of g xh and g (partial:
-// [groups][2][d]).
+// ------------------------------------------------------------------ backward
+// One block of 16 warps an SM in groups of kW; a group walks its rows, 8 kV
+// elements a thread, keeps the columns' sums of g xh and g in registers and writes
+// grad_x. With kVec a thread fetches its own part of the next rows into a ring in
+// shared memory with asynchronous copies: nobody else reads it, so the ring needs
+// no barrier, and the rows in flight hold no registers (loads into registers, one
+// row at a time, ran 32768 x 4096 bf16 in 238 us). 16 elements a thread and packed
+// arithmetic keep the row sums' share of the instructions small (8 elements and
+// single ones: 176 us, 34 instructions an element). At the end the block's groups
+// add up in order: partial is [blocks][2][d].
+constexpr int kBwdWarps = 16;
+constexpr int kBwdThreads = 32 * kBwdWarps;
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                   static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+
+// Rows in the ring: 128 KB of 16-bit rows, 192 KB of fp32 ones.
+template <typename T, int kV>
+__host__ __device__ constexpr int ring_rows() { return sizeof(T) * kV == 8 ? 3 : 4; }
+template <typename T, int kV>
+constexpr size_t ring_bytes() {
+  return sizeof(T) * 8 * kV * 2 * ring_rows<T, kV>() * kBwdThreads;
+}
+
 template <typename T, typename P, int kW, int kV, bool kVec>
-__global__ void __launch_bounds__(block_threads(kW))
+__global__ void __launch_bounds__(kBwdThreads)
 layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma,
                      const float* __restrict__ mean, const float* __restrict__ rstd, int64_t N, int d,
                      T* __restrict__ gx, float* __restrict__ partial) {
-  constexpr int kRows = rows_per_block(kW);
-  __shared__ float2 red[2][kW];
-  const int t = threadIdx.x % (32 * kW);
-  const int64_t group = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / (32 * kW);
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * kRows;
+  constexpr int kGroups = kBwdWarps / kW;
+  constexpr int kRing = ring_rows<T, kV>();
+  __shared__ __align__(16) float2 red[2][kBwdWarps];
+  extern __shared__ __align__(16) uint8_t dyn[];
+  const int t = threadIdx.x % (32 * kW), grp = threadIdx.x / (32 * kW);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + grp;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kGroups;
   const float inv_d = 1.0f / static_cast<float>(d);
-  float gm[kV][8], sg[kV][8], sb[kV][8];
-  load_row<P, kW, kV, kVec>(gamma, t, d, gm);
+  float2 gm[kV][4], sg[kV][4], sb[kV][4];
 #pragma unroll
-  for (int q = 0; q < kV; ++q)
+  for (int q = 0; q < kV; ++q) {
+    load_floats<P, kW, kVec>(gamma, t, q, d, gm[q]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sg[q][e] = sb[q][e] = 0.0f;
-  int buf = 0;
-  for (int64_t row = group; row < N; row += groups, buf ^= 1) {
-    float g[kV][8], h[kV][8];
-    load_row<T, kW, kV, kVec>(grad + row * d, t, d, g);
-    load_row<T, kW, kV, kVec>(x + row * ldx, t, d, h);
-    const float mu = mean[row], r = rstd[row];
-    float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int q = 0; q < kV; ++q)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        h[q][e] = (h[q][e] - mu) * r;  // g is zero behind the row's end
-        sb[q][e] += g[q][e];
-        sg[q][e] = fmaf(g[q][e], h[q][e], sg[q][e]);
-        g[q][e] *= gm[q][e];
-        s.x += g[q][e];
-        s.y = fmaf(g[q][e], h[q][e], s.y);
-      }
-    s = group_sum2<kW>(s, red[buf]);
-    const float a = s.x * inv_d, b = s.y * inv_d;
-#pragma unroll
-    for (int q = 0; q < kV; ++q)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) g[q][e] = r * (g[q][e] - fmaf(h[q][e], b, a));
-    store_row<T, kW, kV, kVec>(gx + row * d, t, d, g);
+    for (int e = 0; e < 4; ++e) sg[q][e] = sb[q][e] = both(0.0f);
   }
-  store_row<float, kW, kV, kVec>(partial + (group * 2) * d, t, d, sg);
-  store_row<float, kW, kV, kVec>(partial + (group * 2 + 1) * d, t, d, sb);
+  // Slot s of the ring: kV eights of grad, then of x; 16-byte pieces of
+  // neighbouring threads next to each other.
+  constexpr int kPieces = sizeof(T) / 2;  // of 16 bytes in an eight
+  auto slot = [&](int s, int which, int q, int piece) -> uint4* {
+    return reinterpret_cast<uint4*>(dyn) + (((s * 2 + which) * kV + q) * kPieces + piece) * kBwdThreads + threadIdx.x;
+  };
+  auto fetch = [&](int64_t row, int s) {
+    if constexpr (kVec) {
+      if (row < N) {
+#pragma unroll
+        for (int q = 0; q < kV; ++q) {
+          const int j = elem_at<kW, true>(t, q, 0);
+          if (j < d) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+              copy16(slot(s, 0, q, i), reinterpret_cast<const uint4*>(grad + row * d + j) + i);
+              copy16(slot(s, 1, q, i), reinterpret_cast<const uint4*>(x + row * ldx + j) + i);
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < kRing - 1; ++s) fetch(first + s * stride, s);
+  int s_now = 0, s_next = kRing - 1, turn = 0;
+  float mu_next = first < N ? mean[first] : 0.0f, r_next = first < N ? rstd[first] : 0.0f;
+  for (int64_t row = first; row < N; row += stride) {
+    const float mu = mu_next, r = r_next;
+    if (row + stride < N) {
+      mu_next = mean[row + stride];
+      r_next = rstd[row + stride];
+    }
+    float2 g[kV][4], h[kV][4];
+    if constexpr (kVec) {
+      fetch(row + (kRing - 1) * stride, s_next);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+#pragma unroll
+      for (int q = 0; q < kV; ++q) {
+        Eight<T> a, b;
+        if (elem_at<kW, true>(t, q, 0) < d) {
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            a.v[i] = *slot(s_now, 0, q, i);
+            b.v[i] = *slot(s_now, 1, q, i);
+          }
+        } else {
+          a.zero();
+          b.zero();
+        }
+        a.get(g[q]);
+        b.get(h[q]);
+      }
+      s_next = s_now;
+      s_now = s_now + 1 == kRing ? 0 : s_now + 1;
+    } else {
+#pragma unroll
+      for (int q = 0; q < kV; ++q) {
+        load_floats<T, kW, kVec>(grad + row * d, t, q, d, g[q]);
+        load_floats<T, kW, kVec>(x + row * ldx, t, q, d, h[q]);
+      }
+    }
+    float2 s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+    for (int q = 0; q < kV; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        h[q][e] = mul2(add2(h[q][e], both(-mu)), both(r));  // g is zero behind the row's end
+        sb[q][e] = add2(sb[q][e], g[q][e]);
+        sg[q][e] = fma2(g[q][e], h[q][e], sg[q][e]);
+        g[q][e] = mul2(g[q][e], gm[q][e]);
+        s1 = add2(s1, g[q][e]);
+        s2 = fma2(g[q][e], h[q][e], s2);
+      }
+    const float2 sums = group_sum<kW>(make_float2(s1.x + s1.y, s2.x + s2.y), red[turn] + grp * kW, grp);
+    turn ^= 1;
+    const float2 na = both(-sums.x * inv_d), nb = both(-sums.y * inv_d);
+#pragma unroll
+    for (int q = 0; q < kV; ++q) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[q][e] = mul2(both(r), add2(g[q][e], fma2(h[q][e], nb, na)));
+      store_eight<T, kW, kVec>(gx + row * d, t, q, d, g[q]);
+    }
+  }
+  if constexpr (kVec) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
+  if constexpr (kGroups == 1) {
+#pragma unroll
+    for (int q = 0; q < kV; ++q) {
+      store_eight<float, kW, kVec>(out, t, q, d, sg[q]);
+      store_eight<float, kW, kVec>(out + d, t, q, d, sb[q]);
+    }
+  } else {
+    // The groups' sums side by side, then added in the groups' order.
+    __syncthreads();  // every thread is done with its part of the ring
+    float* cols = reinterpret_cast<float*>(dyn);  // [kGroups][2][d], d <= 256 kW kV
+#pragma unroll
+    for (int q = 0; q < kV; ++q) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j0 = elem_at<kW, kVec>(t, q, 2 * e), j1 = elem_at<kW, kVec>(t, q, 2 * e + 1);
+        float* c = cols + grp * 2 * d;
+        if (j0 < d) {
+          c[j0] = sg[q][e].x;
+          c[d + j0] = sb[q][e].x;
+        }
+        if (j1 < d) {
+          c[j1] = sg[q][e].y;
+          c[d + j1] = sb[q][e].y;
+        }
+      }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < 2 * d; j += kBwdThreads) {
+      float s = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kGroups; ++k) s += cols[k * 2 * d + j];
+      out[j] = s;
+    }
+  }
 }
 
 // out[j] = sum over groups of partial[group][j], j over the 2 d columns of
@@ -235,36 +392,13 @@ layernorm_param_grad_kernel(const float* __restrict__ partial, int64_t groups, i
     grad_beta[j - d] = t;
 }
 
-// Warps a row and eights a thread for a row of d elements.
-struct RowShape {
-  int warps, eights;
-};
-RowShape fwd_shape(int64_t d) {
-  if (d <= 256) return {1, 1};
-  if (d <= 512) return {1, 2};
-  if (d <= 1024) return {4, 1};
-  if (d <= 2048) return {4, 2};
-  if (d <= 4096) return {8, 2};
-  return {8, 4};
-}
-RowShape bwd_shape(int64_t d) {
-  if (d <= 256) return {1, 1};
-  if (d <= 1024) return {4, 1};
-  if (d <= 2048) return {8, 1};
-  if (d <= 4096) return {16, 1};
-  return {16, 2};
-}
-// Row groups of the backward: enough blocks to fill the GPU, each with the
-// same number of rows up to one.
+// Blocks of the backward: enough to fill the GPU, each group with one row at least.
+int bwd_warps(int64_t d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 int64_t bwd_blocks(int64_t N, int64_t d) {
-  const RowShape sh = bwd_shape(d);
-  const int64_t per_sm = std::max<int64_t>(1, 1024 / block_threads(sh.warps));
-  const int64_t rows = rows_per_block(sh.warps);
-  return std::max<int64_t>(1, std::min<int64_t>((N + rows - 1) / rows, 148 * per_sm));
+  const int64_t groups = kBwdWarps / bwd_warps(d);
+  return std::max<int64_t>(1, std::min<int64_t>((N + groups - 1) / groups, 148));
 }
-size_t bwd_workspace(int64_t N, int64_t d) {
-  return sizeof(float) * 2 * static_cast<size_t>(bwd_blocks(N, d) * rows_per_block(bwd_shape(d).warps)) * d;
-}
+size_t bwd_workspace(int64_t N, int64_t d) { return sizeof(float) * 2 * static_cast<size_t>(bwd_blocks(N, d)) * d; }
 
 bool aligned16(std::initializer_list<const void*> ptrs) {
   for (const void* p : ptrs)
@@ -276,8 +410,8 @@ int check_norm(int64_t N, int64_t d, int64_t pitch, int dtype, int param_dtype) 
   if (!valid_dtype(dtype)) return fail(NIMBLE_ERR_INVALID_ARG, "bad dtype");
   if (param_dtype != dtype && param_dtype != NIMBLE_DTYPE_F32)
     return fail(NIMBLE_ERR_INVALID_ARG, "param_dtype must be the compute dtype or NIMBLE_DTYPE_F32");
-  if (N < 0 || d <= 0 || d > kLnMaxD)
-    return fail(NIMBLE_ERR_INVALID_ARG, "need n_rows >= 0 and 0 < d_model <= 8192");
+  if (N < 0 || N > INT32_MAX || d <= 0 || d > kLnMaxD)
+    return fail(NIMBLE_ERR_INVALID_ARG, "need 0 <= n_rows < 2^31 and 0 < d_model <= 8192");
   if (pitch < d) return fail(NIMBLE_ERR_INVALID_ARG, "row pitch < d_model");
   return NIMBLE_OK;
 }
@@ -304,25 +438,24 @@ extern "C" int nimble_layernorm_forward(const void* x, int64_t x_row_pitch, cons
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int d = static_cast<int>(d_model);
   const bool vec = d % 8 == 0 && (x_row_pitch * elem_size(dtype)) % 16 == 0 && aligned16({x, gamma, beta, y});
-  const RowShape sh = fwd_shape(d);
-  const int64_t blocks = (n_rows + rows_per_block(sh.warps) - 1) / rows_per_block(sh.warps);
-  if (blocks > INT32_MAX) return fail(NIMBLE_ERR_INVALID_ARG, "n_rows is too large for one call");
   NIMBLE_DISPATCH(dtype, T, with_param_type<T>(param_dtype, [&](auto tag) {
     using P = std::remove_cv_t<std::remove_pointer_t<decltype(tag)>>;
     auto go = [&](auto w, auto v) {
       constexpr int kW = decltype(w)::value, kV = decltype(v)::value;
+      const int64_t rows = 2 * (fwd_warps(kW) / kW);
+      const int64_t blocks = (n_rows + rows - 1) / rows;  // n_rows < 2^31, checked above
       auto kern = vec ? layernorm_fwd_kernel<T, P, kW, kV, true> : layernorm_fwd_kernel<T, P, kW, kV, false>;
-      kern<<<static_cast<unsigned>(blocks), block_threads(kW), 0, s>>>(
+      kern<<<static_cast<unsigned>(blocks), 32 * fwd_warps(kW), 0, s>>>(
           static_cast<const T*>(x), x_row_pitch, static_cast<const P*>(gamma), static_cast<const P*>(beta), n_rows, d,
           eps, static_cast<T*>(y), out_mean, out_rstd);
     };
     using std::integral_constant;
     if (d <= 256) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
     else if (d <= 512) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-    else if (d <= 1024) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (d <= 1024) go(integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (d <= 2048) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
     else if (d <= 4096) go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
-    else go(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    else go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
   }));
   NIMBLE_CUDA_TRY(cudaGetLastError());
   return NIMBLE_OK;
@@ -354,27 +487,32 @@ extern "C" int nimble_layernorm_backward(const void* grad, const void* x, int64_
     return fail(NIMBLE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
   float* partial = static_cast<float*>(workspace);
   const bool vec = d % 8 == 0 && (x_row_pitch * elem_size(dtype)) % 16 == 0 && aligned16({grad, x, gamma, grad_x});
-  const RowShape sh = bwd_shape(d);
   const int64_t blocks = bwd_blocks(n_rows, d);
+  cudaError_t err = cudaSuccess;
   NIMBLE_DISPATCH(dtype, T, with_param_type<T>(param_dtype, [&](auto tag) {
     using P = std::remove_cv_t<std::remove_pointer_t<decltype(tag)>>;
     auto go = [&](auto w, auto v) {
       constexpr int kW = decltype(w)::value, kV = decltype(v)::value;
       auto kern = vec ? layernorm_bwd_kernel<T, P, kW, kV, true> : layernorm_bwd_kernel<T, P, kW, kV, false>;
-      kern<<<static_cast<unsigned>(blocks), block_threads(kW), 0, s>>>(
+      // The ring, or the column sums of the block's groups where they are more.
+      const size_t smem = std::max(vec ? ring_bytes<T, kV>() : size_t(0), sizeof(float) * 2 * 8 * kV * kBwdThreads);
+      err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+      if (err != cudaSuccess) return;
+      kern<<<static_cast<unsigned>(blocks), kBwdThreads, smem, s>>>(
           static_cast<const T*>(grad), static_cast<const T*>(x), x_row_pitch, static_cast<const P*>(gamma), mean, rstd,
           n_rows, d, static_cast<T*>(grad_x), partial);
     };
     using std::integral_constant;
-    if (sh.warps == 1) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    else if (sh.warps == 4) go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    else if (sh.warps == 8) go(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    else if (sh.eights == 1) go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (d <= 256) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    else if (d <= 512) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    else if (d <= 1024) go(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else if (d <= 2048) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (d <= 4096) go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
     else go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
   }));
+  NIMBLE_CUDA_TRY(err);
   NIMBLE_CUDA_TRY(cudaGetLastError());
-  const int64_t groups = blocks * rows_per_block(sh.warps);
-  layernorm_param_grad_kernel<<<(2 * d + 31) / 32, 1024, 0, s>>>(partial, groups, d, grad_gamma, grad_beta);
+  layernorm_param_grad_kernel<<<(2 * d + 31) / 32, 1024, 0, s>>>(partial, blocks, d, grad_gamma, grad_beta);
   NIMBLE_CUDA_TRY(cudaGetLastError());
   return NIMBLE_OK;
 }

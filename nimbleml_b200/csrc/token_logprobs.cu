@@ -44,10 +44,6 @@ constexpr float kMinD = -1.0e4f;
 // weight is zero, and products with log2 e may overflow: weights are 1 or 0.
 constexpr float kHuge = 1.0e30f;
 
-// Packed pairs: one instruction for two fp32 operations.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-
 // Max of n vectors' logits, NaN left aside. 16-bit logits are compared in pairs
 // before they are widened.
 template <typename T, int n>
