@@ -359,13 +359,19 @@ NIMBLE_API int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int
                                                            int dtype, size_t* bytes);
 
 /* The same two numbers from hidden states and the tied matrix, without an
- * N x V buffer: statistics of one vocab shard, shard_stats (4, n_tokens) fp32 =
- * row max m, sum 2^d, sum d 2^d with d = s log2 e - fl(m log2 e), and the token's logit
- * (0 where the shard does not hold it). f16 / bf16, fp32 accumulate. */
+ * N x V buffer, on one vocab shard (f16 / bf16, fp32 accumulate). Writes, each
+ * where not null:
+ *   shard_stats (4, n_tokens) fp32: a reference logit f near the row's max,
+ *     sum 2^d, sum d 2^d with d = s log2 e - fl(f log2 e), and the token's logit
+ *     (0 where the shard does not hold it), for nimble_tied_logprobs_combine;
+ *   out_logprob, out_entropy, out_lse (n_tokens; all three or none): the results,
+ *     for a shard that is the whole vocabulary (v_offset 0). Ignored rows and bad
+ *     tokens as in nimble_token_logprobs_forward. */
 NIMBLE_API int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
                                             int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
-                                            int dtype, float* shard_stats, void* workspace, size_t workspace_bytes,
-                                            int* status, void* stream);
+                                            int dtype, int64_t ignore_index, float* shard_stats, float* out_logprob,
+                                            float* out_entropy, float* out_lse, void* workspace,
+                                            size_t workspace_bytes, int* status, void* stream);
 
 /* Merges the statistics of n_shards shards ([n_shards][4][n_tokens]) in order
  * into out_logprob, out_entropy and out_lse; ignored rows and bad tokens as in

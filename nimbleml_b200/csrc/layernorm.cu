@@ -121,7 +121,7 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* red, int group) {
 // bf16 against 0.54 GB).
 __host__ __device__ constexpr int fwd_warps(int kW) { return kW > 8 ? kW : 8; }
 template <typename T, typename P, int kW, int kV, bool kVec>
-__global__ void __launch_bounds__(32 * fwd_warps(kW))
+__global__ void __launch_bounds__(32 * fwd_warps(kW), kW == 16 ? 2 : 4)
 layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma, const P* __restrict__ beta,
                      int64_t N, int d, float eps, T* __restrict__ y, float* __restrict__ out_mean,
                      float* __restrict__ out_rstd) {
@@ -199,16 +199,12 @@ layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const P* __restrict__
 
 // ------------------------------------------------------------------ backward
 // One block of 16 warps an SM in groups of kW; a group walks its rows, 8 kV
-// elements a thread, keeps the columns' sums of g xh and g in registers and writes
-// grad_x. With kVec a thread fetches its own part of the next rows into a ring in
-// shared memory with asynchronous copies: nobody else reads it, so the ring needs
-// no barrier, and the rows in flight hold no registers (loads into registers, one
-// row at a time, ran 32768 x 4096 bf16 in 238 us). 16 elements a thread and packed
-// arithmetic keep the row sums' share of the instructions small (8 elements and
-// single ones: 176 us, 34 instructions an element). At the end the block's groups
-// add up in order: partial is [blocks][2][d].
-constexpr int kBwdWarps = 16;
-constexpr int kBwdThreads = 32 * kBwdWarps;
+// elements of a row a thread. With kVec a thread fetches its own part of the next
+// rows into a ring in shared memory with asynchronous copies: nobody else reads
+// it, so the ring needs no barrier, and the rows in flight hold no registers.
+constexpr int kWarps = 16;
+constexpr int kThreads = 32 * kWarps;
+int group_warps(int64_t d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
@@ -216,23 +212,49 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
                "l"(src)
                : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int n>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory"); }
+
+// A thread's eights in the ring, kPer of them a slot; the 16-byte pieces of
+// neighbouring threads lie next to each other.
+template <typename T, int kPer>
+struct Ring {
+  static constexpr int kPieces = sizeof(T) / 2;  // of 16 bytes in an eight
+  uint4* base;
+  __device__ __forceinline__ uint4* at(int slot, int k, int piece) const {
+    return base + ((slot * kPer + k) * kPieces + piece) * kThreads + threadIdx.x;
+  }
+  __device__ __forceinline__ void fetch(int slot, int k, const T* src) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) copy16(at(slot, k, i), reinterpret_cast<const uint4*>(src) + i);
+  }
+  __device__ __forceinline__ void read(int slot, int k, Eight<T>& o) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) o.v[i] = *at(slot, k, i);
+  }
+  static constexpr size_t bytes(int slots) { return size_t(16) * kPieces * kPer * slots * kThreads; }
+};
+
+// A group keeps the columns' sums of g xh and g in registers and writes grad_x, one
+// row at a time. (Loads into registers, one row ahead of nothing, ran 32768 x 4096
+// bf16 in 238 us; 8 elements a thread and single arithmetic in 176 us, 34
+// instructions an element, most of them for the row sums; the next row's mean and
+// rstd loaded when they are needed, 164 us.) At the end the block's groups add up in
+// order: partial is [blocks][2][d].
 
 // Rows in the ring: 128 KB of 16-bit rows, 192 KB of fp32 ones.
 template <typename T, int kV>
 __host__ __device__ constexpr int ring_rows() { return sizeof(T) * kV == 8 ? 3 : 4; }
-template <typename T, int kV>
-constexpr size_t ring_bytes() {
-  return sizeof(T) * 8 * kV * 2 * ring_rows<T, kV>() * kBwdThreads;
-}
 
 template <typename T, typename P, int kW, int kV, bool kVec>
-__global__ void __launch_bounds__(kBwdThreads)
+__global__ void __launch_bounds__(kThreads)
 layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_t ldx, const P* __restrict__ gamma,
                      const float* __restrict__ mean, const float* __restrict__ rstd, int64_t N, int d,
                      T* __restrict__ gx, float* __restrict__ partial) {
-  constexpr int kGroups = kBwdWarps / kW;
+  constexpr int kGroups = kWarps / kW;
   constexpr int kRing = ring_rows<T, kV>();
-  __shared__ __align__(16) float2 red[2][kBwdWarps];
+  __shared__ __align__(16) float2 red[2][kWarps];
   extern __shared__ __align__(16) uint8_t dyn[];
   const int t = threadIdx.x % (32 * kW), grp = threadIdx.x / (32 * kW);
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups + grp;
@@ -245,28 +267,20 @@ layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_
 #pragma unroll
     for (int e = 0; e < 4; ++e) sg[q][e] = sb[q][e] = both(0.0f);
   }
-  // Slot s of the ring: kV eights of grad, then of x; 16-byte pieces of
-  // neighbouring threads next to each other.
-  constexpr int kPieces = sizeof(T) / 2;  // of 16 bytes in an eight
-  auto slot = [&](int s, int which, int q, int piece) -> uint4* {
-    return reinterpret_cast<uint4*>(dyn) + (((s * 2 + which) * kV + q) * kPieces + piece) * kBwdThreads + threadIdx.x;
-  };
-  auto fetch = [&](int64_t row, int s) {
+  const Ring<T, 2 * kV> ring{reinterpret_cast<uint4*>(dyn)};  // a slot: kV eights of grad, then of x
+  auto fetch = [&](int64_t row, int slot) {
     if constexpr (kVec) {
       if (row < N) {
 #pragma unroll
         for (int q = 0; q < kV; ++q) {
           const int j = elem_at<kW, true>(t, q, 0);
           if (j < d) {
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-              copy16(slot(s, 0, q, i), reinterpret_cast<const uint4*>(grad + row * d + j) + i);
-              copy16(slot(s, 1, q, i), reinterpret_cast<const uint4*>(x + row * ldx + j) + i);
-            }
+            ring.fetch(slot, q, grad + row * d + j);
+            ring.fetch(slot, kV + q, x + row * ldx + j);
           }
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      copy_commit();
     }
   };
 #pragma unroll
@@ -282,16 +296,13 @@ layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_
     float2 g[kV][4], h[kV][4];
     if constexpr (kVec) {
       fetch(row + (kRing - 1) * stride, s_next);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+      copy_wait<kRing - 1>();
 #pragma unroll
       for (int q = 0; q < kV; ++q) {
         Eight<T> a, b;
         if (elem_at<kW, true>(t, q, 0) < d) {
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            a.v[i] = *slot(s_now, 0, q, i);
-            b.v[i] = *slot(s_now, 1, q, i);
-          }
+          ring.read(s_now, q, a);
+          ring.read(s_now, kV + q, b);
         } else {
           a.zero();
           b.zero();
@@ -330,7 +341,7 @@ layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_
       store_eight<T, kW, kVec>(gx + row * d, t, q, d, g[q]);
     }
   }
-  if constexpr (kVec) asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if constexpr (kVec) copy_wait<0>();
   float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * d;
   if constexpr (kGroups == 1) {
 #pragma unroll
@@ -359,7 +370,7 @@ layernorm_bwd_kernel(const T* __restrict__ grad, const T* __restrict__ x, int64_
       }
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < 2 * d; j += kBwdThreads) {
+    for (int j = threadIdx.x; j < 2 * d; j += kThreads) {
       float s = 0.0f;
 #pragma unroll
       for (int k = 0; k < kGroups; ++k) s += cols[k * 2 * d + j];
@@ -393,9 +404,8 @@ layernorm_param_grad_kernel(const float* __restrict__ partial, int64_t groups, i
 }
 
 // Blocks of the backward: enough to fill the GPU, each group with one row at least.
-int bwd_warps(int64_t d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
 int64_t bwd_blocks(int64_t N, int64_t d) {
-  const int64_t groups = kBwdWarps / bwd_warps(d);
+  const int64_t groups = kWarps / group_warps(d);
   return std::max<int64_t>(1, std::min<int64_t>((N + groups - 1) / groups, 148));
 }
 size_t bwd_workspace(int64_t N, int64_t d) { return sizeof(float) * 2 * static_cast<size_t>(bwd_blocks(N, d)) * d; }
@@ -495,10 +505,10 @@ extern "C" int nimble_layernorm_backward(const void* grad, const void* x, int64_
       constexpr int kW = decltype(w)::value, kV = decltype(v)::value;
       auto kern = vec ? layernorm_bwd_kernel<T, P, kW, kV, true> : layernorm_bwd_kernel<T, P, kW, kV, false>;
       // The ring, or the column sums of the block's groups where they are more.
-      const size_t smem = std::max(vec ? ring_bytes<T, kV>() : size_t(0), sizeof(float) * 2 * 8 * kV * kBwdThreads);
+      const size_t smem = std::max(vec ? Ring<T, 2 * kV>::bytes(ring_rows<T, kV>()) : size_t(0), sizeof(float) * 2 * 8 * kV * kThreads);
       err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
       if (err != cudaSuccess) return;
-      kern<<<static_cast<unsigned>(blocks), kBwdThreads, smem, s>>>(
+      kern<<<static_cast<unsigned>(blocks), kThreads, smem, s>>>(
           static_cast<const T*>(grad), static_cast<const T*>(x), x_row_pitch, static_cast<const P*>(gamma), mean, rstd,
           n_rows, d, static_cast<T*>(grad_x), partial);
     };

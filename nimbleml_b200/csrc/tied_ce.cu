@@ -37,6 +37,7 @@
 
 #include "nimbleml_tied_ce.h"
 #include "common.cuh"
+#include "elementwise.cuh"
 #include "sm100_ptx.cuh"
 
 namespace nimble {
@@ -62,7 +63,6 @@ constexpr int kStagesPair = 6;
 // Wide single-CTA tiles: 32 KiB of A + 32 KiB of B per stage.
 constexpr int kStagesWide = 3;
 constexpr int kSmemBytesPair = kStagesPair * (kABytes + kBBytes / 2) + kStoreBytes + 1024 + 256;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // EPI_LP_FWD / EPI_LP_GRAD are the cross-entropy epilogues of the per-token log
 // probabilities: the forward also sums d 2^d (d = (s - max) log2 e) for the
@@ -99,6 +99,10 @@ struct EpiParams {
   float alpha_mult;
   int accum_out;
   int* status;
+  // Split contraction (kSplit): the tiles' K blocks are cut into k_splits runs,
+  // and run s reads src and writes out s * split_stride elements further.
+  int k_splits;
+  int64_t split_stride;
 };
 
 template <typename T> struct ElemInfo;
@@ -170,7 +174,10 @@ __device__ __forceinline__ void store_out_elem(void* p, int64_t i, int dt, float
 // share the B tile, accumulating into all 512 TMEM columns: a third fewer
 // operand bytes per FLOP than 128 x 256 tiles, but the epilogue of a tile no
 // longer overlaps the next tile's MMAs.
-template <typename T, int EPI, bool kAMN, bool kBMN, int kCG, bool kWide = false>
+//
+// kSplit (EPI_STORE) cuts the contraction into ep.k_splits runs with a partial
+// result each, for products with too few tiles to fill the GPU.
+template <typename T, int EPI, bool kAMN, bool kBMN, int kCG, bool kWide = false, bool kSplit = false>
 __global__ void __launch_bounds__(kThreads, 1)
 tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                   const __grid_constant__ CUtensorMap tmC, int M, int N, int K, int group_m, EpiParams ep) {
@@ -204,8 +211,16 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
   const int lane = threadIdx.x & 31;
   const int m_tiles = (M + kTileM - 1) / kTileM;
   const int n_tiles = (N + kBN - 1) / kBN;
-  const int tiles = m_tiles * n_tiles;
-  const int k_blocks = (K + kBK - 1) / kBK;
+  const int plane = m_tiles * n_tiles;
+  const int tiles = kSplit ? plane * ep.k_splits : plane;
+  const int k_blocks_all = (K + kBK - 1) / kBK;
+  // Unit t is tile t % plane of run t / plane: K blocks [k_begin, k_end).
+  auto k_begin = [&](int t) {
+    return kSplit ? static_cast<int>(static_cast<int64_t>(k_blocks_all) * (t / plane) / ep.k_splits) : 0;
+  };
+  auto k_end = [&](int t) {
+    return kSplit ? static_cast<int>(static_cast<int64_t>(k_blocks_all) * (t / plane + 1) / ep.k_splits) : k_blocks_all;
+  };
   const uint32_t rank = kCG == 2 ? ptx::cluster_ctarank() : 0u;
   const bool leader = rank == 0;
   const int unit0 = blockIdx.x / kCG;       // this CTA's first tile
@@ -249,10 +264,11 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       };
       for (int t = unit0; t < tiles && ok; t += units) {
         int mb, nb;
-        tile_coords(t, m_tiles, n_tiles, group_m, mb, nb);
+        tile_coords(kSplit ? t % plane : t, m_tiles, n_tiles, group_m, mb, nb);
         const int a_row0 = mb * kTileM + static_cast<int>(rank) * kBM;
         const int b_row0 = nb * kBN + static_cast<int>(rank) * kBRows;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        const int kb1 = k_end(t);
+        for (int kb = k_begin(t); kb < kb1; ++kb) {
           if (!ptx::mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) { ok = false; break; }
           // The even CTA's full barrier counts both CTAs' bytes.
           if (leader) ptx::mbar_arrive_expect_tx(&full_bar[stage], kCG * (kABytesCta + kBBytesCta));
@@ -308,7 +324,8 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
         if (!ptx::mbar_wait(&tempty_bar[acc], aphase ^ 1, abort_flag)) { ok = false; break; }
         ptx::tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * kBN;
-        for (int kb = 0; kb < k_blocks; ++kb) {
+        const int kb0 = k_begin(t), kb1 = k_end(t);
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!ptx::mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
           ptx::tc_fence_after();
           const uint32_t a_addr = ptx::smem_u32(sA + stage * kABytesCta);
@@ -318,13 +335,13 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 #pragma unroll
           for (int k = 0; k < kKSteps; ++k) {
             if constexpr (kCG == 2)
-              ptx::umma_pair<kTF32>(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, (kb | k) != 0 ? 1u : 0u);
+              ptx::umma_pair<kTF32>(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
             else
-              ptx::umma<kTF32>(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, (kb | k) != 0 ? 1u : 0u);
+              ptx::umma<kTF32>(d_tmem, adesc + kAStep * k, bdesc + kBStep * k, idesc, ((kb - kb0) | k) != 0 ? 1u : 0u);
             if constexpr (kWide) {
               // Second M block: A rows 128..255 sit 16 KiB further in the stage.
               ptx::umma<kTF32>(d_tmem + kBN, adesc + (kABytes >> 4) + kAStep * k, bdesc + kBStep * k, idesc,
-                               (kb | k) != 0 ? 1u : 0u);
+                               ((kb - kb0) | k) != 0 ? 1u : 0u);
             }
           }
           // Frees this stage in both CTAs once the MMAs have read it.
@@ -372,7 +389,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     int store_seq = 0;  // G staging stores issued by this warp
     for (int t = unit0; t < tiles; t += units, ++it) {
       int mb, nb;
-      tile_coords(t, m_tiles, n_tiles, group_m, mb, nb);
+      tile_coords(kSplit ? t % plane : t, m_tiles, n_tiles, group_m, mb, nb);
       const int acc = kWide ? 0 : (it & 1);
       const uint32_t aphase = kWide ? (it & 1) : ((it >> 1) & 1);
       bool ok = ptx::mbar_wait(&tfull_bar[acc], aphase, abort_flag);
@@ -521,7 +538,9 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           }
           ++store_seq;
         }
-      } else {  // EPI_STORE
+      } else {  // EPI_STORE (split: fp32 out)
+        const int64_t split_at = kSplit ? t / plane * ep.split_stride : 0;
+        const bool no_run = kSplit && k_begin(t) == k_end(t);  // nothing was accumulated
 #pragma unroll 1
         for (int c = c_begin; c < c_end; ++c) {
           if (c * 32 >= ncols) break;
@@ -535,10 +554,10 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           const int nv = min(32, ncols - c * 32);
           float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          for (int j = 0; j < 32; ++j) v[j] = no_run ? 0.0f : __uint_as_float(r[j]);
           if (nv == 32) {
             if (ep.src) {
-              const float4* s4 = reinterpret_cast<const float4*>(ep.src + row * ep.ld_src + col);
+              const float4* s4 = reinterpret_cast<const float4*>(ep.src + split_at + row * ep.ld_src + col);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 const float4 a = s4[q];
@@ -548,7 +567,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] *= alpha;
             if (ep.out_dtype == NIMBLE_DTYPE_F32) {
-              float4* o4 = reinterpret_cast<float4*>(static_cast<float*>(ep.out) + row * ep.ld_out + col);
+              float4* o4 = reinterpret_cast<float4*>(static_cast<float*>(ep.out) + split_at + row * ep.ld_out + col);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 float4 o = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -596,9 +615,9 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
             for (int j = 0; j < 32; ++j) {
               if (j >= nv) break;
               float x = v[j];
-              if (ep.src) x += ep.src[row * ep.ld_src + col + j];
+              if (ep.src) x += ep.src[split_at + row * ep.ld_src + col + j];
               x *= alpha;
-              const int64_t oi = row * ep.ld_out + col + j;
+              const int64_t oi = split_at + row * ep.ld_out + col + j;
               if (ep.accum_out) x += load_out_elem(ep.out, oi, ep.out_dtype);
               store_out_elem(ep.out, oi, ep.out_dtype, x);
             }
@@ -811,6 +830,7 @@ const int g_wide = [] {
   return m == 1 ? 15 : m;
 }();
 constexpr int kSmemBytesWide = kStagesWide * (2 * kABytes + kBBytes) + kStoreBytes + 1024 + 256;
+constexpr bool is_lp(int epi) { return epi == EPI_LP_FWD || epi == EPI_LP_GRAD; }
 template <int EPI, bool kAMN>
 constexpr int gemm_kind_bit() {
   return (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) ? 1 : (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) ? 2 : kAMN ? 4 : 8;
@@ -907,7 +927,9 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
     cfg.numAttrs = 1;
     NIMBLE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, static_cast<int>(M), static_cast<int>(N),
                                        static_cast<int>(K), group_m, ep));
-  } else if (g_wide & gemm_kind_bit<EPI, kAMN>()) {
+  } else if ((g_wide & gemm_kind_bit<EPI, kAMN>()) && !(is_lp(EPI) && M <= kBM)) {
+    // (Log probabilities of at most 128 tokens fill half a wide tile and are
+    // bound by reading the weights: 128 x 256 tiles, twice as many.)
     auto kern = tc_gemm_tn_kernel<T, EPI, kAMN, kBMN, 1, true>;
     NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesWide));
     const int64_t tiles = ((M + 2 * kBM - 1) / (2 * kBM)) * ((N + kBN - 1) / kBN);
@@ -942,6 +964,33 @@ int gemm_dispatch(int dtype, const void* A, int64_t lda, const void* B, int64_t 
         return launch_gemm<float, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
   }
   return fail(NIMBLE_ERR_INVALID_ARG, "unknown dtype");
+}
+
+// grad_hidden's product G[M x K] . E[K x N] with the contraction cut into ep.k_splits
+// runs (16-bit operands, 256 x 256 tiles), fp32 partial results.
+template <typename T>
+int launch_split(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, int dtype,
+                 const EpiParams& ep, cudaStream_t stream) {
+  DevInfo di;
+  if (int rc = device_info(&di)) return rc;
+  CUtensorMap ma, mb;
+  if (int rc = make_operand_map(&ma, A, dtype, false, K, M, lda, kBM)) return rc;
+  if (int rc = make_operand_map(&mb, B, dtype, true, K, N, ldb, kBN)) return rc;
+  auto kern = tc_gemm_tn_kernel<T, EPI_STORE, false, true, 1, true, true>;
+  NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesWide));
+  const int64_t units = ((M + 2 * kBM - 1) / (2 * kBM)) * ((N + kBN - 1) / kBN) * ep.k_splits;
+  if (units > INT32_MAX) return fail(NIMBLE_ERR_INVALID_ARG, "too many tiles");
+  kern<<<static_cast<int>(std::min<int64_t>(units, di.sms)), kThreads, kSmemBytesWide, stream>>>(
+      ma, mb, ma, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), g_group_m, ep);
+  NIMBLE_CUDA_TRY(cudaGetLastError());
+  return NIMBLE_OK;
+}
+// Runs for the grad_hidden product of n_tokens x d_model over `cols` columns: one
+// where its 256 x 256 tiles fill the 148 SMs, else as many as do, each of 8 K
+// blocks (512 columns) or more.
+int dh_splits(int64_t n_tokens, int64_t d_model, int64_t cols) {
+  const int64_t tiles = std::max<int64_t>(1, (n_tokens + 255) / 256 * ((d_model + 255) / 256));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({148 / tiles, 16, cols / 512})));
 }
 
 int launch_round(const float* src, float* dst, int64_t n, cudaStream_t s) {
@@ -1140,10 +1189,11 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
                   const float* alpha_den, float alpha_mult, const void* h, const void* E, int64_t n_tokens,
                   int64_t d_model, int64_t v_local, int64_t v_offset, int dtype, void* grad_hidden,
                   int grad_hidden_dtype, void* grad_weights, int grad_weights_dtype, int accumulate_grad_weights,
-                  int* status, cudaStream_t s, void* dh_done_event, int last_de_max_ctas, float capped_fraction) {
+                  int* status, cudaStream_t s, void* dh_done_event, int last_de_max_ctas, float capped_fraction,
+                  int splits = 1) {
   const int64_t es = elem_size(dtype);
   void* g = ws + L.g;
-  float* dh_acc = L.n_slabs > 1 ? reinterpret_cast<float*>(ws + L.dh) : nullptr;
+  float* dh_acc = L.n_slabs > 1 || splits > 1 ? reinterpret_cast<float*>(ws + L.dh) : nullptr;
   for (int64_t sl = 0; sl < L.n_slabs; ++sl) {
     const int64_t c0 = sl * L.slab;
     const int64_t vc = std::min<int64_t>(L.slab, v_local - c0);
@@ -1178,6 +1228,19 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
       if (!grad_hidden) return NIMBLE_OK;
       EpiParams eh{};
       eh.status = status;
+      if (splits > 1) {
+        // Partial sums of each run over all slabs; split_sum_kernel adds the runs.
+        eh.out = dh_acc;
+        eh.out_dtype = NIMBLE_DTYPE_F32;
+        eh.alpha_mult = 1.0f;
+        eh.ld_out = eh.ld_src = d_model;
+        eh.src = sl > 0 ? dh_acc : nullptr;
+        eh.k_splits = splits;
+        eh.split_stride = n_tokens * d_model;
+        return dtype == NIMBLE_DTYPE_F16
+                   ? launch_split<__half>(g, L.slab, E_sl, d_model, n_tokens, d_model, vc, dtype, eh, s)
+                   : launch_split<__nv_bfloat16>(g, L.slab, E_sl, d_model, n_tokens, d_model, vc, dtype, eh, s);
+      }
       if (last) {
         eh.out = grad_hidden;
         eh.out_dtype = grad_hidden_dtype;
@@ -1416,45 +1479,340 @@ extern "C" int nimble_tied_logits_backward(const void* grad_logits, int64_t grad
 namespace nimble {
 namespace {
 
-// Merges the per-tile (max, sum 2^d, sum d 2^d) of each token into the shard's
-// statistics (4, M); the fourth row is the token's logit if the shard owns it.
-// Threads of a column of the block take every kReduceGroups-th tile of 32
-// neighbouring tokens (coalesced), then a fixed-order merge in shared memory.
-constexpr int kReduceGroups = 16;
+// Merges the per-tile (reference f, sum 2^d, sum d 2^d) of each token: the shard's
+// statistics (4, M), the fourth row the token's logit if the shard owns it, and,
+// where `logp` is given, the results of a shard that is the whole vocabulary. The
+// threads of a column of the block take every kReduceGroups-th tile of 32
+// neighbouring tokens (coalesced, four tiles in flight), then a fixed-order merge
+// in shared memory.
+constexpr int kReduceGroups = 32;
+struct LpOut {
+  float* stats;  // (4, M) or null
+  float* logp;   // (M) each, or null
+  float* entropy;
+  float* lse;
+};
+struct LpStats {
+  float f = -INFINITY, s = 0.0f, u = 0.0f;
+  __device__ __forceinline__ void merge(float f2, float s2, float u2) {
+    // The references are f log2 e rounded to fp32, as in the epilogue.
+    const float fn = fmaxf(f, f2);
+    const float d1 = f == fn ? 0.0f : fmaxf(__fmul_rn(f, kLog2e) - __fmul_rn(fn, kLog2e), kMinD);
+    const float d2 = f2 == fn ? 0.0f : fmaxf(__fmul_rn(f2, kLog2e) - __fmul_rn(fn, kLog2e), kMinD);
+    const float w1 = ptx::ex2(d1), w2 = ptx::ex2(d2);
+    u = (u + s * d1) * w1 + (u2 + s2 * d2) * w2;
+    s = s * w1 + s2 * w2;
+    f = fn;
+  }
+};
 __global__ void __launch_bounds__(32 * kReduceGroups)
 lp_row_reduce_kernel(const float2* __restrict__ part, const float* __restrict__ part_u, int n_parts,
                      const float* __restrict__ tgt, const int64_t* __restrict__ tokens, int64_t M, int64_t v_offset,
-                     int64_t v_local, float* __restrict__ stats) {
+                     int64_t v_local, int64_t ignore_index, LpOut out, int* status) {
   __shared__ float sm[3][kReduceGroups][32];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  float m = -INFINITY, s = 0.0f, u = 0.0f;
-  auto merge = [&](float m2, float s2, float u2) {
-    const float mn = fmaxf(m, m2);
-    // The reference points are m log2 e rounded to fp32, as in the epilogue.
-    const float d1 = m == mn ? 0.0f : fmaxf(__fmul_rn(m, kLog2e) - __fmul_rn(mn, kLog2e), kMinD);
-    const float d2 = m2 == mn ? 0.0f : fmaxf(__fmul_rn(m2, kLog2e) - __fmul_rn(mn, kLog2e), kMinD);
-    const float f1 = ptx::ex2(d1), f2 = ptx::ex2(d2);
-    u = (u + s * d1) * f1 + (u2 + s2 * d2) * f2;
-    s = s * f1 + s2 * f2;
-    m = mn;
-  };
-  if (row < M)
-    for (int t = grp; t < n_parts; t += kReduceGroups) {
-      const float2 p = part[static_cast<int64_t>(t) * M + row];
-      merge(p.x, p.y, part_u[static_cast<int64_t>(t) * M + row]);
+  LpStats a;
+  if (row < M) {
+    constexpr int kU = 4;
+    for (int t0 = grp; t0 < n_parts; t0 += kU * kReduceGroups) {
+      float2 p[kU];
+      float u[kU];
+#pragma unroll
+      for (int i = 0; i < kU; ++i) {
+        const int64_t t = t0 + i * kReduceGroups;
+        p[i] = t < n_parts ? part[t * M + row] : make_float2(-INFINITY, 0.0f);
+        u[i] = t < n_parts ? part_u[t * M + row] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kU; ++i) a.merge(p[i].x, p[i].y, u[i]);
     }
-  sm[0][grp][lane] = m;
-  sm[1][grp][lane] = s;
-  sm[2][grp][lane] = u;
+  }
+  sm[0][grp][lane] = a.f;
+  sm[1][grp][lane] = a.s;
+  sm[2][grp][lane] = a.u;
   __syncthreads();
   if (grp != 0 || row >= M) return;
-  for (int g = 1; g < kReduceGroups; ++g) merge(sm[0][g][lane], sm[1][g][lane], sm[2][g][lane]);
-  stats[row] = m;
-  stats[M + row] = s;
-  stats[2 * M + row] = u;
+  for (int g = 1; g < kReduceGroups; ++g) a.merge(sm[0][g][lane], sm[1][g][lane], sm[2][g][lane]);
   const int64_t tok = tokens[row];
-  stats[3 * M + row] = (tok >= v_offset && tok < v_offset + v_local) ? tgt[row] : 0.0f;
+  const bool mine = tok >= v_offset && tok < v_offset + v_local;
+  const float x = mine ? tgt[row] : 0.0f;
+  if (out.stats) {
+    out.stats[row] = a.f;
+    out.stats[M + row] = a.s;
+    out.stats[2 * M + row] = a.u;
+    out.stats[3 * M + row] = x;
+  }
+  if (out.logp) {
+    if (tok == ignore_index) {
+      out.logp[row] = out.entropy[row] = out.lse[row] = 0.0f;
+      return;
+    }
+    if (!mine && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
+    const float ls = logf(a.s), ln2 = 0.6931471805599453f;
+    const float rel = ls - ln2 * fmaf(a.f, kLog2e, -__fmul_rn(a.f, kLog2e));  // lse - f
+    out.logp[row] = mine ? (x - a.f) - rel : __int_as_float(0x7fc00000);
+    out.entropy[row] = ls - ln2 * (a.u / a.s);
+    out.lse[row] = a.f + rel;
+  }
+}
+
+// Forward for at most 32 tokens: reading the weights once is all the work, so the
+// operands change places. A tile is 128 vocabulary rows (M, the TMEM lanes) against
+// kNP padded tokens (N), which keeps all but the weights out of the loads, and every
+// SM has an equal run of vocabulary rows in steps of 32. A lane keeps the running
+// statistics of its vocabulary rows for every token in registers, merged over the
+// lanes once at the end. (With 256 x 256 tiles, 7 tokens x 50257 x 1024 took 37 us:
+// the SMs with two tiles of 197 set the time, and the padding to 256 tokens filled
+// half of each stage.)
+constexpr int kDecThreads = 192;  // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+template <int kNP>
+constexpr int dec_stages() { return kNP == 16 ? 11 : 10; }
+template <int kNP>
+constexpr int dec_smem() { return dec_stages<kNP>() * (kABytes + kNP * kBKBytes) + 4 * kNP * 16 + 1024 + 512; }
+
+template <typename T, int kNP>
+__global__ void __launch_bounds__(kDecThreads, 1)
+lp_decode_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmH, int n_tokens, int V,
+                 int K, const int64_t* __restrict__ tokens, int64_t v_offset, float2* __restrict__ part,
+                 float* __restrict__ part_u, float* __restrict__ tgt, int* status) {
+  constexpr int kS = kNP == 16 ? 11 : 10;
+  constexpr int kBBytesDec = kNP * kBKBytes;
+  constexpr int kBK = kBKBytes / sizeof(T);
+  constexpr int kCols = 2 * kNP;  // two accumulators; a power of two >= 32
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kS * kABytes;
+  float4* sMerge = reinterpret_cast<float4*>(sB + kS * kBBytesDec);  // [4 warps][kNP]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sMerge + 4 * kNP);
+  uint64_t* empty_bar = full_bar + kS;
+  uint64_t* tfull_bar = empty_bar + kS;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int s_tok[kNP];  // the tokens' rows in this shard, -1: another's
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // This block's vocabulary rows, in whole chunks of 32.
+  const int chunks = (V + 31) / 32;
+  const int chunk0 = static_cast<int>(static_cast<int64_t>(chunks) * blockIdx.x / gridDim.x);
+  const int chunk1 = static_cast<int>(static_cast<int64_t>(chunks) * (blockIdx.x + 1) / gridDim.x);
+  const int tiles = (chunk1 - chunk0 + 3) / 4;
+  const int k_blocks = (K + kBK - 1) / kBK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kS; ++s) {
+      ptx::mbar_init(&full_bar[s], 1);
+      ptx::mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(&tfull_bar[a], 1);
+      ptx::mbar_init(&tempty_bar[a], 4);
+    }
+    ptx::mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  if (threadIdx.x < kNP) {
+    const int64_t rel = static_cast<int>(threadIdx.x) < n_tokens ? tokens[threadIdx.x] - v_offset : -1;
+    s_tok[threadIdx.x] = rel >= 0 && rel < V ? static_cast<int>(rel) : -1;
+  }
+  if (warp == 1) ptx::tmem_alloc_cg<1>(tmem_slot, kCols);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      ptx::prefetch_tmap(&tmW);
+      ptx::prefetch_tmap(&tmH);
+      int stage = 0;
+      uint32_t phase = 0, issued = 0;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int c0 = chunk0 + 4 * i;
+        const int boxes = min(4, chunk1 - c0);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!ptx::mbar_wait(&empty_bar[stage], phase ^ 1, abort_flag)) { ok = false; break; }
+          ptx::mbar_arrive_expect_tx(&full_bar[stage], boxes * (kABytes / 4) + kBBytesDec);
+          for (int b = 0; b < boxes; ++b)
+            ptx::tma_load_2d(sA + stage * kABytes + b * (kABytes / 4), &tmW, &full_bar[stage], kb * kBK, (c0 + b) * 32);
+          ptx::tma_load_2d(sB + stage * kBBytesDec, &tmH, &full_bar[stage], kb * kBK, 0);
+          issued |= 1u << stage;
+          if (++stage == kS) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {
+        // Let every load already issued land before the block can exit.
+        for (int s = 0; s < kS; ++s) {
+          if (!(issued & (1u << s))) continue;
+          const uint32_t par = (s < stage) ? phase : (phase ^ 1);
+          const uint64_t t0 = ptx::globaltimer_ns();
+          while (!ptx::mbar_try_wait(&full_bar[s], par) && ptx::globaltimer_ns() - t0 < ptx::kWaitLimitNs) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = ptx::idesc_f32acc(ElemInfo<T>::kFmt, kBM, kNP);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int i = 0; i < tiles && ok; ++i) {
+        const int acc = i & 1;
+        if (!ptx::mbar_wait(&tempty_bar[acc], ((i >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        ptx::tc_fence_after();
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          if (!ptx::mbar_wait(&full_bar[stage], phase, abort_flag)) { ok = false; break; }
+          ptx::tc_fence_after();
+          // Rows behind a short tile's boxes hold what an earlier tile left:
+          // their results are not read.
+          const uint64_t adesc = ptx::sdesc_k_sw128(ptx::smem_u32(sA + stage * kABytes));
+          const uint64_t bdesc = ptx::sdesc_k_sw128(ptx::smem_u32(sB + stage * kBBytesDec));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            ptx::umma<false>(tmem_base + acc * kNP, adesc + 2 * k, bdesc + 2 * k, idesc, (kb | k) != 0 ? 1u : 0u);
+          ptx::umma_commit(&empty_bar[stage]);
+          if (++stage == kS) { stage = 0; phase ^= 1; }
+        }
+        if (ok) ptx::umma_commit(&tfull_bar[acc]);
+      }
+      if (!ok) {
+        ptx::umma_commit(drain_bar);
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (!ptx::mbar_try_wait(drain_bar, 0) && ptx::globaltimer_ns() - t0 < ptx::kWaitLimitNs) {
+        }
+      }
+    }
+  } else {
+    const int wq = warp & 3;  // TMEM lane quarter: chunk wq of a tile
+    float f[kNP], s[kNP], u[kNP];
+#pragma unroll
+    for (int j = 0; j < kNP; ++j) {
+      f[j] = -INFINITY;
+      s[j] = u[j] = 0.0f;
+    }
+    for (int i = 0; i < tiles; ++i) {
+      const int acc = i & 1;
+      bool ok = ptx::mbar_wait(&tfull_bar[acc], (i >> 1) & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      uint32_t r[kNP];
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(wq * 32) << 16) + acc * kNP;
+      if constexpr (kNP == 16) ptx::tmem_ld_16cols(taddr, r);
+      else ptx::tmem_ld_32cols(taddr, r);
+      ptx::tmem_wait_ld();
+      ptx::tmem_fence_regs(r);
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&tempty_bar[acc]);
+      const int chunk = chunk0 + 4 * i + wq;
+      const int row = chunk * 32 + lane;
+      if (chunk < chunk1 && row < V) {
+#pragma unroll
+        for (int j = 0; j < kNP; ++j) {
+          const float v = __uint_as_float(r[j]);
+          float ref = __fmul_rn(f[j], kLog2e);
+          float d = fmaf(v, kLog2e, -ref);
+          if (!(d <= 16.0f)) {  // the first logit, or one far above the reference
+            const float next = __fmul_rn(v, kLog2e);
+            const float dm = fmaxf(ref - next, kMinD);
+            const float w = ptx::ex2(dm);
+            u[j] = (u[j] + s[j] * dm) * w;
+            s[j] *= w;
+            f[j] = v;
+            d = fmaf(v, kLog2e, -next);
+          }
+          const float e = ptx::ex2(d);
+          s[j] += e;
+          u[j] = fmaf(e, fmaxf(d, kMinD), u[j]);
+          if (row == s_tok[j]) tgt[j] = v;
+        }
+      }
+    }
+    // Over the lanes: the highest reference, then one rescaling and two sums.
+#pragma unroll
+    for (int j = 0; j < kNP; ++j) {
+      float top = f[j];
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      const float dm = f[j] == top ? 0.0f : fmaxf(__fmul_rn(f[j], kLog2e) - __fmul_rn(top, kLog2e), kMinD);
+      const float w = ptx::ex2(dm);
+      float uj = (u[j] + s[j] * dm) * w, sj = s[j] * w;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) {
+        sj += __shfl_xor_sync(0xffffffffu, sj, off);
+        uj += __shfl_xor_sync(0xffffffffu, uj, off);
+      }
+      if (lane == 0) sMerge[wq * kNP + j] = make_float4(top, sj, uj, 0.0f);
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < n_tokens) {
+    LpStats a;
+    for (int q = 0; q < 4; ++q) {
+      const float4 m = sMerge[q * kNP + threadIdx.x];
+      a.merge(m.x, m.y, m.z);
+    }
+    part[static_cast<int64_t>(blockIdx.x) * n_tokens + threadIdx.x] = make_float2(a.f, a.s);
+    part_u[static_cast<int64_t>(blockIdx.x) * n_tokens + threadIdx.x] = a.u;
+  }
+  if (threadIdx.x == 0 && *abort_flag && status) atomicOr(status, NIMBLE_STATUS_WAIT_TIMEOUT);
+  if (warp == 1) {
+    __syncwarp();
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_cg<1>(tmem_base, kCols);
+  }
+}
+
+constexpr int kDecTokens = 32;
+template <typename T, int kNP>
+int launch_decode(const void* hidden, const void* weights, const int64_t* tokens, int64_t n, int64_t d, int64_t V,
+                  int64_t v_offset, int dtype, const EpiParams& ep, cudaStream_t s, int* n_parts) {
+  DevInfo di;
+  if (int rc = device_info(&di)) return rc;
+  CUtensorMap mw, mh;
+  if (int rc = make_operand_map(&mw, weights, dtype, false, d, V, d, 32)) return rc;
+  if (int rc = make_operand_map(&mh, hidden, dtype, false, d, n, d, kNP)) return rc;
+  auto kern = lp_decode_kernel<T, kNP>;
+  NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, dec_smem<kNP>()));
+  // No more blocks than partial results have room for (one per 128 columns or so).
+  const int64_t grid = std::min<int64_t>(di.sms, (V + kBN - 1) / kBN * kColHalves);
+  kern<<<static_cast<unsigned>(grid), kDecThreads, dec_smem<kNP>(), s>>>(
+      mw, mh, static_cast<int>(n), static_cast<int>(V), static_cast<int>(d), tokens, v_offset, ep.part, ep.part_u,
+      ep.tgt, ep.status);
+  NIMBLE_CUDA_TRY(cudaGetLastError());
+  *n_parts = static_cast<int>(grid);
+  return NIMBLE_OK;
+}
+
+// out = alpha * (sum over runs of partial[run]), eight elements a thread.
+template <typename O>
+__global__ void split_sum_kernel(const float* __restrict__ partial, int runs, int64_t stride, int64_t n8,
+                                 const float* __restrict__ alpha, O* __restrict__ out) {
+  const float a = *alpha;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n8;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    float v[8];
+    load8<float>(partial + 8 * i, v);
+    for (int r = 1; r < runs; ++r) {
+      float w[8];
+      load8<float>(partial + r * stride + 8 * i, w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += w[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] *= a;
+    store8<O>(out + 8 * i, v);
+  }
 }
 
 // Row coefficients of the gradient epilogue, scaled by a power of two that
@@ -1525,12 +1883,19 @@ LpFwdLayout lp_fwd_layout(int64_t N, int64_t V) {
 // The slab backward's workspace, then the row coefficients and the scale.
 struct LpBwdLayout {
   BwdLayout slabs;
+  int splits = 1;
   size_t rowp = 0, scale = 0, total = 0;
 };
 LpBwdLayout lp_bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t slab_bytes) {
   LpBwdLayout L;
   L.slabs = bwd_layout(N, d, V, dtype, slab_bytes);
+  L.splits = dh_splits(N, d, L.slabs.slab);
   size_t off = L.slabs.total;
+  if (L.splits > 1) {  // the runs' partial grad_hidden in place of the slabs' one
+    if (L.slabs.n_slabs > 1) off = L.slabs.dh;
+    L.slabs.dh = off;
+    off = align_up(off + sizeof(float) * N * d * L.splits);
+  }
   L.rowp = off; off = align_up(off + sizeof(float4) * N);
   L.scale = off; off = align_up(off + sizeof(float));
   L.total = off;
@@ -1551,13 +1916,16 @@ extern "C" int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int
 
 extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
                                             int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
-                                            int dtype, float* shard_stats, void* workspace, size_t workspace_bytes,
-                                            int* status, void* stream) {
+                                            int dtype, int64_t ignore_index, float* shard_stats, float* out_logprob,
+                                            float* out_entropy, float* out_lse, void* workspace,
+                                            size_t workspace_bytes, int* status, void* stream) {
   if (int rc = check_half(dtype)) return rc;
   if (int rc = check_common(hidden, weights, tokens, n_tokens, d_model, v_local, dtype)) return rc;
   if (v_offset < 0) return fail(NIMBLE_ERR_INVALID_ARG, "v_offset must be >= 0");
+  if (v_local > INT32_MAX - 256) return fail(NIMBLE_ERR_INVALID_ARG, "GEMM extent exceeds 2^31");
   if (n_tokens == 0) return NIMBLE_OK;
-  if (!shard_stats) return fail(NIMBLE_ERR_INVALID_ARG, "null output pointer");
+  if (out_logprob ? !out_entropy || !out_lse || v_offset != 0 : !shard_stats)
+    return fail(NIMBLE_ERR_INVALID_ARG, "need shard_stats, or the three results of a whole vocabulary");
   const LpFwdLayout L = lp_fwd_layout(n_tokens, v_local);
   if (!workspace || workspace_bytes < L.total)
     return fail(NIMBLE_ERR_WORKSPACE, "log probability forward workspace too small");
@@ -1570,11 +1938,22 @@ extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weig
   ep.part_u = reinterpret_cast<float*>(ws + L.part_u);
   ep.tgt = reinterpret_cast<float*>(ws + L.tgt);
   ep.status = status;
-  if (int rc = gemm_dispatch<EPI_LP_FWD>(dtype, hidden, d_model, weights, d_model, n_tokens, v_local, d_model, ep, s))
-    return rc;
-  const int n_parts = static_cast<int>((v_local + kBN - 1) / kBN * kColHalves);
+  int n_parts = static_cast<int>((v_local + kBN - 1) / kBN * kColHalves);
+  int rc;
+  if (n_tokens <= kDecTokens / 2)
+    rc = dtype == NIMBLE_DTYPE_F16
+             ? launch_decode<__half, 16>(hidden, weights, tokens, n_tokens, d_model, v_local, v_offset, dtype, ep, s, &n_parts)
+             : launch_decode<__nv_bfloat16, 16>(hidden, weights, tokens, n_tokens, d_model, v_local, v_offset, dtype, ep, s, &n_parts);
+  else if (n_tokens <= kDecTokens)
+    rc = dtype == NIMBLE_DTYPE_F16
+             ? launch_decode<__half, 32>(hidden, weights, tokens, n_tokens, d_model, v_local, v_offset, dtype, ep, s, &n_parts)
+             : launch_decode<__nv_bfloat16, 32>(hidden, weights, tokens, n_tokens, d_model, v_local, v_offset, dtype, ep, s, &n_parts);
+  else
+    rc = gemm_dispatch<EPI_LP_FWD>(dtype, hidden, d_model, weights, d_model, n_tokens, v_local, d_model, ep, s);
+  if (rc) return rc;
+  const LpOut out{shard_stats, out_logprob, out_entropy, out_lse};
   lp_row_reduce_kernel<<<static_cast<unsigned>((n_tokens + 31) / 32), 32 * kReduceGroups, 0, s>>>(
-      ep.part, ep.part_u, n_parts, ep.tgt, tokens, n_tokens, v_offset, v_local, shard_stats);
+      ep.part, ep.part_u, n_parts, ep.tgt, tokens, n_tokens, v_offset, v_local, ignore_index, out, status);
   NIMBLE_CUDA_TRY(cudaGetLastError());
   return NIMBLE_OK;
 }
@@ -1626,9 +2005,21 @@ extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const fl
   eg.ignore_index = ignore_index;
   eg.rowp = rowp;
   eg.status = status;
-  return slab_backward<EPI_LP_GRAD>(L.slabs, ws, eg, scale, nullptr, 1.0f, hidden, weights, n_tokens, d_model, v_local,
-                                    v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
-                                    grad_weights_dtype, accumulate_grad_weights, status, s, nullptr, 0, 1.0f);
+  if (int rc = slab_backward<EPI_LP_GRAD>(L.slabs, ws, eg, scale, nullptr, 1.0f, hidden, weights, n_tokens, d_model,
+                                          v_local, v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
+                                          grad_weights_dtype, accumulate_grad_weights, status, s, nullptr, 0, 1.0f,
+                                          L.splits))
+    return rc;
+  if (grad_hidden && L.splits > 1) {
+    const float* partial = reinterpret_cast<const float*>(ws + L.slabs.dh);
+    const int64_t n = n_tokens * d_model, n8 = n / 8;  // d_model is a multiple of 8
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n8 + 255) / 256, 148 * 8));
+    NIMBLE_DISPATCH(grad_hidden_dtype, O,
+                    split_sum_kernel<O><<<grid, 256, 0, s>>>(partial, L.splits, n, n8, scale,
+                                                             static_cast<O*>(grad_hidden)));
+    NIMBLE_CUDA_TRY(cudaGetLastError());
+  }
+  return NIMBLE_OK;
 }
 
 // ============================================ allocation-free forward variant

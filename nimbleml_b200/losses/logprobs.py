@@ -183,18 +183,23 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     return TokenLogProbs(lp, ent, top_lp, top_id)
 
 
-def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0) -> torch.Tensor:
-    """(4, N) statistics of one weight shard: max, sum 2^d, sum d 2^d (d = (s - max) log2 e)
-    and the token's logit (0 where the shard does not hold it)."""
+def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0, *,
+                        whole: Optional[int] = None) -> torch.Tensor:
+    """(4, N) statistics of one weight shard: a reference logit, sum 2^d, sum d 2^d (d = (s - reference) log2 e) and the
+    token's logit (0 where the shard does not hold it). With ``whole`` (the ignore index) the shard is
+    the whole vocabulary and the result is (3, N): log probabilities, entropies, lse."""
     n, d = h.shape
     v_local = w.shape[0]
     dt = compute_dtype_of(h)
     dev = h.device
-    out = torch.empty((4, n), dtype=torch.float32, device=dev)
-    ws = _workspace(native.tied_logprobs_forward_workspace_size(n, d, v_local, dt), dev)
+    out = torch.empty((4 if whole is None else 3, n), dtype=torch.float32, device=dev)
+    ws_bytes = native.tied_logprobs_forward_workspace_size(n, d, v_local, dt)
+    ws = _workspace(ws_bytes, dev)
+    at = out.data_ptr()
+    results = (at, None, None, None) if whole is None else (None, at, at + 4 * n, at + 8 * n)
     native.call("nimble_tied_logprobs_forward", h.data_ptr(), w.data_ptr(), tokens.data_ptr(), n, d, v_local,
-                vocab_offset, dt, out.data_ptr(), ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(),
-                _stream_ptr(dev))
+                vocab_offset, dt, _NO_IGNORE if whole is None else whole, *results, ws.data_ptr(), ws_bytes,
+                status_word(dev).data_ptr(), _stream_ptr(dev))
     return out
 
 
@@ -246,12 +251,16 @@ def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_siz
     watch = not torch.cuda.is_current_stream_capturing()
     if watch:
         poll_status(dev)
-    part = shard_logprob_stats(h, w, tokens, vocab_offset)
-    if vocab_parallel.world_size(group) > 1:
-        part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
+    world = vocab_parallel.world_size(group)
+    if world == 1 and vocab_offset == 0 and w.shape[0] == vocab_size:
+        out = shard_logprob_stats(h, w, tokens, whole=ignore_index)
     else:
-        part = part.unsqueeze(0)
-    out = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
+        part = shard_logprob_stats(h, w, tokens, vocab_offset)
+        if world > 1:
+            part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
+        else:
+            part = part.unsqueeze(0)
+        out = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
     if watch:
         snapshot_status(dev)
     if CHECK_BOUNDS:

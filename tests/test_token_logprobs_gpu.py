@@ -339,7 +339,8 @@ def check_tied_grads(gh, gw, h, w, tokens, a, b, base=None):
         assert (off <= tol * (1 + 2.0**-6) + fin.smallest_normal * fin.eps).all(), float((off / (tol + 1e-300)).max())
 
 
-TIED = [(1, 8, 1), (1, 8, 3), (2, 64, 5), (7, 64, 257), (129, 136, 1000), (300, 72, 5003), (513, 256, 256), (1, 1024, 20011)]
+TIED = [(1, 8, 1), (1, 8, 3), (2, 64, 5), (7, 64, 257), (129, 136, 1000), (300, 72, 5003), (513, 256, 256), (1, 1024, 20011), (16, 520, 4801),
+        (17, 64, 33), (32, 128, 19001), (33, 72, 600), (128, 64, 3000), (260, 320, 6000)]
 
 
 @pytest.mark.parametrize("dtype", HALF)
