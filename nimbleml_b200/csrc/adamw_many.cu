@@ -33,7 +33,12 @@ namespace nimble {
 namespace {
 
 constexpr int kAdamThreads = 256;
-constexpr int kChunk = 8192;     // elements of one tensor a block updates
+// Elements of one tensor that a block updates: few where the tensors are small (a
+// short step then spreads over the GPU; 2048 for 8192 took a step over 116 k weights
+// from 9.0 to 4.1 us), more where they are large (finding the tensor costs a block
+// about a microsecond, and an 8-bit block then runs its loads one step ahead: 32768
+// for 8192 took 353 M weights from 1476 to 1184 us; fp32 moments gain nothing).
+constexpr int kMinChunk = 2048, kMaxChunk = 8192, kMaxChunk8 = 32768;
 constexpr int kQBlock = 128;     // elements that share a scale
 constexpr float kE4M3Max = 448.0f;
 constexpr float kE4M3Min = 1.0f / 512.0f;  // smallest positive e4m3 value
@@ -50,6 +55,7 @@ struct AdamScalars {
 template <int kMax>
 struct AdamTable {
   int n;
+  int chunk;
   int first_chunk[kMax + 1];  // tensor t owns chunks [first_chunk[t], first_chunk[t + 1])
   nimble_adamw_tensor t[kMax];
 };
@@ -99,8 +105,8 @@ __global__ void __launch_bounds__(kAdamThreads)
 adamw_many_kernel(const __grid_constant__ AdamTable<kMax> tab, const AdamScalars a) {
   const int ti = find_tensor(tab, blockIdx.x);
   const nimble_adamw_tensor& t = tab.t[ti];
-  const int64_t lo = static_cast<int64_t>(blockIdx.x - tab.first_chunk[ti]) * kChunk;
-  const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), t.n - lo));
+  const int64_t lo = static_cast<int64_t>(blockIdx.x - tab.first_chunk[ti]) * tab.chunk;
+  const int n = static_cast<int>(min(static_cast<int64_t>(tab.chunk), t.n - lo));
   float* w = t.weights + lo;
   float* m = static_cast<float*>(t.exp_avg) + lo;
   float* v = static_cast<float*>(t.exp_avg_sq) + lo;
@@ -141,61 +147,44 @@ adamw_many_kernel(const __grid_constant__ AdamTable<kMax> tab, const AdamScalars
 }
 
 // ------------------------------------------------------------ 8-bit moments
-// Every operation below is rounded on its own (no fused multiply-add), so the
-// step is defined bit by bit: a code next to a border comes out the same
-// wherever these operations are carried out in fp32.
-__device__ __forceinline__ float4 decode4(uint32_t codes, float scale) {
+// Everything that a code depends on is rounded operation by operation (no fused
+// multiply-add, correctly rounded roots), so the
+// moments are defined bit by bit: a code next to a border comes out the same
+// wherever these operations are carried out in fp32. The weight's step is not
+// rounded to anything coarse and takes an approximate quotient (2 ulp of the step).
+struct Four {
+  float2 a, b;
+};
+__device__ __forceinline__ Four decode4(uint32_t codes, float scale) {
   const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes & 0xFFFFu), __NV_E4M3);
   const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes >> 16), __NV_E4M3);
-  const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
-  return make_float4(__fmul_rn(a.x, scale), __fmul_rn(a.y, scale), __fmul_rn(b.x, scale), __fmul_rn(b.y, scale));
+  return {mul2(__half22float2(__half2(lo)), both(scale)), mul2(__half22float2(__half2(hi)), both(scale))};
 }
 
 // Codes of four values of a block whose 128 elements lie in a warp (lane l has
 // elements 4 l .. 4 l + 3; the elements behind a tensor's end are zero).
 template <bool kRoot>
-__device__ __forceinline__ uint32_t encode4(const float (&x)[4], float& scale) {
-  uint32_t top = 0;  // bits of a magnitude order like the magnitude, NaN above all
-#pragma unroll
-  for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-  const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+__device__ __forceinline__ uint32_t encode4(const Four& x, float& scale) {
+  // Bits of a magnitude order like the magnitude, NaN above all.
+  constexpr uint32_t kAbs = 0x7FFFFFFFu;
+  const uint32_t t0 = max(__float_as_uint(x.a.x) & kAbs, __float_as_uint(x.a.y) & kAbs);
+  const uint32_t t1 = max(__float_as_uint(x.b.x) & kAbs, __float_as_uint(x.b.y) & kAbs);
+  const float big = __uint_as_float(__reduce_max_sync(0xffffffffu, max(t0, t1)));
   const bool live = !(big < kQZero);
   const float up = live ? __fdiv_rn(kE4M3Max, big) : 0.0f;
   scale = live ? __fmul_rn(big, 1.0f / kE4M3Max) : 0.0f;
-  float y[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    y[e] = __fmul_rn(x[e], up);
-    if (kRoot && x[e] > 0.0f && y[e] < kE4M3Min) y[e] = kE4M3Min;
+  float2 y0 = mul2(x.a, both(up)), y1 = mul2(x.b, both(up));
+  if constexpr (kRoot) {
+    // Roots are >= 0: a positive one is raised to the smallest code, a NaN stays.
+    auto lift = [](float r, float y) { return r > 0.0f && y < kE4M3Min ? kE4M3Min : y; };
+    y0 = make_float2(lift(x.a.x, y0.x), lift(x.a.y, y0.y));
+    y1 = make_float2(lift(x.b.x, y1.x), lift(x.b.y, y1.y));
   }
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(y0, __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(y1, __NV_SATFINITE, __NV_E4M3);
   return lo | (hi << 16);
 }
 
-// Four elements at p, zero behind the tensor's end (n of them are left).
-__device__ __forceinline__ void load_grad4(const void* g, int64_t i, int n, int dt, bool vec, float (&o)[4]) {
-  if (vec && n >= 4) {
-    if (dt == NIMBLE_DTYPE_F32) {
-      const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(g) + i);
-      o[0] = f.x; o[1] = f.y; o[2] = f.z; o[3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g) + i);
-      if (dt == NIMBLE_DTYPE_F16) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-        o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
-      } else {
-        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x));
-        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
-        o[0] = a.x; o[1] = a.y; o[2] = b.x; o[3] = b.y;
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = e < n ? load_grad(g, i + e, dt) : 0.0f;
-}
 __device__ __forceinline__ uint32_t load_codes4(const uint8_t* p, int n, bool vec) {
   if (vec && n >= 4) return *reinterpret_cast<const uint32_t*>(p);
   uint32_t c = 0;
@@ -214,103 +203,221 @@ __device__ __forceinline__ void store_codes4(uint8_t* p, int n, bool vec, uint32
     if (e < n) p[e] = static_cast<uint8_t>(c >> (8 * e));
 }
 
-template <int kMax>
-__global__ void __launch_bounds__(kAdamThreads)
-adamw_many_8bit_kernel(const __grid_constant__ AdamTable<kMax> tab, const AdamScalars a) {
-  const int ti = find_tensor(tab, blockIdx.x);
-  const nimble_adamw_tensor& t = tab.t[ti];
-  const int64_t lo = static_cast<int64_t>(blockIdx.x - tab.first_chunk[ti]) * kChunk;
-  const int n = static_cast<int>(min(static_cast<int64_t>(kChunk), t.n - lo));
+// Four gradients, not yet widened.
+template <typename G>
+struct RawFour {
+  uint2 v[sizeof(G) / 2];
+  __device__ __forceinline__ Four get() const {
+    const G* p = reinterpret_cast<const G*>(v);
+    return {make_float2(to_f<G>(p[0]), to_f<G>(p[1])), make_float2(to_f<G>(p[2]), to_f<G>(p[3]))};
+  }
+};
+template <typename G>
+__device__ __forceinline__ void load_raw4(const G* p, RawFour<G>& o) {
+  if constexpr (sizeof(G) == 4) *reinterpret_cast<uint4*>(&o) = *reinterpret_cast<const uint4*>(p);
+  else o.v[0] = *reinterpret_cast<const uint2*>(p);
+}
+
+// One block of 128: new weights, codes and scales from the old.
+__device__ __forceinline__ void update_8bit(const Four& g, Four& w, uint32_t& mcode, uint32_t& vcode, float& mscale,
+                                            float& vscale, const AdamScalars& a) {
+  Four m = decode4(mcode, mscale), r = decode4(vcode, vscale);
+  auto pair = [&](float2 g, float2& w, float2& m, float2& r) {
+    // Products that are added next are single ones: a packed product and sum would be
+    // fused into one rounding.
+    auto times = [](float s, float2 x) { return make_float2(__fmul_rn(s, x.x), __fmul_rn(s, x.y)); };
+    m = add2(times(a.b1, m), times(a.omb1, g));
+    const float2 v = add2(times(a.b2, mul2(r, r)), times(a.omb2, mul2(g, g)));
+    r = make_float2(__fsqrt_rn(v.x), __fsqrt_rn(v.y));
+    const float2 den = fma2(r, both(a.c2), both(a.eps));
+    const float2 num = mul2(m, both(a.c1));
+    w = fma2(w, both(a.decay), make_float2(-__fdividef(num.x, den.x), -__fdividef(num.y, den.y)));
+  };
+  pair(g.a, w.a, m.a, r.a);
+  pair(g.b, w.b, m.b, r.b);
+  mcode = encode4<false>(m, mscale);
+  vcode = encode4<true>(r, vscale);
+}
+
+// Pointers of one chunk of a tensor.
+struct Chunk8 {
+  float* w;
+  uint8_t *mc, *vc;
+  float *ms, *vs;
+  const void* g;
+  void* c;
+  int n;
+};
+
+// Chunks whose pointers allow vectors and whose length is whole blocks of 128: a
+// warp takes kU blocks at a time, all their loads first.
+template <typename G, typename C, bool kCopy>
+__device__ __forceinline__ void chunk_8bit_vec(const Chunk8& k, const AdamScalars& a) {
+  constexpr int kU = 2;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float* w = t.weights + lo;
-  uint8_t* mc = static_cast<uint8_t*>(t.exp_avg) + lo;
-  uint8_t* vc = static_cast<uint8_t*>(t.exp_avg_sq) + lo;
-  float* ms = t.exp_avg_scale + lo / kQBlock;
-  float* vs = t.exp_avg_sq_scale + lo / kQBlock;
-  const int gdt = t.grad_dtype, cdt = t.weights_copy_dtype;
-  const int ges = gdt == NIMBLE_DTYPE_F32 ? 4 : 2, ces = cdt == NIMBLE_DTYPE_F32 ? 4 : 2;
-  const void* g = static_cast<const uint8_t*>(t.grad) + lo * ges;
-  void* c = t.weights_copy ? static_cast<uint8_t*>(t.weights_copy) + lo * ces : nullptr;
-  const bool vw = aligned(w, 16), vg = aligned(g, 4 * ges), vm = aligned(mc, 4), vv = aligned(vc, 4),
-             vcopy = aligned(c, 4 * ces);
-  for (int b = warp; b * kQBlock < n; b += kAdamThreads / 32) {  // one block of 128 a warp
-    const int i = b * kQBlock + 4 * lane;
-    const int left = n - i;  // may be <= 0
-    float gv[4], wv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    load_grad4(g, i, left, gdt, vg, gv);
-    const uint32_t mcode = load_codes4(mc + i, left, vm), vcode = load_codes4(vc + i, left, vv);
-    if (vw && left >= 4) {
-      const float4 f = *reinterpret_cast<const float4*>(w + i);
-      wv[0] = f.x; wv[1] = f.y; wv[2] = f.z; wv[3] = f.w;
-    } else {
+  const int blocks = k.n / kQBlock;
+  struct Raw {
+    RawFour<G> g;
+    float4 w;
+    uint32_t mc, vc;
+    float ms, vs;
+  };
+  auto load = [&](int b0, Raw (&r)[kU]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) wv[e] = w[i + e];
+    for (int u = 0; u < kU; ++u) {
+      const int b = min(b0 + u, blocks - 1);  // the last block again where there is no other
+      const int i = b * kQBlock + 4 * lane;
+      load_raw4<G>(static_cast<const G*>(k.g) + i, r[u].g);
+      r[u].w = *reinterpret_cast<const float4*>(k.w + i);
+      r[u].mc = *reinterpret_cast<const uint32_t*>(k.mc + i);
+      r[u].vc = *reinterpret_cast<const uint32_t*>(k.vc + i);
+      r[u].ms = k.ms[b];
+      r[u].vs = k.vs[b];
     }
-    const float4 m4 = decode4(mcode, ms[b]), r4 = decode4(vcode, vs[b]);
-    float m[4] = {m4.x, m4.y, m4.z, m4.w}, r[4] = {r4.x, r4.y, r4.z, r4.w};
+  };
+  constexpr int kStride = kAdamThreads / 32 * kU;
+  Raw next[kU];
+  if (warp * kU < blocks) load(warp * kU, next);
+  for (int b0 = warp * kU; b0 < blocks; b0 += kStride) {
+    Raw now[kU];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      m[e] = __fadd_rn(__fmul_rn(a.b1, m[e]), __fmul_rn(a.omb1, gv[e]));
-      const float vn = __fadd_rn(__fmul_rn(a.b2, __fmul_rn(r[e], r[e])), __fmul_rn(a.omb2, __fmul_rn(gv[e], gv[e])));
-      r[e] = __fsqrt_rn(vn);
-      const float den = __fadd_rn(__fmul_rn(r[e], a.c2), a.eps);
-      wv[e] = __fsub_rn(__fmul_rn(wv[e], a.decay), __fdiv_rn(__fmul_rn(m[e], a.c1), den));
-    }
-    float mscale, vscale;
-    const uint32_t mnew = encode4<false>(m, mscale), vnew = encode4<true>(r, vscale);
-    __syncwarp();  // every lane has read the block's scales
-    if (lane == 0) {
-      ms[b] = mscale;
-      vs[b] = vscale;
-    }
-    if (left <= 0) continue;
-    store_codes4(mc + i, left, vm, mnew);
-    store_codes4(vc + i, left, vv, vnew);
-    if (vw && left >= 4) {
-      *reinterpret_cast<float4*>(w + i) = make_float4(wv[0], wv[1], wv[2], wv[3]);
-    } else {
+    for (int u = 0; u < kU; ++u) now[u] = next[u];
+    // The next blocks' loads are in flight while these are updated (other warps'
+    // blocks lie between, so nothing that is written here is read there).
+    if (b0 + kStride < blocks) load(b0 + kStride, next);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) w[i + e] = wv[e];
-    }
-    if (c) {
-      if (vcopy && left >= 4 && ces == 2) {
-        uint2 u;
-        if (cdt == NIMBLE_DTYPE_F16) {
-          *reinterpret_cast<__half2*>(&u.x) = __floats2half2_rn(wv[0], wv[1]);
-          *reinterpret_cast<__half2*>(&u.y) = __floats2half2_rn(wv[2], wv[3]);
-        } else {
-          *reinterpret_cast<__nv_bfloat162*>(&u.x) = __floats2bfloat162_rn(wv[0], wv[1]);
-          *reinterpret_cast<__nv_bfloat162*>(&u.y) = __floats2bfloat162_rn(wv[2], wv[3]);
-        }
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(c) + i) = u;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < left) store_copy(c, i + e, cdt, wv[e]);
+    for (int u = 0; u < kU; ++u) {
+      const int b = b0 + u, i = b * kQBlock + 4 * lane;
+      if (b >= blocks) break;
+      const float4 w = now[u].w;
+      uint32_t mc = now[u].mc, vc = now[u].vc;
+      float ms = now[u].ms, vs = now[u].vs;
+      Four wn = {make_float2(w.x, w.y), make_float2(w.z, w.w)};
+      update_8bit(now[u].g.get(), wn, mc, vc, ms, vs, a);
+      if (lane == 0) {
+        k.ms[b] = ms;
+        k.vs[b] = vs;
+      }
+      *reinterpret_cast<uint32_t*>(k.mc + i) = mc;
+      *reinterpret_cast<uint32_t*>(k.vc + i) = vc;
+      *reinterpret_cast<float4*>(k.w + i) = make_float4(wn.a.x, wn.a.y, wn.b.x, wn.b.y);
+      if constexpr (kCopy) {
+        RawFour<C> o;
+        C* p = reinterpret_cast<C*>(&o);
+        p[0] = from_f<C>(wn.a.x);
+        p[1] = from_f<C>(wn.a.y);
+        p[2] = from_f<C>(wn.b.x);
+        p[3] = from_f<C>(wn.b.y);
+        if constexpr (sizeof(C) == 4)
+          *reinterpret_cast<uint4*>(static_cast<C*>(k.c) + i) = *reinterpret_cast<const uint4*>(&o);
+        else
+          *reinterpret_cast<uint2*>(static_cast<C*>(k.c) + i) = o.v[0];
       }
     }
   }
 }
 
-// Values of codes: one warp per block of 128.
+// Any alignment and length, element by element.
+__device__ __noinline__ void chunk_8bit_any(const Chunk8& k, int gdt, int cdt, const AdamScalars& a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int b = warp; b * kQBlock < k.n; b += kAdamThreads / 32) {
+    const int i = b * kQBlock + 4 * lane;
+    const int left = k.n - i;  // may be <= 0
+    float g[4], w[4];
+    uint32_t mc = load_codes4(k.mc + i, left, false), vc = load_codes4(k.vc + i, left, false);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      g[e] = e < left ? load_grad(k.g, i + e, gdt) : 0.0f;
+      w[e] = e < left ? k.w[i + e] : 0.0f;
+    }
+    float ms = k.ms[b], vs = k.vs[b];
+    Four wn = {make_float2(w[0], w[1]), make_float2(w[2], w[3])};
+    update_8bit({make_float2(g[0], g[1]), make_float2(g[2], g[3])}, wn, mc, vc, ms, vs, a);
+    __syncwarp();  // every lane has read the block's scales
+    if (lane == 0) {
+      k.ms[b] = ms;
+      k.vs[b] = vs;
+    }
+    store_codes4(k.mc + i, left, false, mc);
+    store_codes4(k.vc + i, left, false, vc);
+    const float out[4] = {wn.a.x, wn.a.y, wn.b.x, wn.b.y};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) {
+        k.w[i + e] = out[e];
+        if (k.c) store_copy(k.c, i + e, cdt, out[e]);
+      }
+  }
+}
+
+template <int kMax>
+__global__ void __launch_bounds__(kAdamThreads, 3)
+adamw_many_8bit_kernel(const __grid_constant__ AdamTable<kMax> tab, const AdamScalars a) {
+  const int ti = find_tensor(tab, blockIdx.x);
+  const nimble_adamw_tensor& t = tab.t[ti];
+  const int64_t lo = static_cast<int64_t>(blockIdx.x - tab.first_chunk[ti]) * tab.chunk;
+  const int gdt = t.grad_dtype, cdt = t.weights_copy ? t.weights_copy_dtype : -1;
+  const int ges = gdt == NIMBLE_DTYPE_F32 ? 4 : 2, ces = cdt == NIMBLE_DTYPE_F32 ? 4 : 2;
+  Chunk8 k;
+  k.n = static_cast<int>(min(static_cast<int64_t>(tab.chunk), t.n - lo));
+  k.w = t.weights + lo;
+  k.mc = static_cast<uint8_t*>(t.exp_avg) + lo;
+  k.vc = static_cast<uint8_t*>(t.exp_avg_sq) + lo;
+  k.ms = t.exp_avg_scale + lo / kQBlock;
+  k.vs = t.exp_avg_sq_scale + lo / kQBlock;
+  k.g = static_cast<const uint8_t*>(t.grad) + lo * ges;
+  k.c = t.weights_copy ? static_cast<uint8_t*>(t.weights_copy) + lo * ces : nullptr;
+  const bool vec = k.n % kQBlock == 0 && aligned(k.w, 16) && aligned(k.g, 4 * ges) && aligned(k.mc, 4) &&
+                   aligned(k.vc, 4) && aligned(k.c, 4 * ces);
+  if (!vec) {
+    chunk_8bit_any(k, gdt, cdt, a);
+    return;
+  }
+  auto with_copy = [&](auto tag) {
+    using G = decltype(tag);
+    if (cdt < 0) chunk_8bit_vec<G, float, false>(k, a);
+    else if (cdt == NIMBLE_DTYPE_F32) chunk_8bit_vec<G, float, true>(k, a);
+    else if (cdt == NIMBLE_DTYPE_F16) chunk_8bit_vec<G, __half, true>(k, a);
+    else chunk_8bit_vec<G, __nv_bfloat16, true>(k, a);
+  };
+  if (gdt == NIMBLE_DTYPE_F32) with_copy(float{});
+  else if (gdt == NIMBLE_DTYPE_F16) with_copy(__half{});
+  else with_copy(__nv_bfloat16{});
+}
+
+// Values of codes: a warp takes kDeqBlocks blocks of 128, all their loads first.
+constexpr int kDeqBlocks = 4;
 template <bool kRoot>
 __global__ void __launch_bounds__(kAdamThreads)
 dequantize_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales, int64_t n,
                   float* __restrict__ out) {
-  const int64_t b = static_cast<int64_t>(blockIdx.x) * (kAdamThreads / 32) + (threadIdx.x >> 5);
-  const int64_t i = b * kQBlock + 4 * (threadIdx.x & 31);
-  if (i >= n) return;
-  const int left = static_cast<int>(min(static_cast<int64_t>(4), n - i));
-  float4 f = decode4(load_codes4(codes + i, left, aligned(codes, 4)), scales[b]);
-  if (kRoot) f = make_float4(__fmul_rn(f.x, f.x), __fmul_rn(f.y, f.y), __fmul_rn(f.z, f.z), __fmul_rn(f.w, f.w));
-  if (left == 4 && aligned(out, 16)) {
-    *reinterpret_cast<float4*>(out + i) = f;
-    return;
+  const int64_t b0 = (static_cast<int64_t>(blockIdx.x) * (kAdamThreads / 32) + (threadIdx.x >> 5)) * kDeqBlocks;
+  const bool vec_in = aligned(codes, 4), vec_out = aligned(out, 16);
+  uint32_t c[kDeqBlocks];
+  float scale[kDeqBlocks];
+#pragma unroll
+  for (int k = 0; k < kDeqBlocks; ++k) {
+    const int64_t i = (b0 + k) * kQBlock + 4 * (threadIdx.x & 31);
+    const int left = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(4), n - i)));
+    c[k] = load_codes4(codes + i, left, vec_in);
+    scale[k] = left > 0 ? scales[b0 + k] : 0.0f;
   }
-  const float v[4] = {f.x, f.y, f.z, f.w};
-  for (int e = 0; e < left; ++e) out[i + e] = v[e];
+#pragma unroll
+  for (int k = 0; k < kDeqBlocks; ++k) {
+    const int64_t i = (b0 + k) * kQBlock + 4 * (threadIdx.x & 31);
+    if (i >= n) return;
+    Four q = decode4(c[k], scale[k]);
+    if (kRoot) q = {mul2(q.a, q.a), mul2(q.b, q.b)};
+    const float4 f = make_float4(q.a.x, q.a.y, q.b.x, q.b.y);
+    if (vec_out && n - i >= 4) {
+      *reinterpret_cast<float4*>(out + i) = f;
+      continue;
+    }
+    const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (i + e < n) out[i + e] = v[e];
+  }
 }
 
 template <bool kRoot>
@@ -328,7 +435,7 @@ quantize_kernel(const float* __restrict__ x, int64_t n, uint8_t* __restrict__ co
     if (kRoot) v[e] = __fsqrt_rn(v[e]);
   }
   float scale;
-  const uint32_t c = encode4<kRoot>(v, scale);
+  const uint32_t c = encode4<kRoot>({make_float2(v[0], v[1]), make_float2(v[2], v[3])}, scale);
   if (lane == 0) scales[b] = scale;
   if (left > 0) store_codes4(codes + i, left, aligned(codes, 4), c);
 }
@@ -336,6 +443,10 @@ quantize_kernel(const float* __restrict__ x, int64_t n, uint8_t* __restrict__ co
 template <int kMax>
 int launch_adamw(const nimble_adamw_tensor* tensors, int n, bool eight, const AdamScalars& a, cudaStream_t s) {
   AdamTable<kMax> tab;
+  int64_t total = 0;
+  for (int i = 0; i < n; ++i) total += tensors[i].n;
+  tab.chunk = kMinChunk;
+  while (tab.chunk < (eight ? kMaxChunk8 : kMaxChunk) && total / tab.chunk > 148 * 16) tab.chunk *= 2;
   tab.n = 0;
   int64_t chunks = 0;
   auto flush = [&]() -> int {
@@ -352,7 +463,7 @@ int launch_adamw(const nimble_adamw_tensor* tensors, int n, bool eight, const Ad
   };
   for (int i = 0; i < n; ++i) {
     if (tensors[i].n == 0) continue;
-    const int64_t c = (tensors[i].n + kChunk - 1) / kChunk;
+    const int64_t c = (tensors[i].n + tab.chunk - 1) / tab.chunk;
     if (tab.n == kMax || chunks + c > INT32_MAX)
       if (int rc = flush()) return rc;
     tab.first_chunk[tab.n] = static_cast<int>(chunks);
@@ -379,7 +490,7 @@ extern "C" int nimble_adamw_step_many(const nimble_adamw_tensor* tensors, int n_
   const bool eight = moment_bits == 8;
   for (int i = 0; i < n_tensors; ++i) {
     const nimble_adamw_tensor& t = tensors[i];
-    if (t.n < 0 || (t.n + kChunk - 1) / kChunk > INT32_MAX) return fail(NIMBLE_ERR_INVALID_ARG, "bad tensor size");
+    if (t.n < 0 || (t.n + kMinChunk - 1) / kMinChunk > INT32_MAX) return fail(NIMBLE_ERR_INVALID_ARG, "bad tensor size");
     if (t.n == 0) continue;
     if (!valid_dtype(t.grad_dtype) || (t.weights_copy && !valid_dtype(t.weights_copy_dtype)))
       return fail(NIMBLE_ERR_INVALID_ARG, "bad dtype");
@@ -416,7 +527,8 @@ extern "C" int nimble_adamw_dequantize(const void* codes, const float* scales, i
   if (n < 0 || n > static_cast<int64_t>(INT32_MAX) * kAdamThreads) return fail(NIMBLE_ERR_INVALID_ARG, "bad size");
   if (n == 0) return NIMBLE_OK;
   if (!codes || !scales || !out) return fail(NIMBLE_ERR_INVALID_ARG, "null pointer argument");
-  const unsigned grid = static_cast<unsigned>((n + 4 * kAdamThreads - 1) / (4 * kAdamThreads));
+  constexpr int64_t kPerBlock = 4 * kAdamThreads * kDeqBlocks;
+  const unsigned grid = static_cast<unsigned>((n + kPerBlock - 1) / kPerBlock);
   auto kern = root ? dequantize_kernel<true> : dequantize_kernel<false>;
   kern<<<grid, kAdamThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(codes), scales, n, out);
   NIMBLE_CUDA_TRY(cudaGetLastError());

@@ -103,6 +103,8 @@ struct EpiParams {
   // and run s reads src and writes out s * split_stride elements further.
   int k_splits;
   int64_t split_stride;
+  // Host only: the launch takes 128 x 256 tiles where the product is short (below).
+  bool log_probs;
 };
 
 template <typename T> struct ElemInfo;
@@ -830,7 +832,14 @@ const int g_wide = [] {
   return m == 1 ? 15 : m;
 }();
 constexpr int kSmemBytesWide = kStagesWide * (2 * kABytes + kBBytes) + kStoreBytes + 1024 + 256;
-constexpr bool is_lp(int epi) { return epi == EPI_LP_FWD || epi == EPI_LP_GRAD; }
+// The log probabilities' products take 128 x 256 tiles, whose epilogues overlap the
+// next tile's multiplications, up to this contraction length: a wide tile's
+// multiplications are too short there to hide its epilogue's share. Forward /
+// recompute / dE in us, wide against 128 x 256: 2048 x 768 x 50257 142 / 171 / 156
+// against 115 / 135 / 142, 4096 x 1024 x 32000 214 / 243 / 215 against 183 / 211 / 237
+// (dE contracts over 4096 tokens), 4096 x 2048 x 32000 383 / 410 / 431 against 379 /
+// 421 / 430. At most 128 rows fill half a wide tile and take the small ones too.
+constexpr int64_t kShortK = 2048;
 template <int EPI, bool kAMN>
 constexpr int gemm_kind_bit() {
   return (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) ? 1 : (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) ? 2 : kAMN ? 4 : 8;
@@ -927,9 +936,7 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
     cfg.numAttrs = 1;
     NIMBLE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, static_cast<int>(M), static_cast<int>(N),
                                        static_cast<int>(K), group_m, ep));
-  } else if ((g_wide & gemm_kind_bit<EPI, kAMN>()) && !(is_lp(EPI) && M <= kBM)) {
-    // (Log probabilities of at most 128 tokens fill half a wide tile and are
-    // bound by reading the weights: 128 x 256 tiles, twice as many.)
+  } else if ((g_wide & gemm_kind_bit<EPI, kAMN>()) && !(ep.log_probs && (M <= kBM || K <= kShortK))) {
     auto kern = tc_gemm_tn_kernel<T, EPI, kAMN, kBMN, 1, true>;
     NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesWide));
     const int64_t tiles = ((M + 2 * kBM - 1) / (2 * kBM)) * ((N + kBN - 1) / kBN);
@@ -1219,6 +1226,7 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
       ee.alpha_mult = alpha_mult;
       ee.accum_out = accumulate_grad_weights ? 1 : 0;
       ee.status = status;
+      ee.log_probs = eg_base.log_probs;
       return gemm_dispatch<EPI_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
                                                   r1 - r0, d_model, n_tokens, ee, s, max_ctas);
     };
@@ -1938,6 +1946,7 @@ extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weig
   ep.part_u = reinterpret_cast<float*>(ws + L.part_u);
   ep.tgt = reinterpret_cast<float*>(ws + L.tgt);
   ep.status = status;
+  ep.log_probs = true;
   int n_parts = static_cast<int>((v_local + kBN - 1) / kBN * kColHalves);
   int rc;
   if (n_tokens <= kDecTokens / 2)
@@ -2005,6 +2014,7 @@ extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const fl
   eg.ignore_index = ignore_index;
   eg.rowp = rowp;
   eg.status = status;
+  eg.log_probs = true;
   if (int rc = slab_backward<EPI_LP_GRAD>(L.slabs, ws, eg, scale, nullptr, 1.0f, hidden, weights, n_tokens, d_model,
                                           v_local, v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
                                           grad_weights_dtype, accumulate_grad_weights, status, s, nullptr, 0, 1.0f,
