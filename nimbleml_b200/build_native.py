@@ -8,7 +8,8 @@ loads on hosts without a GPU. Run ``python -m nimbleml_b200.build_native``.
 The same step builds ``_lib/nimbleml_tied_ce_native*.so``, the pybind11
 module with the reference-style ``*_device`` entry points
 (``csrc/tied_ce_pybind.cpp``), linked against the library with an
-``$ORIGIN`` run path.
+``$ORIGIN`` run path, and ``_lib/nimbleml_b200_host*.so``, the torch host side of
+the operators whose calls are short (``csrc/torch_host.cpp``).
 """
 from __future__ import annotations
 
@@ -29,6 +30,7 @@ SOURCES = [CSRC / "tied_ce.cu", CSRC / "rowwise.cu", CSRC / "token_logprobs.cu",
 HEADERS = [CSRC / "sm100_ptx.cuh", CSRC / "common.cuh", CSRC / "elementwise.cuh",
            REPO_DIR / "include" / "nimbleml_tied_ce.h"]
 PYBIND_SOURCE = CSRC / "tied_ce_pybind.cpp"
+HOST_SOURCE = CSRC / "torch_host.cpp"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -48,6 +50,11 @@ def _nvcc() -> str:
 def pybind_module_path() -> Path:
     ext = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     return LIB_DIR / f"nimbleml_tied_ce_native{ext}"
+
+
+def host_module_path() -> Path:
+    ext = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    return LIB_DIR / f"nimbleml_b200_host{ext}"
 
 
 def _stale(target: Path, deps) -> bool:
@@ -75,8 +82,34 @@ def build_pybind(force: bool = False, verbose: bool = False) -> Path:
     return out
 
 
+def build_host(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the torch host module (g++ against the installed torch) if it is older than its source or the library."""
+    out = host_module_path()
+    if not force and not _stale(out, [HOST_SOURCE, LIB_PATH, HEADERS[-1]]):
+        return out
+    import torch
+
+    base = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1]
+    tmp = out.with_suffix(".tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-I", str(base / "include"), "-I", str(base / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], "-I", str(REPO_DIR / "include"),
+           str(HOST_SOURCE), "-L", str(LIB_DIR), "-l:" + LIB_PATH.name, "-L", str(base / "lib"), "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch", "-ltorch_python",
+           # The shared C++ runtime that torch uses, by its file name: a compiler whose libstdc++.so link is missing
+           # would take the static one, and two copies of its locale facets break the first formatted message.
+           "-l:libstdc++.so.6", "-Wl,-rpath,$ORIGIN", "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, out)
+    return out
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the library if a source is newer than the .so (or ``force``), then the pybind11 module."""
+    """Compile the library if a source is newer than the .so (or ``force``), then the two host modules."""
     if force or _stale(LIB_PATH, SOURCES + HEADERS):
         LIB_DIR.mkdir(parents=True, exist_ok=True)
         tmp = LIB_PATH.with_suffix(".so.tmp")
@@ -86,6 +119,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         subprocess.run(cmd, check=True)
         os.replace(tmp, LIB_PATH)
     build_pybind(force=force, verbose=verbose)
+    build_host(force=force, verbose=verbose)
     return LIB_PATH
 
 

@@ -1,0 +1,378 @@
+// torch_host.cpp — the host side of the operators whose calls are short against
+// Python's: layer norm and token log probabilities as autograd nodes, and the
+// many-tensor AdamW step with its checks. Everything on the GPU goes through the
+// C ABI (include/nimbleml_tied_ce.h); this file only checks arguments, allocates
+// outputs and workspaces on torch's current stream, and keeps what the backward
+// needs. Errors are Python's: ValueError for arguments, RuntimeError with the
+// library's message for a failing call.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
+#include <optional>
+#include <string>
+#include <unordered_set>
+#include <vector>
+
+#include "nimbleml_tied_ce.h"
+
+namespace py = pybind11;
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+void check_rc(int rc, const char* name) {
+  TORCH_CHECK(rc == 0, name, " failed (", rc, "): ", nimble_tied_ce_last_error());
+}
+
+int dtype_or(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return NIMBLE_DTYPE_F32;
+    case at::kHalf: return NIMBLE_DTYPE_F16;
+    case at::kBFloat16: return NIMBLE_DTYPE_BF16;
+    default: return -1;
+  }
+}
+int dtype_of(const Tensor& t) {
+  const int d = dtype_or(t);
+  TORCH_CHECK_VALUE(d >= 0, "unsupported compute dtype torch.", at::toString(t.scalar_type()),
+                    "; use float32, float16 or bfloat16");
+  return d;
+}
+
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
+  return at::empty(shape, like.options().dtype(type).memory_format(c10::nullopt).requires_grad(false));
+}
+
+// (n, d) rows of x: a view where its rows are contiguous and do not overlap, else a
+// copy; and their pitch.
+Tensor rows_of(const Tensor& x, int64_t& n, int64_t& d, int64_t& pitch) {
+  d = x.size(-1);
+  Tensor r = x.dim() == 2 ? x : x.reshape({-1, d});
+  n = r.size(0);
+  if (r.stride(1) != 1 || (n > 1 && r.stride(0) < d)) r = r.contiguous();
+  pitch = std::max(r.stride(0), d);
+  return r;
+}
+
+// ------------------------------------------------------------------ layer norm
+constexpr int64_t kMaxNorm = 8192;
+
+struct NormArgs {
+  Tensor x, gamma, beta;  // rows; parameters in the rows' type or fp32
+  int64_t n, d, pitch;
+};
+
+NormArgs norm_args(const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta) {
+  NormArgs a;
+  a.x = rows_of(x, a.n, a.d, a.pitch);
+  const auto own = x.scalar_type();
+  const bool same = gamma.scalar_type() == own && (!beta || beta->scalar_type() == own);
+  const auto type = same ? own : at::kFloat;
+  a.gamma = gamma.to(type).contiguous();
+  if (beta) a.beta = beta->to(type).contiguous();
+  return a;
+}
+
+Tensor norm_forward(const NormArgs& a, const Tensor& x, double eps, Tensor* stats) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = empty(x.sizes(), x, x.scalar_type());
+  float* mean = nullptr;
+  if (stats) {
+    *stats = empty({2, a.n}, x, at::kFloat);
+    mean = stats->mutable_data_ptr<float>();
+  }
+  check_rc(nimble_layernorm_forward(a.x.const_data_ptr(), a.pitch, a.gamma.const_data_ptr(),
+                                    a.beta.defined() ? a.beta.const_data_ptr() : nullptr, a.n, a.d,
+                                    static_cast<float>(eps), dtype_of(a.x), dtype_of(a.gamma), y.mutable_data_ptr(),
+                                    mean, stats ? mean + a.n : nullptr, stream_of(x)),
+           "nimble_layernorm_forward");
+  return y;
+}
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta,
+                        double eps) {
+    const NormArgs a = norm_args(x, gamma, beta);
+    Tensor stats;
+    Tensor y = norm_forward(a, x, eps, &stats);
+    ctx->save_for_backward({a.x, a.gamma, stats});
+    ctx->saved_data["gamma"] = static_cast<int64_t>(gamma.scalar_type());
+    ctx->saved_data["beta"] = beta ? static_cast<int64_t>(beta->scalar_type()) : int64_t(-1);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm's backward is not differentiable itself");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &gamma = saved[1], &stats = saved[2];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t n = x.size(0), d = x.size(1);
+    const int64_t beta_type = ctx->saved_data["beta"].toInt();
+    const Tensor gy = grads[0].to(x.scalar_type()).contiguous();
+    Tensor gx = empty(gy.sizes(), x, x.scalar_type());
+    Tensor gg = empty({d}, x, at::kFloat), gb;
+    if (beta_type >= 0) gb = empty({d}, x, at::kFloat);
+    size_t bytes = 0;
+    check_rc(nimble_layernorm_backward_workspace_size(n, d, &bytes), "nimble_layernorm_backward_workspace_size");
+    const Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, x, at::kByte);
+    const float* mean = stats.const_data_ptr<float>();
+    check_rc(nimble_layernorm_backward(gy.const_data_ptr(), x.const_data_ptr(), std::max(x.stride(0), d),
+                                       gamma.const_data_ptr(), mean, mean + n, n, d, dtype_of(x), dtype_of(gamma),
+                                       gx.mutable_data_ptr(), gg.mutable_data_ptr<float>(),
+                                       gb.defined() ? gb.mutable_data_ptr<float>() : nullptr, ws.mutable_data_ptr(),
+                                       bytes, stream_of(x)),
+             "nimble_layernorm_backward");
+    gg = gg.to(static_cast<at::ScalarType>(ctx->saved_data["gamma"].toInt()));
+    if (gb.defined()) gb = gb.to(static_cast<at::ScalarType>(beta_type));
+    return {gx, gg, gb, Tensor()};
+  }
+};
+
+Tensor layer_norm(const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta, double eps) {
+  TORCH_CHECK(x.is_cuda(), "layer_norm on B200 needs CUDA tensors; there is no CPU path");
+  dtype_of(x);
+  const int64_t d = x.dim() ? x.size(-1) : 0;
+  auto check = [&](const Tensor& p, const char* name) {
+    TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == d, "Expected ", name, " of shape (", d, ",), got ", p.sizes());
+    TORCH_CHECK_VALUE(p.device() == x.device(), name, " is on ", p.device(), ", x on ", x.device());
+    dtype_of(p);
+  };
+  check(gamma, "gamma");
+  if (beta) check(*beta, "beta");
+  TORCH_CHECK_VALUE(d > 0 && d <= kMaxNorm, "layer_norm takes rows of 1 to ", kMaxNorm, " elements, got ", d);
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || gamma.requires_grad() || (beta && beta->requires_grad())))
+    return LayerNormNode::apply(x, gamma, beta, eps);
+  return norm_forward(norm_args(x, gamma, beta), x, eps, nullptr);
+}
+
+// -------------------------------------------------------- token log probabilities
+struct RowsOut {
+  Tensor x, logprob, entropy, stats, top_logprob, top_id;  // x: the rows as read; stats: max, ln sum
+};
+
+RowsOut rows_forward(const Tensor& logits, const Tensor& tokens, int64_t ignore_index, int64_t top_k, int64_t status) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  RowsOut o;
+  int64_t n, v, pitch;
+  o.x = rows_of(logits, n, v, pitch);
+  const auto shape = logits.sizes().slice(0, logits.dim() - 1);
+  o.logprob = empty(shape, logits, at::kFloat);
+  o.entropy = empty(shape, logits, at::kFloat);
+  o.stats = empty({2, n}, logits, at::kFloat);
+  if (top_k) {
+    std::vector<int64_t> wide(shape.begin(), shape.end());
+    wide.push_back(top_k);
+    o.top_logprob = empty(wide, logits, at::kFloat);
+    o.top_id = empty(wide, logits, at::kLong);
+  }
+  float* stats = o.stats.mutable_data_ptr<float>();
+  check_rc(nimble_token_logprobs_forward(
+               o.x.const_data_ptr(), pitch, tokens.const_data_ptr<int64_t>(), n, v, dtype_of(logits), ignore_index,
+               static_cast<int>(top_k), o.logprob.mutable_data_ptr<float>(), o.entropy.mutable_data_ptr<float>(),
+               stats, stats + n, top_k ? o.top_logprob.mutable_data_ptr<float>() : nullptr,
+               top_k ? o.top_id.mutable_data_ptr<int64_t>() : nullptr, reinterpret_cast<int*>(status),
+               stream_of(logits)),
+           "nimble_token_logprobs_forward");
+  return o;
+}
+
+Tensor grad_rows(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; }
+const float* ptr_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+struct TokenLogProbsNode : torch::autograd::Function<TokenLogProbsNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, int64_t ignore_index,
+                               int64_t top_k, int64_t status) {
+    RowsOut o = rows_forward(logits, tokens, ignore_index, top_k, status);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({o.x, tokens, o.stats, o.entropy});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["shape"] = logits.sizes().vec();
+    variable_list out{o.logprob, o.entropy};
+    if (top_k) {
+      ctx->mark_non_differentiable({o.top_logprob, o.top_id});
+      out.push_back(o.top_logprob);
+      out.push_back(o.top_id);
+    }
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the log probabilities' backward is not differentiable itself");
+    if (!grads[0].defined() && !grads[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &tokens = saved[1], &stats = saved[2], &entropy = saved[3];
+    const c10::cuda::CUDAGuard guard(x.device());
+    const int64_t n = x.size(0), v = x.size(1), pitch = std::max(x.stride(0), v);
+    // Rows of whole 16 bytes where the logits have them, so that both sides use vectors.
+    const int64_t per16 = 16 / static_cast<int64_t>(x.element_size());
+    const int64_t grad_pitch = pitch % per16 == 0 ? (v + per16 - 1) / per16 * per16 : v;
+    Tensor g = empty({n, grad_pitch}, x, x.scalar_type());
+    const Tensor a = grad_rows(grads[0]), b = grad_rows(grads[1]);
+    const float* s = stats.const_data_ptr<float>();
+    check_rc(nimble_token_logprobs_backward(ptr_or_null(a), ptr_or_null(b), x.const_data_ptr(), pitch,
+                                            tokens.const_data_ptr<int64_t>(), s, s + n,
+                                            entropy.const_data_ptr<float>(), n, v, dtype_of(x),
+                                            ctx->saved_data["ignore_index"].toInt(), g.mutable_data_ptr(), grad_pitch,
+                                            stream_of(x)),
+             "nimble_token_logprobs_backward");
+    if (grad_pitch != v) g = g.narrow(1, 0, v);
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    if (shape.size() != 2) g = g.reshape(shape);
+    return {g, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t ignore_index, int64_t top_k,
+                         int64_t status) {
+  variable_list out;
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    out = TokenLogProbsNode::apply(logits, tokens, ignore_index, top_k, status);
+  } else {
+    RowsOut o = rows_forward(logits, tokens, ignore_index, top_k, status);
+    out = {o.logprob, o.entropy};
+    if (top_k) {
+      out.push_back(o.top_logprob);
+      out.push_back(o.top_id);
+    }
+  }
+  if (top_k) return py::make_tuple(out[0], out[1], out[2], out[3]);
+  return py::make_tuple(out[0], out[1], py::none(), py::none());
+}
+
+// ------------------------------------------------------------------------- AdamW
+const Tensor& tensor_in(PyObject* o, const char* what) {
+  TORCH_CHECK_VALUE(THPVariable_Check(o), what, " must be a tensor");
+  return THPVariable_Unpack(o);
+}
+
+// Items of a list or tuple, borrowed.
+struct Items {
+  py::object seq;
+  PyObject** at;
+  Py_ssize_t n;
+  explicit Items(const py::object& o) {
+    seq = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "expected a sequence of tensors"));
+    if (!seq) throw py::error_already_set();
+    at = PySequence_Fast_ITEMS(seq.ptr());
+    n = PySequence_Fast_GET_SIZE(seq.ptr());
+  }
+};
+
+constexpr int64_t kQuantBlock = 128;
+void check_quantized(const Tensor& codes, const Tensor& scales) {
+  TORCH_CHECK_VALUE(codes.scalar_type() == at::kFloat8_e4m3fn && codes.is_contiguous(),
+                    "8-bit moments are contiguous float8_e4m3fn codes");
+  TORCH_CHECK_VALUE(scales.scalar_type() == at::kFloat && scales.is_contiguous() &&
+                        scales.numel() == (codes.numel() + kQuantBlock - 1) / kQuantBlock,
+                    "8-bit moments need one contiguous float32 scale per ", kQuantBlock, " elements");
+  TORCH_CHECK_VALUE(codes.is_cuda() && scales.device() == codes.device(), "8-bit moments live on one CUDA device");
+}
+
+void adamw_step_many(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_,
+                     const py::object& copies_, int64_t step, double lr, double beta1, double beta2, double eps,
+                     double wd) {
+  const Items params(params_), grads(grads_), ms(m_), vs(v_);
+  std::optional<Items> copies;
+  if (!copies_.is_none()) copies.emplace(copies_);
+  TORCH_CHECK_VALUE(grads.n == params.n && ms.n == params.n && vs.n == params.n && (!copies || copies->n == params.n),
+                    "params, grads, exp_avgs, exp_avg_sqs and copies must have one entry per tensor");
+  TORCH_CHECK_VALUE(step >= 1, "step counts from 1, got ", step);
+  std::vector<nimble_adamw_tensor> rows;
+  rows.reserve(params.n);
+  std::unordered_set<const void*> seen;
+  std::vector<Tensor> keep;  // contiguous copies of gradients, until the launch is queued
+  std::optional<at::Device> dev;
+  bool eight = false;
+  auto launch = [&] {
+    if (rows.empty()) return;
+    const c10::cuda::CUDAGuard guard(*dev);
+    check_rc(nimble_adamw_step_many(rows.data(), static_cast<int>(rows.size()), eight ? 8 : 32, lr, beta1, beta2,
+                                    1.0 - std::pow(beta1, static_cast<double>(step)),
+                                    1.0 - std::pow(beta2, static_cast<double>(step)), eps, wd,
+                                    c10::cuda::getCurrentCUDAStream(dev->index()).stream()),
+             "nimble_adamw_step_many");
+  };
+  for (Py_ssize_t i = 0; i < params.n; ++i) {
+    if (grads.at[i] == Py_None) continue;
+    const Tensor& p = tensor_in(params.at[i], "a parameter");
+    const Tensor* g = &tensor_in(grads.at[i], "a gradient");
+    if (!dev) {
+      dev = p.device();
+      TORCH_CHECK_VALUE(p.is_cuda(), "adamw_step_many needs CUDA tensors; there is no CPU path");
+      eight = !THPVariable_Check(ms.at[i]);
+    }
+    const int64_t n = p.numel();
+    TORCH_CHECK_VALUE(p.scalar_type() == at::kFloat && p.is_contiguous(),
+                      "AdamW master weights must be contiguous float32 tensors");
+    const int gdt = dtype_or(*g);
+    TORCH_CHECK_VALUE(gdt >= 0 && g->numel() == n, "a gradient of ", g->numel(), " elements in ", g->scalar_type(),
+                      " for ", n, " weights");
+    TORCH_CHECK_VALUE(p.device() == *dev && g->device() == *dev, "all tensors of a step must be on one device");
+    if (!g->is_contiguous()) {
+      const c10::cuda::CUDAGuard guard(*dev);
+      keep.push_back(g->contiguous());
+      g = &keep.back();
+    }
+    nimble_adamw_tensor r{};
+    auto moment = [&](PyObject* o, void*& values, float*& scales) {
+      if (eight) {
+        TORCH_CHECK_VALUE(PyTuple_Check(o) && PyTuple_GET_SIZE(o) == 2,
+                          "moments are all fp32 tensors or all (codes, scales) pairs");
+        const Tensor& codes = tensor_in(PyTuple_GET_ITEM(o, 0), "codes");
+        const Tensor& s = tensor_in(PyTuple_GET_ITEM(o, 1), "scales");
+        check_quantized(codes, s);
+        TORCH_CHECK_VALUE(codes.numel() == n && codes.device() == *dev,
+                          "moments must have the sizes and the device of their weights");
+        values = codes.data_ptr();
+        scales = static_cast<float*>(s.data_ptr());
+      } else {
+        TORCH_CHECK_VALUE(THPVariable_Check(o), "moments are all fp32 tensors or all (codes, scales) pairs");
+        const Tensor& t = THPVariable_Unpack(o);
+        TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.is_contiguous(),
+                          "fp32 moments must be contiguous float32 tensors");
+        TORCH_CHECK_VALUE(t.numel() == n && t.device() == *dev,
+                          "moments must have the sizes and the device of their weights");
+        values = t.data_ptr();
+      }
+    };
+    moment(ms.at[i], r.exp_avg, r.exp_avg_scale);
+    moment(vs.at[i], r.exp_avg_sq, r.exp_avg_sq_scale);
+    if (copies && copies->at[i] != Py_None) {
+      const Tensor& c = tensor_in(copies->at[i], "a copy");
+      r.weights_copy_dtype = dtype_or(c);
+      TORCH_CHECK_VALUE(r.weights_copy_dtype >= 0 && c.numel() == n && c.is_contiguous() && c.device() == *dev,
+                        "a copy must be contiguous, on the device and of the size of its weights");
+      r.weights_copy = c.data_ptr();
+    }
+    if (n == 0) continue;
+    r.weights = static_cast<float*>(p.data_ptr());
+    r.grad = g->data_ptr();
+    r.n = n;
+    r.grad_dtype = gdt;
+    if (!seen.insert(r.weights).second) {  // listed twice: its second update follows the first
+      launch();
+      rows.clear();
+      seen.clear();
+      seen.insert(r.weights);
+    }
+    rows.push_back(r);
+  }
+  launch();
+}
+
+}  // namespace
+
+PYBIND11_MODULE(nimbleml_b200_host, m) {
+  m.doc() = "Host side of layer_norm, token_logprobs and adamw_step_many over the C ABI";
+  m.def("layer_norm", &layer_norm);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("adamw_step_many", &adamw_step_many);
+}

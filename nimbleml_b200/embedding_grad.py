@@ -13,11 +13,11 @@
 from __future__ import annotations
 
 import contextlib
-from array import array
 from typing import Iterable, NamedTuple, Optional, Sequence, Union
 
 import torch
 
+from nimbleml_b200._host import host
 from nimbleml_b200.kernels.fused_tied_crossentropy import _TORCH_TO_NIMBLE, _stream_ptr, native, status_word
 
 
@@ -102,7 +102,6 @@ def dequantize_moment(codes: torch.Tensor, scales: torch.Tensor, *, root: bool =
 Moment = Union[torch.Tensor, QuantizedMoment]
 
 
-@torch.no_grad()
 def adamw_step_many(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]],
                     exp_avgs: Sequence[Moment], exp_avg_sqs: Sequence[Moment], *, step: int,
                     learning_rate: float = 0.001, beta1: float = 0.9, beta2: float = 0.999, epsilon: float = 1e-8,
@@ -125,74 +124,8 @@ def adamw_step_many(params: Sequence[torch.Tensor], grads: Sequence[Optional[tor
     with 8-bit moments, the block of 128 it lies in. A captured step keeps the
     scalars it was captured with.
     """
-    n = len(params)
-    copies = copies if copies is not None else [None] * n
-    if not len(grads) == len(exp_avgs) == len(exp_avg_sqs) == len(copies) == n:
-        raise ValueError("params, grads, exp_avgs, exp_avg_sqs and copies must have one entry per tensor")
-    if step < 1:
-        raise ValueError("step counts from 1")
-    eight: Optional[bool] = None
-    dev = -1
-    rows, keep, seen = array("q"), [], set()
-    dtypes = _TORCH_TO_NIMBLE
-    f32 = torch.float32
-
-    def launch() -> None:
-        if not seen:
-            return
-        device = torch.device("cuda", dev)
-        with _on(device):
-            native.call("nimble_adamw_step_many", rows.buffer_info()[0], len(seen), 8 if eight else 32, learning_rate,
-                        beta1, beta2, 1.0 - beta1 ** step, 1.0 - beta2 ** step, epsilon, weight_decay,
-                        _stream_ptr(device))
-
-    for p, g, m, v, c in zip(params, grads, exp_avgs, exp_avg_sqs, copies):
-        if g is None:
-            continue
-        size = p.numel()
-        at = p.get_device()
-        if dev < 0:
-            dev, eight = at, not isinstance(m, torch.Tensor)
-            if dev < 0:
-                raise ValueError("adamw_step_many needs CUDA tensors; there is no CPU path")
-        if p.dtype is not f32 or not p.is_contiguous():
-            raise ValueError("AdamW master weights must be contiguous float32 tensors")
-        if g.dtype not in dtypes or g.numel() != size:
-            raise ValueError(f"a gradient of {g.numel()} elements in {g.dtype} for {size} weights")
-        if not g.is_contiguous():
-            g = g.contiguous()
-            keep.append(g)
-        if at != dev or g.get_device() != dev:
-            raise ValueError("all tensors of a step must be on one device")
-        ms = vs = 0
-        if eight:
-            if isinstance(m, torch.Tensor) or isinstance(v, torch.Tensor):
-                raise ValueError("moments are all fp32 tensors or all (codes, scales) pairs")
-            (m, m_scales), (v, v_scales) = m, v
-            _check_quantized(m, m_scales)
-            _check_quantized(v, v_scales)
-            ms, vs = m_scales.data_ptr(), v_scales.data_ptr()
-        elif not isinstance(m, torch.Tensor) or not isinstance(v, torch.Tensor):
-            raise ValueError("moments are all fp32 tensors or all (codes, scales) pairs")
-        elif m.dtype is not f32 or v.dtype is not f32 or not m.is_contiguous() or not v.is_contiguous():
-            raise ValueError("fp32 moments must be contiguous float32 tensors")
-        if m.numel() != size or v.numel() != size or m.get_device() != dev or v.get_device() != dev:
-            raise ValueError("moments must have the sizes and the device of their weights")
-        c_ptr = c_dt = 0
-        if c is not None:
-            if c.dtype not in dtypes or c.numel() != size or not c.is_contiguous() or c.get_device() != dev:
-                raise ValueError("a copy must be contiguous, on the device and of the size of its weights")
-            c_ptr, c_dt = c.data_ptr(), dtypes[c.dtype]
-        if size == 0:
-            continue
-        ptr = p.data_ptr()
-        if ptr in seen:  # listed twice: its second update follows the first
-            launch()
-            rows, seen = array("q"), set()
-        seen.add(ptr)
-        # One nimble_adamw_tensor: seven pointers, the size, two 32-bit dtypes.
-        rows.extend((ptr, g.data_ptr(), m.data_ptr(), v.data_ptr(), ms, vs, c_ptr, size, dtypes[g.dtype] | c_dt << 32))
-    launch()
+    host.adamw_step_many(params, grads, exp_avgs, exp_avg_sqs, copies, int(step), float(learning_rate), float(beta1),
+                         float(beta2), float(epsilon), float(weight_decay))
 
 
 class AdamW:

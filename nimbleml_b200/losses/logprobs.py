@@ -23,6 +23,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
+from nimbleml_b200._host import host
 from nimbleml_b200.kernels.fused_tied_crossentropy import (
     _NO_IGNORE,
     _TORCH_TO_NIMBLE,
@@ -78,70 +79,6 @@ def _refuse_double_backward() -> None:
         raise RuntimeError("the log probabilities' backward is not differentiable itself")
 
 
-def _rows_forward(x2d, tokens, ignore_index, top_k):
-    """(x2d as the kernel read it, (4, n) log probability, entropy, max, ln sum; alternatives)."""
-    dev = x2d.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _rows_forward(x2d, tokens, ignore_index, top_k)
-    n, v = x2d.shape
-    # Rows may be a view of wider ones; a broadcast or a transposed matrix is copied.
-    if x2d.stride(1) != 1 or (n > 1 and x2d.stride(0) < v):
-        x2d = x2d.contiguous()
-    out = torch.empty((4, n), dtype=torch.float32, device=dev)
-    top_lp = torch.empty((n, top_k), dtype=torch.float32, device=dev) if top_k else None
-    top_id = torch.empty((n, top_k), dtype=torch.int64, device=dev) if top_k else None
-    at = out.data_ptr()
-    native.call("nimble_token_logprobs_forward", x2d.data_ptr(), max(x2d.stride(0), v), tokens.data_ptr(), n, v,
-                _TORCH_TO_NIMBLE[x2d.dtype], ignore_index, top_k, at, at + 4 * n, at + 8 * n, at + 12 * n,
-                _ptr(top_lp), _ptr(top_id), status_word(dev).data_ptr(), _stream_ptr(dev))
-    if CHECK_BOUNDS:
-        check_status(dev)
-    return x2d, out, top_lp, top_id
-
-
-def _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index):
-    dev = x2d.device
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index)
-    n, v = x2d.shape
-    ld = max(x2d.stride(0), v)
-    # Rows of whole 16 bytes where the logits have them, so that both sides use vectors.
-    per16 = 16 // x2d.element_size()
-    pitch = -(-v // per16) * per16 if ld % per16 == 0 else v
-    g = torch.empty((n, pitch), dtype=x2d.dtype, device=dev)
-    a, b, at = _grad_rows(g_lp), _grad_rows(g_ent), out.data_ptr()
-    native.call("nimble_token_logprobs_backward", _ptr(a), _ptr(b), x2d.data_ptr(), ld, tokens.data_ptr(),
-                at + 8 * n, at + 12 * n, at + 4 * n, n, v, _TORCH_TO_NIMBLE[x2d.dtype], ignore_index, g.data_ptr(),
-                pitch, _stream_ptr(dev))
-    return g if pitch == v else g[:, :v]
-
-
-class _TokenLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, ignore_index, top_k):
-        v = logits.shape[-1]
-        x2d, out, top_lp, top_id = _rows_forward(logits if logits.ndim == 2 else logits.reshape(-1, v), tokens,
-                                                 ignore_index, top_k)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x2d, tokens, out)
-        ctx.meta = (ignore_index, logits.shape)
-        if top_k:
-            ctx.mark_non_differentiable(top_lp, top_id)
-        return out[0], out[1], top_lp, top_id
-
-    @staticmethod
-    def backward(ctx, g_lp, g_ent, *_):
-        _refuse_double_backward()
-        if g_lp is None and g_ent is None:
-            return None, None, None, None
-        x2d, tokens, out = ctx.saved_tensors
-        ignore_index, shape = ctx.meta
-        g = _rows_backward(g_lp, g_ent, x2d, tokens, out, ignore_index)
-        return g if len(shape) == 2 else g.reshape(shape), None, None, None
-
-
 def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = None, *, top_k: int = 0) -> TokenLogProbs:
     """Log probability of ``tokens`` under ``logits`` (..., classes), the entropy of each
     row and, with ``top_k`` (at most 64), its best classes.
@@ -168,19 +105,13 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     top_k = int(top_k)
     if not 0 <= top_k <= min(MAX_TOP_K, v):
         raise ValueError(f"top_k must lie in [0, {min(MAX_TOP_K, v)}], got {top_k}")
-    shape = shape[:-1]
-    ids = _token_ids(tokens, math.prod(shape), logits.device)
+    dev = logits.device
+    ids = _token_ids(tokens, math.prod(shape[:-1]), dev)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
-    if logits.requires_grad and torch.is_grad_enabled():
-        lp, ent, top_lp, top_id = _TokenLogProbs.apply(logits, ids, ign, top_k)
-    else:
-        _, out, top_lp, top_id = _rows_forward(logits if len(shape) == 1 else logits.reshape(-1, v), ids, ign, top_k)
-        lp, ent = out[0], out[1]
-    if len(shape) != 1:
-        lp, ent = lp.view(shape), ent.view(shape)
-        if top_k:
-            top_lp, top_id = top_lp.view(*shape, top_k), top_id.view(*shape, top_k)
-    return TokenLogProbs(lp, ent, top_lp, top_id)
+    out = TokenLogProbs(*host.token_logprobs(logits, ids, ign, top_k, status_word(dev).data_ptr()))
+    if CHECK_BOUNDS:
+        check_status(dev)
+    return out
 
 
 def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0, *,
