@@ -1888,6 +1888,7 @@ LpFwdLayout lp_fwd_layout(int64_t N, int64_t V) {
   return L;
 }
 
+constexpr int64_t kOneSlabBytes = 32 << 20;
 // The slab backward's workspace, then the row coefficients and the scale.
 struct LpBwdLayout {
   BwdLayout slabs;
@@ -1896,7 +1897,10 @@ struct LpBwdLayout {
 };
 LpBwdLayout lp_bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t slab_bytes) {
   LpBwdLayout L;
-  L.slabs = bwd_layout(N, d, V, dtype, slab_bytes);
+  // G of at most kOneSlabBytes is one slab (launches count there, memory does not):
+  // only larger ones are kept to half of the N x V logits and less.
+  const bool whole = elem_size(dtype) * N * round_up(V, kBN) > kOneSlabBytes;
+  L.slabs = bwd_layout(N, d, V, dtype, slab_bytes, whole);
   L.splits = dh_splits(N, d, L.slabs.slab);
   size_t off = L.slabs.total;
   if (L.splits > 1) {  // the runs' partial grad_hidden in place of the slabs' one

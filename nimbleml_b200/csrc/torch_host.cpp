@@ -247,6 +247,49 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t ign
   return py::make_tuple(out[0], out[1], py::none(), py::none());
 }
 
+// ------------------------------------------------ tied log probabilities (one shard)
+// Results of a shard that is the whole vocabulary (3, N), or its statistics (4, N).
+Tensor tied_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_t v_offset, int64_t ignore_index,
+                    bool whole, int64_t status) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
+  Tensor out = empty({whole ? 3 : 4, n}, h, at::kFloat);
+  size_t bytes = 0;
+  check_rc(nimble_tied_logprobs_forward_workspace_size(n, d, v, dtype_of(h), &bytes),
+           "nimble_tied_logprobs_forward_workspace_size");
+  const Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, h, at::kByte);
+  float* o = out.mutable_data_ptr<float>();
+  check_rc(nimble_tied_logprobs_forward(h.const_data_ptr(), w.const_data_ptr(), tokens.const_data_ptr<int64_t>(), n, d,
+                                        v, v_offset, dtype_of(h), ignore_index, whole ? nullptr : o,
+                                        whole ? o : nullptr, whole ? o + n : nullptr, whole ? o + 2 * n : nullptr,
+                                        ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status), stream_of(h)),
+           "nimble_tied_logprobs_forward");
+  return out;
+}
+
+// Fills grad_hidden and fills or adds to grad_weights, those that are given.
+void tied_backward(const std::optional<Tensor>& g_logprob, const std::optional<Tensor>& g_entropy, const Tensor& h,
+                   const Tensor& w, const Tensor& tokens, const Tensor& lse, const Tensor& entropy, int64_t v_offset,
+                   int64_t vocab_size, int64_t ignore_index, const std::optional<Tensor>& grad_hidden,
+                   const std::optional<Tensor>& grad_weights, bool accumulate, int64_t slab_bytes, int64_t status) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
+  const int dt = dtype_of(h);
+  const Tensor a = g_logprob ? grad_rows(*g_logprob) : Tensor(), b = g_entropy ? grad_rows(*g_entropy) : Tensor();
+  size_t bytes = 0;
+  check_rc(nimble_tied_logprobs_backward_workspace_size(n, d, v, dt, static_cast<size_t>(slab_bytes), &bytes),
+           "nimble_tied_logprobs_backward_workspace_size");
+  const Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, h, at::kByte);
+  check_rc(nimble_tied_logprobs_backward(
+               ptr_or_null(a), ptr_or_null(b), h.const_data_ptr(), w.const_data_ptr(),
+               tokens.const_data_ptr<int64_t>(), lse.const_data_ptr<float>(), entropy.const_data_ptr<float>(), n, d, v,
+               v_offset, vocab_size, ignore_index, dt, grad_hidden ? grad_hidden->data_ptr() : nullptr,
+               grad_hidden ? dtype_of(*grad_hidden) : dt, grad_weights ? grad_weights->data_ptr() : nullptr,
+               grad_weights ? dtype_of(*grad_weights) : dt, accumulate ? 1 : 0, static_cast<size_t>(slab_bytes),
+               ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status), stream_of(h)),
+           "nimble_tied_logprobs_backward");
+}
+
 // ------------------------------------------------------------------------- AdamW
 const Tensor& tensor_in(PyObject* o, const char* what) {
   TORCH_CHECK_VALUE(THPVariable_Check(o), what, " must be a tensor");
@@ -371,8 +414,10 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
 }  // namespace
 
 PYBIND11_MODULE(nimbleml_b200_host, m) {
-  m.doc() = "Host side of layer_norm, token_logprobs and adamw_step_many over the C ABI";
+  m.doc() = "Host side of layer_norm, the token log probabilities and adamw_step_many over the C ABI";
   m.def("layer_norm", &layer_norm);
   m.def("token_logprobs", &token_logprobs);
+  m.def("tied_forward", &tied_forward);
+  m.def("tied_backward", &tied_backward);
   m.def("adamw_step_many", &adamw_step_many);
 }

@@ -9,28 +9,29 @@ terms of every token instead:
   log-sum-exp, the token's log probability, the entropy and the ``k`` best
   classes.
 * ``tied_token_logprobs(hidden, weights, tokens)`` straight from the hidden
-  states and the tied matrix. As in ``CrossEntropyLoss.forward_tied`` no N x V
-  buffer exists: the forward keeps the lse and the entropy of each token, the
-  backward recomputes the logits slab by slab.
+  states and the tied matrix. As in ``CrossEntropyLoss.forward_tied`` the logits
+  are not kept: the forward keeps the lse and the entropy of each token, the
+  backward recomputes the logits slab by slab (a slab holds at most half of them,
+  or all where they take 32 MiB or less).
 
 Both are differentiable in the log probabilities and in the entropies:
 d/dx_j (a logp_t + b H) = a [j = t] - p_j (a + b (H + log p_j)).
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import NamedTuple, Optional
 
 import torch
 
+from nimbleml_b200 import vocab_parallel
 from nimbleml_b200._host import host
 from nimbleml_b200.kernels.fused_tied_crossentropy import (
     _NO_IGNORE,
-    _TORCH_TO_NIMBLE,
     CHECK_BOUNDS,
     SLAB_BYTES,
     _stream_ptr,
-    _workspace,
     as_label_indices,
     check_status,
     compute_dtype_of,
@@ -55,16 +56,9 @@ class TokenLogProbs(NamedTuple):
     top_ids: Optional[torch.Tensor] = None
 
 
-def _grad_rows(grad: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if grad is None:
-        return None
-    if grad.dtype != torch.float32:
-        grad = grad.float()
-    return grad if grad.is_contiguous() else grad.contiguous()
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _on(device: torch.device):
+    """Makes ``device`` current where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _token_ids(tokens, n: int, device: torch.device) -> torch.Tensor:
@@ -114,24 +108,10 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     return out
 
 
-def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0, *,
-                        whole: Optional[int] = None) -> torch.Tensor:
+def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0) -> torch.Tensor:
     """(4, N) statistics of one weight shard: a reference logit, sum 2^d, sum d 2^d (d = (s - reference) log2 e) and the
-    token's logit (0 where the shard does not hold it). With ``whole`` (the ignore index) the shard is
-    the whole vocabulary and the result is (3, N): log probabilities, entropies, lse."""
-    n, d = h.shape
-    v_local = w.shape[0]
-    dt = compute_dtype_of(h)
-    dev = h.device
-    out = torch.empty((4 if whole is None else 3, n), dtype=torch.float32, device=dev)
-    ws_bytes = native.tied_logprobs_forward_workspace_size(n, d, v_local, dt)
-    ws = _workspace(ws_bytes, dev)
-    at = out.data_ptr()
-    results = (at, None, None, None) if whole is None else (None, at, at + 4 * n, at + 8 * n)
-    native.call("nimble_tied_logprobs_forward", h.data_ptr(), w.data_ptr(), tokens.data_ptr(), n, d, v_local,
-                vocab_offset, dt, _NO_IGNORE if whole is None else whole, *results, ws.data_ptr(), ws_bytes,
-                status_word(dev).data_ptr(), _stream_ptr(dev))
-    return out
+    token's logit (0 where the shard does not hold it)."""
+    return host.tied_forward(h, w, tokens, vocab_offset, _NO_IGNORE, False, status_word(h.device).data_ptr())
 
 
 def combine_logprob_stats(stats: torch.Tensor, tokens: torch.Tensor, vocab_size: int, ignore_index: int):
@@ -148,17 +128,9 @@ def combine_logprob_stats(stats: torch.Tensor, tokens: torch.Tensor, vocab_size:
 def shard_logprob_backward(g_lp, g_ent, h, w, tokens, lse, ent, *, vocab_offset=0, vocab_size=None, ignore_index,
                            grad_hidden=None, grad_weights=None, accumulate=False):
     """Fills ``grad_hidden`` (this shard's partial) and fills or adds to ``grad_weights``, those that are given."""
-    n, d = h.shape
-    v_local = w.shape[0]
-    dt = compute_dtype_of(h)
-    dev = h.device
-    ws = _workspace(native.tied_logprobs_backward_workspace_size(n, d, v_local, dt, SLAB_BYTES), dev)
-    native.call("nimble_tied_logprobs_backward", _ptr(g_lp), _ptr(g_ent), h.data_ptr(), w.data_ptr(),
-                tokens.data_ptr(), lse.data_ptr(), ent.data_ptr(), n, d, v_local, vocab_offset,
-                v_local if vocab_size is None else vocab_size, ignore_index, dt, _ptr(grad_hidden),
-                _TORCH_TO_NIMBLE[grad_hidden.dtype] if grad_hidden is not None else dt, _ptr(grad_weights),
-                _TORCH_TO_NIMBLE[grad_weights.dtype] if grad_weights is not None else dt, 1 if accumulate else 0,
-                SLAB_BYTES, ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream_ptr(dev))
+    host.tied_backward(g_lp, g_ent, h, w, tokens, lse, ent, vocab_offset, w.shape[0] if vocab_size is None else vocab_size,
+                       ignore_index, grad_hidden, grad_weights, accumulate, SLAB_BYTES,
+                       status_word(h.device).data_ptr())
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -169,8 +141,6 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group):
     """(h, w as the kernels read them, (3, n) log probability, entropy, lse)."""
-    from nimbleml_b200 import vocab_parallel
-
     dev = hidden.device
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
@@ -184,7 +154,7 @@ def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_siz
         poll_status(dev)
     world = vocab_parallel.world_size(group)
     if world == 1 and vocab_offset == 0 and w.shape[0] == vocab_size:
-        out = shard_logprob_stats(h, w, tokens, whole=ignore_index)
+        out = host.tied_forward(h, w, tokens, 0, ignore_index, True, status_word(dev).data_ptr())
     else:
         part = shard_logprob_stats(h, w, tokens, vocab_offset)
         if world > 1:
@@ -211,8 +181,6 @@ class _TiedTokenLogProbs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_lp, g_ent):
-        from nimbleml_b200 import vocab_parallel
-
         _refuse_double_backward()
         none = (None,) * 6
         if g_lp is None and g_ent is None:
@@ -222,7 +190,7 @@ class _TiedTokenLogProbs(torch.autograd.Function):
         buf = ctx.grad_buffer
         dev = h.device
         world = vocab_parallel.world_size(group)
-        with torch.cuda.device(dev):
+        with _on(dev):
             gh = gw = None
             if ctx.needs_input_grad[0]:
                 gh = torch.empty(h.shape, dtype=vocab_parallel.dh_reduce_dtype(h.dtype) if world > 1 else h.dtype,
@@ -234,7 +202,7 @@ class _TiedTokenLogProbs(torch.autograd.Function):
             watch = not torch.cuda.is_current_stream_capturing()
             if watch:
                 poll_status(dev)
-            shard_logprob_backward(_grad_rows(g_lp), _grad_rows(g_ent), h, w, tokens, out[2], out[1],
+            shard_logprob_backward(g_lp, g_ent, h, w, tokens, out[2], out[1],
                                    vocab_offset=vocab_offset, vocab_size=vocab_size, ignore_index=ignore_index,
                                    grad_hidden=gh, grad_weights=gw, accumulate=buf is not None)
             if watch:
