@@ -565,6 +565,205 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   }
 }
 
+// ------------------------------------------------------------ forward, short rows
+// Rows of at most kShortVecs 16-byte vectors (4096 16-bit logits, 2048 fp32 ones): a
+// warp has a row, eight rows a block, nothing waits for another warp. (A block of
+// 256 threads lives about 4 us for a short row, mostly latency: 8000 x 2000 fp16
+// took 34 us, 68 us with 5 alternatives; by warps 12.5 and 22.7.) The top k is found
+// as above, from the maxima of single vectors.
+constexpr int kShortVecs = 512;
+constexpr int kLaneVecs = kShortVecs / 32;
+constexpr int kShortWarps = 8;
+constexpr int kShortCap = 512;
+// Fewer rows take a block each: a warp alone is slower than a block where there are
+// no other rows to hide it (600 / 1200 / 8000 rows of 2000 fp16 logits: 7.0 / 8.4 / 34
+// us by blocks, 7.1 / 7.2 / 12.5 by warps; with 64 alternatives 12.4 / 17.8 / 84
+// against 16.0 / 16.7 / 43).
+constexpr int64_t kShortRows = 1024;
+constexpr int kShortWater = 128;  // of the second scan, whose steps offer at most 128 logits
+
+struct ShortTopK {
+  uint64_t keys[kShortCap];
+  uint64_t best[kMaxTopK];
+  float vec_max[kLaneVecs][32];
+  int count;
+};
+
+// As topk_prune, by one warp; returns the threshold too.
+__device__ int short_prune(ShortTopK& sh, int n, int k, uint64_t& tau) {
+  const int lane = threadIdx.x & 31, left = min(n, k);
+  __syncwarp();
+  for (int i = lane; i < n; i += 32) {
+    const uint64_t key = sh.keys[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += sh.keys[j] > key;
+    if (rank < k) sh.best[rank] = key;
+  }
+  __syncwarp();
+  for (int i = lane; i < left; i += 32) sh.keys[i] = sh.best[i];
+  if (lane == 0) sh.count = left;
+  __syncwarp();
+  if (n >= k) tau = sh.best[k - 1];
+  return left;
+}
+
+template <typename T, bool kTopK>
+__global__ void __launch_bounds__(32 * kShortWarps)
+logprobs_short_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens, int64_t N, int V,
+                      int64_t ignore_index, int k, float* __restrict__ out_logp, float* __restrict__ out_ent,
+                      float* __restrict__ out_max, float* __restrict__ out_logsum, float* __restrict__ top_logp,
+                      int64_t* __restrict__ top_ids, int* status) {
+  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kU = 4;
+  extern __shared__ __align__(16) uint8_t dyn[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ShortTopK& sh = reinterpret_cast<ShortTopK*>(dyn)[warp];  // dereferenced only with kTopK
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kShortWarps + warp;
+  if (row >= N) return;
+  const int64_t tok = tokens[row];
+  if (tok == ignore_index) {  // the row's logits are not read
+    if (lane == 0) out_logp[row] = out_ent[row] = out_max[row] = out_logsum[row] = 0.0f;
+    if constexpr (kTopK)
+      for (int j = lane; j < k; j += 32) {
+        top_logp[row * k + j] = -INFINITY;
+        top_ids[row * k + j] = -1;
+      }
+    return;
+  }
+  const T* r = x + row * ld;
+  const int head = min(V, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(r) & 15)) & 15) / sizeof(T)));
+  const int nvec = (V - head) / kVec;
+  const int tail0 = head + nvec * kVec;
+  const uint4* r4 = reinterpret_cast<const uint4*>(r + head);
+  SoftStats acc;
+  float group_max[kU] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // of vectors s0 + i
+  for (int s0 = 0; 32 * s0 < nvec; s0 += kU) {
+    uint4 raw[kU];
+    auto vec_at = [&](int i) { return (s0 + i) * 32 + lane; };
+#pragma unroll
+    for (int i = 0; i < kU; ++i) raw[i] = vec_at(i) < nvec ? __ldg(r4 + vec_at(i)) : no_vec<T>();
+    float hi;
+    if constexpr (kTopK) {
+      hi = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kU; ++i) {
+        const uint4 one[1] = {raw[i]};
+        const float v = vec_max<T, 1>(one);
+        sh.vec_max[s0 + i][lane] = v;  // s0 + i < kLaneVecs: nvec <= kShortVecs, a multiple of 32 kU
+        group_max[i] = fmaxf(group_max[i], v);
+        hi = fmaxf(hi, v);
+      }
+    } else {
+      hi = vec_max<T, kU>(raw);
+    }
+    if (!acc.template add_vecs<T, kU>(raw, hi)) {
+#pragma unroll 1
+      for (int i = 0; i < kU; ++i)
+#pragma unroll 1
+        for (int j = 0; j < kVec && vec_at(i) < nvec; ++j) acc.add(to_f<T>(r[head + vec_at(i) * kVec + j]));
+    }
+  }
+  const bool ragged = lane < head + (V - tail0);
+  const int ragged_j = lane < head ? lane : tail0 + (lane - head);
+  float ragged_v = -INFINITY;
+  if (ragged) {
+    ragged_v = to_f<T>(r[ragged_j]);
+    acc.add(ragged_v);
+  }
+  __syncwarp();
+  lanes_merge(acc, 32);
+  const RowResult res = row_result(acc);
+  if (lane == 0) {
+    const bool bad = tok < 0 || tok >= V;
+    if (bad && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
+    out_logp[row] = bad ? __int_as_float(0x7fc00000) : token_logprob(to_f<T>(r[tok]), res.max, res.logsum);
+    out_ent[row] = res.entropy;
+    out_max[row] = res.max;
+    out_logsum[row] = res.logsum;
+  }
+  if constexpr (kTopK) {
+    const int lanes_of = (nvec + 31) / 32;  // vectors a lane
+    // Largest 16-bit prefix of an ordered value that the maxima of k groups of
+    // vectors reach: a lane's vectors for up to 16 alternatives, four groups a lane
+    // for more. A group without vectors counts for nothing.
+    uint32_t reach[kU];
+#pragma unroll
+    for (int i = 0; i < kU; ++i) reach[i] = i * 32 + lane < nvec ? ordered(group_max[i]) : 0u;
+    const uint32_t of_lane = max(max(reach[0], reach[1]), max(reach[2], reach[3]));
+    uint32_t prefix = 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t t = prefix | (1u << bit);
+      int count = 0;
+      if (k <= 16) {
+        count = __popc(__ballot_sync(0xffffffffu, of_lane >= (t << 16)));
+      } else {
+#pragma unroll
+        for (int i = 0; i < kU; ++i) count += __popc(__ballot_sync(0xffffffffu, reach[i] >= (t << 16)));
+      }
+      if (count >= k) prefix = t;
+    }
+    float tau_v = prefix <= 0x007Fu ? -INFINITY : unordered(prefix << 16);
+    uint64_t tau = 0;
+    auto offer = [&](float v, uint32_t col) {
+      if (!(v >= tau_v)) return;
+      const uint64_t key = make_key(v, col);
+      if (key <= tau) return;
+      const int slot = atomicAdd(&sh.count, 1);
+      if (slot < kShortCap) sh.keys[slot] = key;
+    };
+    if (lane == 0) sh.count = 0;
+    __syncwarp();
+    if (ragged) offer(ragged_v, ragged_j);
+#pragma unroll 1
+    for (int s = 0; s < lanes_of; ++s) {
+      const int q = s * 32 + lane;
+      if (q >= nvec || !(sh.vec_max[s][lane] >= tau_v)) continue;
+      const uint4 raw = __ldg(r4 + q);
+#pragma unroll 1
+      for (uint32_t mask = vec_at_least<T>(raw, tau_v); mask != 0; mask &= mask - 1) {
+        const int j = __ffs(mask) - 1;
+        offer(vec_elem<T>(raw, j), head + q * kVec + j);
+      }
+    }
+    __syncwarp();
+    int kept = sh.count;
+    __syncwarp();
+    if (kept <= kShortCap) {
+      kept = short_prune(sh, kept, k, tau);
+    } else {
+      // More candidates than room (many equal logits): scan the row again from the
+      // threshold that those at hand give, cutting back between steps.
+      short_prune(sh, kShortCap, k, tau);
+      tau -= 1;
+      tau_v = key_value(tau + 1);
+      if (lane == 0) sh.count = 0;
+      __syncwarp();
+      kept = 0;
+      for (int j0 = 0; j0 < V; j0 += 128) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = j0 + e * 32 + lane;
+          if (j < V) offer(to_f<T>(r[j]), j);
+        }
+        __syncwarp();
+        kept = sh.count;
+        __syncwarp();
+        if (kept > kShortWater) {
+          kept = short_prune(sh, kept, k, tau);
+          tau_v = key_value(tau);
+        }
+      }
+      kept = short_prune(sh, kept, k, tau);
+    }
+    for (int j = lane; j < k; j += 32) {
+      const bool have = j < kept;  // fewer than k only where logits are NaN
+      top_logp[row * k + j] = have ? token_logprob(key_value(sh.keys[j]), res.max, res.logsum) : -INFINITY;
+      top_ids[row * k + j] = have ? static_cast<int64_t>(key_col(sh.keys[j])) : -1;
+    }
+  }
+}
+
 // ------------------------------------------------------------------ backward
 // grad = a [j = t] - p (a + b H + b log p), rows with an ignored or
 // out-of-range token zero. A block handles kGradVecs vectors a thread of one
@@ -697,13 +896,28 @@ extern "C" int nimble_token_logprobs_forward(const void* logits, int64_t row_pit
   if (n_rows == 0) return NIMBLE_OK;
   if (!tokens || !out_logprob || !out_entropy || !out_max || !out_logsum || (top_k > 0 && (!top_logprobs || !top_ids)))
     return fail(NIMBLE_ERR_INVALID_ARG, "null pointer argument");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n_classes * elem_size(dtype) <= kShortVecs * 16 && n_rows >= kShortRows) {
+    if (n_rows > static_cast<int64_t>(INT32_MAX)) return fail(NIMBLE_ERR_INVALID_ARG, "n_rows exceeds 2^31 - 1");
+    const unsigned grid = static_cast<unsigned>((n_rows + kShortWarps - 1) / kShortWarps);
+    const size_t smem = top_k > 0 ? sizeof(ShortTopK) * kShortWarps : 0;
+    NIMBLE_DISPATCH(dtype, T, {
+      auto kern = top_k > 0 ? logprobs_short_kernel<T, true> : logprobs_short_kernel<T, false>;
+      if (smem) NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      kern<<<grid, 32 * kShortWarps, smem, s>>>(static_cast<const T*>(logits), row_pitch, tokens, n_rows,
+                                                static_cast<int>(n_classes), ignore_index, top_k, out_logprob,
+                                                out_entropy, out_max, out_logsum, top_logprobs, top_ids, status);
+    });
+    NIMBLE_CUDA_TRY(cudaGetLastError());
+    return NIMBLE_OK;
+  }
   const int parts = row_parts(n_rows, n_classes);
   if (n_rows > INT32_MAX / parts) return fail(NIMBLE_ERR_INVALID_ARG, "n_rows exceeds 2^31 - 1");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(n_rows * parts));
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = top_k > 0 ? sizeof(TopKShared) : 0;
-  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts;

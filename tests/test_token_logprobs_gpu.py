@@ -103,7 +103,9 @@ def check_grad(got, x, tokens, a, b):
 
 
 SHAPES = [(1, 1), (3, 2), (2, 7), (5, 100), (33, 1001), (4, 2047), (3, 2304), (300, 4099), (6, 50257), (2, 128259),
-          (700, 8200)]
+          (700, 8200),
+          # 1024 rows and more of at most 8 KB: a warp a row.
+          (1024, 1), (1030, 7), (1100, 130), (1025, 1001), (1027, 2047), (1033, 2049), (1026, 4096), (1024, 4104)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -165,7 +167,7 @@ def test_strides(dtype, layout):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,v", [(3, 300), (2, 9000), (400, 9000)])
+@pytest.mark.parametrize("rows,v", [(3, 300), (2, 9000), (400, 9000), (1040, 300), (1030, 2043), (1025, 4091)])
 def test_masks_ties_and_orders(dtype, rows, v):
     """-inf masks, a row of -inf only, the type's lowest value, ties, and rows that rise or fall to their end."""
     from nimbleml_b200.losses import token_logprobs
@@ -201,17 +203,19 @@ def test_masks_ties_and_orders(dtype, rows, v):
         check_grad(gx, y, tokens, a, b)
 
 
-def test_nan_inf_ignored_and_bad_tokens():
+@pytest.mark.parametrize("rows", [6, 1030])
+def test_nan_inf_ignored_and_bad_tokens(rows):
     from nimbleml_b200.kernels.fused_tied_crossentropy import check_status
     from nimbleml_b200.losses import token_logprobs
 
-    x, tokens, _ = make_logits(6, 5000, torch.float32, 9)
+    n = 5000 if rows == 6 else 2000
+    x, tokens, _ = make_logits(rows, n, torch.float32, 9)
     x[0] = torch.nan  # ignored: not read
     tokens[0] = IGN
     x[1, 17] = torch.inf
-    x[2, 4999] = torch.nan
-    x[3, :4000] = -torch.inf
-    x[3, 4500] = torch.nan
+    x[2, n - 1] = torch.nan
+    x[3, :n - 1000] = -torch.inf
+    x[3, n - 500] = torch.nan
     leaf = x.detach().requires_grad_()
     r = token_logprobs(leaf, tokens, IGN, top_k=5)
     assert r.logprobs[0] == 0 and r.entropy[0] == 0
@@ -221,7 +225,7 @@ def test_nan_inf_ignored_and_bad_tokens():
     (gx,) = torch.autograd.grad(r.logprobs.sum(), leaf)
     assert (gx[0] == 0).all() and torch.isfinite(gx[4:]).all()
     check_status(x.device)
-    tokens[5] = 5000
+    tokens[5] = n
     leaf = x.detach().requires_grad_()
     r = token_logprobs(leaf, tokens, IGN)
     assert torch.isnan(r.logprobs[5]) and torch.isfinite(r.logprobs[4])
