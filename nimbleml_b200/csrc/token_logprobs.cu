@@ -40,9 +40,10 @@ constexpr float kLn2 = 0.6931471805599453f;
 // before (fp32 ends at 2^-149), and 0 * -inf must not become NaN.
 constexpr float kMinD = -1.0e4f;
 
-// Beyond this size two different logits are so far apart that the smaller one's
-// weight is zero, and products with log2 e may overflow: weights are 1 or 0.
-constexpr float kHuge = 1.0e30f;
+// References of this size and more (bf16 and fp32 logits only) are not taken as
+// f log2 e rounded, which would leave a rest of 0.1 and more, and overflow in the
+// end: d is (x - f) log2 e there, logit by logit.
+constexpr float kPlain = 1048576.0f;  // 2^20
 
 // Max of n vectors' logits, NaN left aside. 16-bit logits are compared in pairs
 // before they are widened.
@@ -113,55 +114,54 @@ __device__ __forceinline__ uint32_t vec_at_least(const uint4& raw, float t) {
   }
   return mask;
 }
-// Running statistics of a set of logits: max m, reference f (r = f log2 e), s, u. A
-// NaN makes s and u NaN; a set of -inf only (or the empty set) has m = f = -inf and
-// s = u = 0.
+// What a reference's rounding left of it, in powers of two.
+__device__ __forceinline__ float rest_of(float f) {
+  return fabsf(f) < kPlain ? fmaf(f, kLog2e, -__fmul_rn(f, kLog2e)) : 0.0f;
+}
+
+// Running statistics of a set of logits: max m, reference f (r = f log2 e rounded), s,
+// u. A NaN makes s and u NaN; a set of -inf only (or the empty set) has m = f = -inf
+// and s = u = 0.
 struct SoftStats {
   static constexpr float kLag = 16.0f;  // most that a logit's d may exceed zero
   float f = -INFINITY, r = -INFINITY, s = 0.0f, u = 0.0f, m = -INFINITY;
 
-  // d of one reference in terms of another that is not below it.
-  __device__ __forceinline__ static float shift(float f_low, float r_low, float f_high, float r_high) {
-    const float d = r_low - r_high;
-    return f_low == f_high ? 0.0f : (d > kMinD ? d : kMinD);  // NaN (both overflowed): far apart
+  __device__ __forceinline__ bool plain() const { return fabsf(f) < kPlain; }
+  // d of one reference in terms of another that is not below it; NaN (infinities) and
+  // all that is too far for a weight is kMinD.
+  __device__ __forceinline__ static float shift(float low, float high) {
+    const float d = (low - high) * kLog2e + (rest_of(high) - rest_of(low));
+    return low == high ? 0.0f : (d > kMinD ? d : kMinD);
   }
   __device__ __forceinline__ void raise(float f2) {
-    const float r2 = f2 * kLog2e;
-    const float d = shift(f, r, f2, r2);
+    const float d = shift(f, f2);
     const float w = ex2(d);
     u = (u + s * d) * w;
     s *= w;
     f = f2;
-    r = r2;
+    r = __fmul_rn(f2, kLog2e);
   }
   __device__ __forceinline__ bool too_low(float v) const {
-    return v > f && (fmaf(v, kLog2e, -r) > kLag || !(fabsf(f) < kHuge));
+    return v > f && (plain() ? fmaf(v, kLog2e, -r) : (v - f) * kLog2e) > kLag;
   }
   // Any logit.
   __device__ __forceinline__ void add(float v) {
     m = fmaxf(m, v);
     if (too_low(v)) raise(v);
-    float d = 0.0f, e;
-    if (fabsf(f) < kHuge) {
-      d = fmaf(v, kLog2e, -r);
-      e = ex2(d);
-    } else if (v == f) {  // huge: weight 1; -inf: 0; +inf: NaN
-      e = f == -INFINITY ? 0.0f : 1.0f + (f - f);
-    } else {  // far below, or NaN
-      e = v != v ? v : 0.0f;
-    }
+    // Nothing but -inf and NaN so far: 2^v. A reference of +inf: NaN for +inf.
+    const float d = plain() ? fmaf(v, kLog2e, -r) : (f == -INFINITY ? v : (v - f) * kLog2e);
+    const float e = ex2(d);
     s += e;
     u = fmaf(e, fmaxf(d, kMinD), u);
   }
-  // n vectors of logits whose max is hi; false (and nothing done) where weights
-  // are not to be taken as exponentials (huge logits).
+  // n vectors of logits whose max is hi; false (and nothing summed) where they have to
+  // be added one by one.
   template <typename T, int n>
   __device__ __forceinline__ bool add_vecs(const uint4 (&raw)[n], float hi) {
     constexpr int kPairs = 8 / sizeof(T);
-    if (hi >= kHuge) return false;
     m = fmaxf(m, hi);
     if (too_low(hi)) raise(hi);
-    if (fabsf(f) >= kHuge && f != -INFINITY) return false;
+    if (!plain() && f != -INFINITY) return false;
     const float2 l2 = make_float2(kLog2e, kLog2e);
     const float nr1 = f == -INFINITY ? 0.0f : -r;  // nothing but -inf and NaN so far
     const float2 nr = make_float2(nr1, nr1);
@@ -190,7 +190,7 @@ struct SoftStats {
       s += s2;
       u += u2;
     } else {
-      const float d = shift(f2, f2 * kLog2e, f, r);
+      const float d = shift(f2, f);
       const float w = ex2(d);
       u += (u2 + s2 * d) * w;
       s += s2 * w;
@@ -224,7 +224,7 @@ struct RowResult {
 __device__ __forceinline__ RowResult row_result(const SoftStats& a) {
   if (a.m == -INFINITY && a.s == 0.0f) return {-INFINITY, 0.0f, 0.0f};
   const float ls = logf(a.s);
-  const float c = fabsf(a.f) < kHuge ? kLn2 * fmaf(a.f, kLog2e, -a.r) : 0.0f;
+  const float c = kLn2 * rest_of(a.f);
   return {a.m, (a.f == a.m ? 0.0f : a.f - a.m) + (ls - c), ls - kLn2 * (a.u / a.s)};
 }
 // A row of -inf only gives every token -inf instead of NaN.

@@ -187,11 +187,14 @@ class AdamW:
 
     def _step_alone(self, i: int, g: torch.Tensor) -> None:
         p, m, v, c = self.params[i], self.m[i], self.v[i], self.copies[i]
-        native.call("nimble_adamw_step", p.data_ptr(), g.data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
-                    v.data_ptr(), p.numel(), self.lr, self.beta1, self.beta2, 1.0 - self.beta1 ** self.t,
-                    1.0 - self.beta2 ** self.t, self.epsilon, self.weight_decay,
-                    c.data_ptr() if c is not None else None, _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0,
-                    _stream_ptr(p.device))
+        if not p.is_cuda or any(t is not None and t.device != p.device for t in (g, m, v, c)):
+            raise ValueError("AdamW needs its weights, gradients, moments and copies on one CUDA device")
+        with _on(p.device):
+            native.call("nimble_adamw_step", p.data_ptr(), g.data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
+                        v.data_ptr(), p.numel(), self.lr, self.beta1, self.beta2, 1.0 - self.beta1 ** self.t,
+                        1.0 - self.beta2 ** self.t, self.epsilon, self.weight_decay,
+                        c.data_ptr() if c is not None else None, _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0,
+                        _stream_ptr(p.device))
 
     def zero_grad(self, set_to_none: bool = True):
         for p in self.params:

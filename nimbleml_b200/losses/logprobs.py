@@ -31,6 +31,7 @@ from nimbleml_b200.kernels.fused_tied_crossentropy import (
     _NO_IGNORE,
     CHECK_BOUNDS,
     SLAB_BYTES,
+    _status_words,
     _stream_ptr,
     as_label_indices,
     check_status,
@@ -68,6 +69,14 @@ def _token_ids(tokens, n: int, device: torch.device) -> torch.Tensor:
     return as_label_indices(tokens, batch_size=n, device=device)
 
 
+def _status_ptr(device: torch.device) -> int:
+    """Address of the device's status word, which a captured launch must find in place: made by the first
+    call on a device, it would otherwise lie in the graph's own memory."""
+    if device.index not in _status_words and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("call the operator once on this device before capturing it into a CUDA graph")
+    return status_word(device).data_ptr()
+
+
 def _refuse_double_backward() -> None:
     if torch.is_grad_enabled():
         raise RuntimeError("the log probabilities' backward is not differentiable itself")
@@ -102,7 +111,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     dev = logits.device
     ids = _token_ids(tokens, math.prod(shape[:-1]), dev)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
-    out = TokenLogProbs(*host.token_logprobs(logits, ids, ign, top_k, status_word(dev).data_ptr()))
+    out = TokenLogProbs(*host.token_logprobs(logits, ids, ign, top_k, _status_ptr(dev)))
     if CHECK_BOUNDS:
         check_status(dev)
     return out
@@ -111,7 +120,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
 def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0) -> torch.Tensor:
     """(4, N) statistics of one weight shard: a reference logit, sum 2^d, sum d 2^d (d = (s - reference) log2 e) and the
     token's logit (0 where the shard does not hold it)."""
-    return host.tied_forward(h, w, tokens, vocab_offset, _NO_IGNORE, False, status_word(h.device).data_ptr())
+    return host.tied_forward(h, w, tokens, vocab_offset, _NO_IGNORE, False, _status_ptr(h.device))
 
 
 def combine_logprob_stats(stats: torch.Tensor, tokens: torch.Tensor, vocab_size: int, ignore_index: int):
@@ -130,7 +139,7 @@ def shard_logprob_backward(g_lp, g_ent, h, w, tokens, lse, ent, *, vocab_offset=
     """Fills ``grad_hidden`` (this shard's partial) and fills or adds to ``grad_weights``, those that are given."""
     host.tied_backward(g_lp, g_ent, h, w, tokens, lse, ent, vocab_offset, w.shape[0] if vocab_size is None else vocab_size,
                        ignore_index, grad_hidden, grad_weights, accumulate, SLAB_BYTES,
-                       status_word(h.device).data_ptr())
+                       _status_ptr(h.device))
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -154,7 +163,7 @@ def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_siz
         poll_status(dev)
     world = vocab_parallel.world_size(group)
     if world == 1 and vocab_offset == 0 and w.shape[0] == vocab_size:
-        out = host.tied_forward(h, w, tokens, 0, ignore_index, True, status_word(dev).data_ptr())
+        out = host.tied_forward(h, w, tokens, 0, ignore_index, True, _status_ptr(dev))
     else:
         part = shard_logprob_stats(h, w, tokens, vocab_offset)
         if world > 1:

@@ -32,6 +32,11 @@ def test_adamw_lists_and_state():
     adamw_step_many([torch.zeros(3)], [None], [torch.zeros(3)], [torch.zeros(3)], step=1)
     with pytest.raises(ValueError, match="state_bits"):
         AdamW([torch.zeros(3)], state_bits=16)
+    for size in (3, 16):  # a step of its own, and one of the list
+        opt = AdamW([torch.zeros(size)])
+        opt.params[0].grad = torch.zeros(size)
+        with pytest.raises(ValueError, match="CUDA"):
+            opt.step()
     opt = AdamW([torch.zeros(300)], state_bits=8)
     assert isinstance(opt.m[0], QuantizedMoment) and opt.m[0].scales.numel() == 3
     with pytest.raises(ValueError, match="float32"):

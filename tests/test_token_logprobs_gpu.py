@@ -27,12 +27,14 @@ def half_step(dtype):
 def exact_rows(x, tokens):
     """(logp, entropy, p, logq, d) in 64 bits; a row of -inf only: -inf, 0, 0, -inf, 0.
 
-    log p is (x - m) - ln sum exp(x - m): next to an m of -3.4e38 even 64 bits lose the logarithm."""
+    log p is (x - m) - ln sum exp(x - m): next to an m of -3.4e38 even 64 bits lose the logarithm. A row with +inf
+    or NaN has NaN everywhere."""
     x = x.double()
     m = x.amax(1, keepdim=True)
     d = x - torch.where(torch.isneginf(m), torch.zeros_like(m), m)
     total = d.exp().sum(1, keepdim=True)
     logq = torch.where(total > 0, d - total.log(), torch.full_like(d, -torch.inf))
+    logq = torch.where((torch.isnan(x) | torch.isposinf(x)).any(1, keepdim=True), torch.full_like(d, torch.nan), logq)
     p = logq.exp()
     h = -(p * torch.where(p > 0, logq, torch.zeros_like(logq))).sum(1)
     return logq.gather(1, tokens.clamp(min=0).unsqueeze(1)).squeeze(1), h, p, logq, torch.where(p > 0, d, torch.zeros_like(d))
@@ -63,27 +65,32 @@ def check_rows(r, x, tokens, ignored=None):
     lp, h, p, logq, d = exact_rows(x, tokens)
     t_ls, t_h = row_bounds(p, d, h)
     used = tokens != IGN
+    spoilt = used & torch.isnan(p).any(1)
+    assert torch.isnan(r.logprobs[spoilt]).all() and torch.isnan(r.entropy[spoilt]).all()
+    every, used = used, used & ~spoilt
     assert torch.isneginf(r.logprobs[used]).equal(torch.isneginf(lp[used]))
     fin = used & torch.isfinite(lp)
     # x - m and the result are rounded: 2^-24 of each, |x - m| <= |logp| + ln s.
     tol = t_ls + 2.0**-24 * (2 * lp.abs() + h + (p * d.abs()).sum(1))
     assert ((r.logprobs.double() - lp).abs() <= tol)[fin].all()
     assert ((r.entropy.double() - h).abs() <= t_h)[used].all()
-    assert (r.logprobs[~used] == 0).all() and (r.entropy[~used] == 0).all()
+    assert (r.logprobs[~every] == 0).all() and (r.entropy[~every] == 0).all()
     if r.top_ids is not None:
         k = r.top_ids.shape[1]
         ids = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :k]
-        assert r.top_ids[used].equal(ids[used])
+        assert r.top_ids[used].equal(ids[used])  # (+inf is the best)
+        assert r.top_ids[spoilt].equal(ids[spoilt]) or torch.isnan(x).any()
         want = logq.gather(1, ids)
         off = (r.top_logprobs.double() - want).abs()
         same = torch.isneginf(want) & torch.isneginf(r.top_logprobs)
         tol = t_ls.unsqueeze(1) + 2.0**-24 * (2 * want.abs() + (h + (p * d.abs()).sum(1)).unsqueeze(1))
         assert (same | (off <= tol))[used].all()
-        assert (r.top_ids[~used] == -1).all() and torch.isneginf(r.top_logprobs[~used]).all()
+        assert (r.top_ids[~every] == -1).all() and torch.isneginf(r.top_logprobs[~every]).all()
 
 
 def check_grad(got, x, tokens, a, b):
-    """Rounded once, from a p off by the sum's error, 2^-22 and 4 u (|x - m| + ln s) relative."""
+    """Rounded once, from a p off by the sum's error, 2^-22 and 4 u (|x - m| + ln s) relative; one below 2^-126 is
+    zero (ex2 without subnormal results), off by at most that."""
     _, h, p, logq, d = exact_rows(x, tokens)
     zero = torch.zeros_like(p)
     lq = torch.where(p > 0, logq, zero)
@@ -95,10 +102,11 @@ def check_grad(got, x, tokens, a, b):
     h = h.unsqueeze(1)
     e_lp = t_ls + 2.0**-22 * (d.abs() + lq.abs())  # of log p
     coef = a.abs() + b.abs() * (h + lq.abs())
-    slack = p * (coef * (e_lp + 2.0**-21) + b.abs() * (t_h + e_lp))
+    slack = p * (coef * (e_lp + 2.0**-21) + b.abs() * (t_h + e_lp)) + torch.where(p > 0, 2.0**-126 * coef, zero)
     fin = torch.finfo(got.dtype)
     tol = half_step(got.dtype) * want.abs() + (1 + 2.0**-7) * slack + 2.0**-23 * a.abs() * onehot
-    assert ((got.double() - want).abs() <= tol * (1 + 2.0**-7) + fin.smallest_normal * fin.eps).all()
+    fine = ((got.double() - want).abs() <= tol * (1 + 2.0**-7) + fin.smallest_normal * fin.eps) | torch.isnan(want)
+    assert fine.all()
     assert (got[dead.squeeze(1)] == 0).all()
 
 
@@ -186,6 +194,15 @@ def test_masks_ties_and_orders(dtype, rows, v):
     lowest[0] = low
     kinds["lowest"] = lowest
     kinds["constant"] = torch.zeros_like(x)
+    # Far apart from each other: one weight is 1, or some equal ones share it.
+    huge = x * (1e4 if dtype == torch.float16 else 1e33)
+    huge[0, 3:9] = huge[0].max()
+    huge[1] = -huge[1].abs()
+    kinds["huge"] = huge
+    # A common offset, below, above and around where references stop being products with log2 e.
+    for name, off in (("offset", 3e4 if dtype == torch.float16 else 3e6), ("below", -3e4 if dtype == torch.float16 else -2e7),
+                      ("around", 2.0**15 if dtype == torch.float16 else 2.0**20)):
+        kinds[name] = (x.double() * 6 + off).to(dtype)
     ties = (x * 1.0).round()
     ties[:, 5] = -0.0
     kinds["ties"] = ties
@@ -236,6 +253,21 @@ def test_nan_inf_ignored_and_bad_tokens(rows):
     # No rows at all.
     r = token_logprobs(x[:0], tokens[:0], top_k=3)
     assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
+
+
+def test_one_row_without_a_batch():
+    from nimbleml_b200.losses import token_logprobs
+
+    x, _, _ = make_logits(1, 500, torch.float16, 3)
+    r = token_logprobs(x[0], torch.tensor(7), top_k=4)
+    q = token_logprobs(x, torch.tensor([7]).cuda(), top_k=4)
+    assert r.logprobs.shape == () and r.top_ids.shape == (4,)
+    assert r.logprobs == q.logprobs[0] and r.top_ids.equal(q.top_ids[0])
+    y = x[0].detach().requires_grad_()
+    (g,) = torch.autograd.grad(token_logprobs(y, 7).logprobs, y, create_graph=False)
+    assert g.shape == (500,)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(token_logprobs(y, 7).logprobs, y, create_graph=True)
 
 
 def test_gradient_against_differences():
