@@ -780,7 +780,8 @@ logprobs_grad_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   const int chunk = blockIdx.x % chunks;
   const int64_t tok = tokens[row];
   const float m = row_max[row];
-  const bool live = tok != ignore_index && tok >= 0 && tok < V && m != -INFINITY;
+  // A row of -inf only has no gradient; one of -inf and NaN keeps its NaN.
+  const bool live = tok != ignore_index && tok >= 0 && tok < V && !(m == -INFINITY && logsum[row] == 0.0f);
   const float a = live && g_logp ? g_logp[row] : 0.0f;
   const float b = live && g_ent ? g_ent[row] : 0.0f;
   const float ls2 = logsum[row] * kLog2e;

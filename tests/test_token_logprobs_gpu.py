@@ -255,6 +255,21 @@ def test_nan_inf_ignored_and_bad_tokens(rows):
     assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_row_with_a_nan(dtype):
+    """A NaN among classes that are all ruled out reaches the results and the gradient; a row of -inf only has none."""
+    from nimbleml_b200.losses import token_logprobs
+
+    x = torch.full((3, 700), -torch.inf, dtype=dtype, device="cuda")
+    x[1, 333] = torch.nan
+    x[2, 5] = 1.0
+    tokens = torch.tensor([4, 7, 5], device="cuda")
+    r = token_logprobs(x.requires_grad_(True), tokens)
+    assert torch.isneginf(r.logprobs[0]) and torch.isnan(r.logprobs[1]) and torch.isnan(r.entropy[1])
+    (g,) = torch.autograd.grad((r.logprobs + r.entropy).sum(), x)
+    assert (g[0] == 0).all() and torch.isnan(g[1]).all() and (g[2] == 0).all()
+
+
 def test_one_row_without_a_batch():
     from nimbleml_b200.losses import token_logprobs
 
