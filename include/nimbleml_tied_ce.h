@@ -383,7 +383,7 @@ NIMBLE_API int nimble_tied_logprobs_combine(const float* shard_stats, int n_shar
 
 /* Bytes of workspace nimble_tied_logprobs_backward needs; slab_bytes as in
  * nimble_tied_ce_backward_workspace_size, except that gradient tiles of at most
- * 32 MiB in all are one slab. */
+ * 256 MiB in all are one slab. */
 NIMBLE_API int nimble_tied_logprobs_backward_workspace_size(int64_t n_tokens, int64_t d_model, int64_t v_local,
                                                             int dtype, size_t slab_bytes, size_t* bytes);
 

@@ -17,7 +17,9 @@
 // new weight uses the moments before they are rounded.
 //
 // The step reads and writes each weight, moment and copy once and is bound by
-// HBM.
+// HBM: 353 M weights with fp16 gradients and copies take 1466 us with fp32 moments
+// (6.75 TB/s) and 1115 us with 8-bit ones (5.2 TB/s: 78 registers a thread leave a third
+// of the warps, and DRAM is busy 62% of the time); the values of a moment 264 us.
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 

@@ -114,11 +114,15 @@ __device__ __forceinline__ float2 group_sum(float2 v, float2* red, int group) {
 }
 
 // ------------------------------------------------------------------- forward
-// A group of kW warps has two rows, up to 32 elements of each a thread, which stay
-// in registers in their own type: rows of up to 1024 need one warp and no barrier.
-// Two rows share the loads of gamma and beta: one row a group was bound by the
-// L1 cache (fp32 parameters are twice the row's bytes; 115 us for 32768 x 4096
-// bf16 against 0.54 GB).
+// A group of kW warps has two rows, 8 kV = 16 elements of each a thread (8 for rows of
+// up to 256), which stay in registers in their own type; rows of up to 512 need one
+// warp and no barrier. Two rows share the loads of gamma and beta: with one row a
+// group the L1 cache was the limit (fp32 parameters are twice the row's bytes).
+// 32768 x 4096 bf16: 101 us, 5.33 TB/s read and written; one row a group 115. With 32
+// elements a thread instead of 16 fewer loads are in flight, with 8 there is more
+// summing than work: 32768 x 4096 123 and 162 us, 8192 x 1024 14.6 and 11.2 for 10.0,
+// 16384 x 2048 37 and 35 for 29.5. Rows held in shared memory by asynchronous copies,
+// as in the backward, took 113 us, streaming loads that skip L1 124.
 __host__ __device__ constexpr int fwd_warps(int kW) { return kW > 8 ? kW : 8; }
 template <typename T, typename P, int kW, int kV, bool kVec>
 __global__ void __launch_bounds__(32 * fwd_warps(kW), kW == 16 ? 2 : 4)
@@ -198,10 +202,15 @@ layernorm_fwd_kernel(const T* __restrict__ x, int64_t ldx, const P* __restrict__
 }
 
 // ------------------------------------------------------------------ backward
-// One block of 16 warps an SM in groups of kW; a group walks its rows, 8 kV
-// elements of a row a thread. With kVec a thread fetches its own part of the next
-// rows into a ring in shared memory with asynchronous copies: nobody else reads
-// it, so the ring needs no barrier, and the rows in flight hold no registers.
+// One block of 16 warps an SM in groups of kW; a group walks its rows, 8 kV elements
+// of a row a thread. A group keeps the columns' sums of g xh and g in registers and
+// writes grad_x, one row at a time; at the end the block's groups add up in order:
+// partial is [blocks][2][d]. With kVec a thread fetches its own part of the next rows
+// into a ring in shared memory with asynchronous copies: nobody else reads it, so the
+// ring needs no barrier, and the rows in flight hold no registers.
+// 32768 x 4096 bf16: 135 us, 5.97 TB/s; before: loads into registers, none ahead, 238;
+// 8 elements a thread and single arithmetic 176 (34 instructions an element, most of
+// them for the row sums); mean and rstd loaded when they are needed 164.
 constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 int group_warps(int64_t d) { return d <= 512 ? 1 : d <= 1024 ? 2 : d <= 2048 ? 4 : d <= 4096 ? 8 : 16; }
@@ -235,13 +244,6 @@ struct Ring {
   }
   static constexpr size_t bytes(int slots) { return size_t(16) * kPieces * kPer * slots * kThreads; }
 };
-
-// A group keeps the columns' sums of g xh and g in registers and writes grad_x, one
-// row at a time. (Loads into registers, one row ahead of nothing, ran 32768 x 4096
-// bf16 in 238 us; 8 elements a thread and single arithmetic in 176 us, 34
-// instructions an element, most of them for the row sums; the next row's mean and
-// rstd loaded when they are needed, 164 us.) At the end the block's groups add up in
-// order: partial is [blocks][2][d].
 
 // Rows in the ring: 128 KB of 16-bit rows, 192 KB of fp32 ones.
 template <typename T, int kV>

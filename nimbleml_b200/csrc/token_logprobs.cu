@@ -329,6 +329,9 @@ __device__ int topk_prune(TopKShared& sh, int n, int k) {
 // ------------------------------------------------------------------- forward
 // A cluster of `parts` blocks per row, each block on one contiguous part of
 // the columns; its first block merges the parts over distributed shared memory.
+// 4096 x 128256 bf16: 149 us without alternatives (7.0 TB/s, some of the rows still in
+// L2), 183 with 5; 2048 x 32000 fp16 28 to 31 us (4.3 TB/s; the exponentials alone, 16 a
+// clock and SM, are 15). Fetching the next vectors ahead in registers gained nothing.
 template <typename T, bool kTopK>
 __global__ void __launch_bounds__(kRowThreads, kTopK ? 5 : 6)
 logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restrict__ tokens, int64_t V,
@@ -767,7 +770,7 @@ logprobs_short_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __rest
 // ------------------------------------------------------------------ backward
 // grad = a [j = t] - p (a + b H + b log p), rows with an ignored or
 // out-of-range token zero. A block handles kGradVecs vectors a thread of one
-// row.
+// row: 2048 x 32000 fp16 41 us, 6.4 TB/s read and written.
 constexpr int kGradVecs = 4;
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)

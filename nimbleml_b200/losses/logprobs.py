@@ -12,7 +12,7 @@ terms of every token instead:
   states and the tied matrix. As in ``CrossEntropyLoss.forward_tied`` the logits
   are not kept: the forward keeps the lse and the entropy of each token, the
   backward recomputes the logits slab by slab (a slab holds at most half of them,
-  or all where they take 32 MiB or less).
+  or all where they take 256 MiB or less).
 
 Both are differentiable in the log probabilities and in the entropies:
 d/dx_j (a logp_t + b H) = a [j = t] - p_j (a + b (H + log p_j)).
