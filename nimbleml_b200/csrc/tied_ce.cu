@@ -832,14 +832,20 @@ const int g_wide = [] {
   return m == 1 ? 15 : m;
 }();
 constexpr int kSmemBytesWide = kStagesWide * (2 * kABytes + kBBytes) + kStoreBytes + 1024 + 256;
-// The log probabilities' products take 128 x 256 tiles, whose epilogues overlap the
-// next tile's multiplications, up to this contraction length: a wide tile's
-// multiplications are too short there to hide its epilogue's share. Forward /
-// recompute / dE in us, wide against 128 x 256: 2048 x 768 x 50257 142 / 171 / 156
-// against 115 / 135 / 142, 4096 x 1024 x 32000 214 / 243 / 215 against 183 / 211 / 237
-// (dE contracts over 4096 tokens), 4096 x 2048 x 32000 383 / 410 / 431 against 379 /
-// 421 / 430. At most 128 rows fill half a wide tile and take the small ones too.
+// The log probabilities' products take tiles whose epilogues overlap the next tile's
+// multiplications, up to this contraction length: a wide tile's multiplications are
+// too short there to hide its epilogue's share. Forward / recompute / dE in us, wide
+// against 128 x 256: 2048 x 768 x 50257 142 / 171 / 156 against 115 / 135 / 142, 4096 x
+// 1024 x 32000 214 / 243 / 215 against 183 / 211 / 237 (dE contracts over 4096 tokens),
+// 4096 x 2048 x 32000 383 / 410 / 431 against 379 / 421 / 430. At most 128 rows fill
+// half a wide tile and take the small ones too.
 constexpr int64_t kShortK = 2048;
+// Of these short ones CTA pairs take the recompute from 512 tokens and dE from 1024 on
+// (2048 x 768 x 50257: 134 -> 124 us and 133 -> 115). With fewer a pair has too little
+// to do between two tiles: the backward of 320 x 768 x 50257 takes 131 us, 140 with the
+// recompute in pairs, 139 with dE; that of 1024 tokens 233, 231 and 228. The forward
+// gains nothing (119 against 120).
+constexpr int64_t kPairTokensGrad = 512, kPairTokensDe = 1024;
 template <int EPI, bool kAMN>
 constexpr int gemm_kind_bit() {
   return (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) ? 1 : (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) ? 2 : kAMN ? 4 : 8;
@@ -912,7 +918,10 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
   } else {
     mc = ma;  // unused by the other epilogues
   }
-  const bool pairs = (g_cta_pairs & gemm_kind_bit<EPI, kAMN>()) != 0;
+  const bool lp_short = ep.log_probs && K <= kShortK;
+  const bool lp_pairs = lp_short && (EPI == EPI_LP_GRAD ? M >= kPairTokensGrad
+                                                        : EPI == EPI_STORE && kAMN && K >= kPairTokensDe);
+  const bool pairs = (g_cta_pairs & gemm_kind_bit<EPI, kAMN>()) != 0 || lp_pairs;
   if (int rc = make_operand_map(&mb, B, dtype, kBMN, K, N, ldb, pairs ? kBN / 2 : kBN)) return rc;
   const int group_m = g_group_m;
   if (pairs) {
@@ -936,7 +945,7 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
     cfg.numAttrs = 1;
     NIMBLE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, mc, static_cast<int>(M), static_cast<int>(N),
                                        static_cast<int>(K), group_m, ep));
-  } else if ((g_wide & gemm_kind_bit<EPI, kAMN>()) && !(ep.log_probs && (M <= kBM || K <= kShortK))) {
+  } else if ((g_wide & gemm_kind_bit<EPI, kAMN>()) && !lp_short && !(ep.log_probs && M <= kBM)) {
     auto kern = tc_gemm_tn_kernel<T, EPI, kAMN, kBMN, 1, true>;
     NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesWide));
     const int64_t tiles = ((M + 2 * kBM - 1) / (2 * kBM)) * ((N + kBN - 1) / kBN);
@@ -974,7 +983,8 @@ int gemm_dispatch(int dtype, const void* A, int64_t lda, const void* B, int64_t 
 }
 
 // grad_hidden's product G[M x K] . E[K x N] with the contraction cut into ep.k_splits
-// runs (16-bit operands, 256 x 256 tiles), fp32 partial results.
+// runs (16-bit operands, 256 x 256 tiles of CTA pairs), fp32 partial results. Single CTAs
+// with wide tiles took 5 to 15 us longer for 64 to 2048 tokens.
 template <typename T>
 int launch_split(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, int dtype,
                  const EpiParams& ep, cudaStream_t stream) {
@@ -982,23 +992,48 @@ int launch_split(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t
   if (int rc = device_info(&di)) return rc;
   CUtensorMap ma, mb;
   if (int rc = make_operand_map(&ma, A, dtype, false, K, M, lda, kBM)) return rc;
-  if (int rc = make_operand_map(&mb, B, dtype, true, K, N, ldb, kBN)) return rc;
-  auto kern = tc_gemm_tn_kernel<T, EPI_STORE, false, true, 1, true, true>;
-  NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesWide));
+  if (int rc = make_operand_map(&mb, B, dtype, true, K, N, ldb, kBN / 2)) return rc;
+  auto kern = tc_gemm_tn_kernel<T, EPI_STORE, false, true, 2, false, true>;
+  NIMBLE_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytesPair));
   const int64_t units = ((M + 2 * kBM - 1) / (2 * kBM)) * ((N + kBN - 1) / kBN) * ep.k_splits;
   if (units > INT32_MAX) return fail(NIMBLE_ERR_INVALID_ARG, "too many tiles");
-  kern<<<static_cast<int>(std::min<int64_t>(units, di.sms)), kThreads, kSmemBytesWide, stream>>>(
-      ma, mb, ma, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), g_group_m, ep);
-  NIMBLE_CUDA_TRY(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::min<int64_t>(units, di.sms / 2)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytesPair;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  NIMBLE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ma, mb, ma, static_cast<int>(M), static_cast<int>(N),
+                                     static_cast<int>(K), g_group_m, ep));
   return NIMBLE_OK;
 }
-// Runs for the grad_hidden product of n_tokens x d_model over `cols` columns: one
-// where its 256 x 256 tiles fill the 148 SMs, else as many as do, each of 8 K
-// blocks (512 columns) or more. The whole backward of 64 / 512 / 2048 tokens (d 768, 1024,
-// 768; V 50257, 32000, 50257): 543 / 399 / 795 us with one run, 116 / 138 / 428 with these.
+// Runs for the grad_hidden product of n_tokens x d_model over `cols` columns. In units of
+// the time that a pair of SMs takes for a tile's whole contraction, r runs take
+// ceil(tiles r / 74) / r, and their partial results, written and read once in fp32, r
+// 1000 / cols of the product's own tiles / 74 (bytes at 6.5 TB/s against operations at
+// 1.6 PFLOP/s); without a split a tile stays with one SM, at half the pair's speed. A run
+// has 512 columns or more. The whole backward of 64 / 512 / 2048 tokens (d 768, 1024, 768;
+// V 50257, 32000, 50257): 543 / 399 / 795 us with one run, 104 / 128 / 395 with these.
 int dh_splits(int64_t n_tokens, int64_t d_model, int64_t cols) {
+  constexpr int kPairs = 74, kMaxRuns = 32;
   const int64_t tiles = std::max<int64_t>(1, (n_tokens + 255) / 256 * ((d_model + 255) / 256));
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({148 / tiles, 16, cols / 512})));
+  const double per_run = 1000.0 / static_cast<double>(std::max<int64_t>(1, cols)) * static_cast<double>(tiles) / kPairs;
+  int best = 1;
+  double cost = 2.0 * static_cast<double>((tiles + 2 * kPairs - 1) / (2 * kPairs));
+  for (int r = 2; r <= std::min<int64_t>(kMaxRuns, cols / 512); ++r) {
+    const double c = static_cast<double>((tiles * r + kPairs - 1) / kPairs) / r + per_run * r;
+    if (c < cost) {
+      cost = c;
+      best = r;
+    }
+  }
+  return best;
 }
 
 int launch_round(const float* src, float* dst, int64_t n, cudaStream_t s) {
@@ -1889,9 +1924,10 @@ LpFwdLayout lp_fwd_layout(int64_t N, int64_t V) {
   return L;
 }
 
-// G of at most this is one slab: three launches fewer and longer products, 116 us
-// against 145 (64 x 768 x 50257 fp16), 148 / 206 (320 tokens), 243 / 290 (1024), 428 /
-// 480 (2048); from d = 2048 on both took the same. Larger G is held by halves and less.
+// G of at most this is one slab: three launches fewer and longer products. The backward
+// (before the pairs above) took 116 us against 145 (64 x 768 x 50257 fp16), 148 / 206 (320
+// tokens), 243 / 290 (1024), 428 / 480 (2048); from d = 2048 on both took the same. Larger
+// G is held by halves and less.
 constexpr int64_t kOneSlabBytes = 256 << 20;
 // The slab backward's workspace, then the row coefficients and the scale.
 struct LpBwdLayout {

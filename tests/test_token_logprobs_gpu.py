@@ -422,6 +422,29 @@ def test_tied(dtype, shape):
     check_tied_grads(None, gw4, h.detach(), w.detach(), tokens, a, torch.zeros_like(b))
 
 
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape", [(1024, 72, 700), (1153, 264, 2100), (2049, 64, 1300), (600, 2056, 900)])
+@pytest.mark.parametrize("buffer", [False, True])
+def test_tied_many_tokens(dtype, shape, buffer, monkeypatch):
+    """Enough tokens for every kind of tile; grad_hidden in several runs, over one slab and over several."""
+    import nimbleml_b200.losses.logprobs as mod
+
+    n, d, v = shape
+    h, w, tokens, g = make_tied(n, d, v, dtype, n + v)
+    tokens[::7] = IGN
+    a, b = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    base = torch.randn(v, d, generator=g).cuda() if buffer else None
+    for slab in (0, 512 * n * 2):  # at most 512 columns
+        monkeypatch.setattr(mod, "SLAB_BYTES", slab)
+        buf = base.clone() if buffer else None
+        hl, wl = h.detach().requires_grad_(), w.detach().requires_grad_(not buffer)
+        r = mod.tied_token_logprobs(hl, wl, tokens, IGN, grad_weights_buffer=buf)
+        check_tied(r, h, w, tokens)
+        grads = torch.autograd.grad((r.logprobs, r.entropy), (hl,) if buffer else (hl, wl), (a, b))
+        check_tied_grads(grads[0], buf if buffer else grads[1], h, w, tokens, a, b, base)
+        assert (grads[0][tokens == IGN] == 0).all()
+
+
 @pytest.mark.parametrize("size", [1e-12, 1e-6, 1.0, 1e6])
 def test_tied_fp16_upstream_sizes(size):
     """Upstream gradients of any size keep the 16-bit G in range; the fp32 weight grad shows it."""
