@@ -1,11 +1,13 @@
 // torch_host.cpp — the host side of the operators whose calls are short against
-// Python's: layer norm and token log probabilities as autograd nodes, and the
+// Python's: layer norm and token log probabilities (over logits, and from the tied
+// matrix on one rank) as autograd nodes, and the
 // many-tensor AdamW step with its checks. Everything on the GPU goes through the
 // C ABI (include/nimbleml_tied_ce.h); this file only checks arguments, allocates
 // outputs and workspaces on torch's current stream, and keeps what the backward
 // needs. Errors are Python's: ValueError for arguments, RuntimeError with the
 // library's message for a failing call.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -247,23 +249,54 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t ign
   return py::make_tuple(out[0], out[1], py::none(), py::none());
 }
 
-// ------------------------------------------------ tied log probabilities (one shard)
-// Results of a shard that is the whole vocabulary (3, N), or its statistics (4, N).
-Tensor tied_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_t v_offset, int64_t ignore_index,
-                    bool whole, int64_t status) {
-  const c10::cuda::CUDAGuard guard(h.device());
+// ------------------------------------------------------- tied log probabilities
+// The package's hooks around a tied call: `poll` raises what an earlier call's status
+// copy shows, `snapshot` queues the copy that the next one reads. A captured launch must
+// not be joined by either.
+py::object* status_hooks[2] = {nullptr, nullptr};
+enum Hook { kPoll = 0, kSnapshot = 1 };
+void set_status_hooks(py::object poll, py::object snapshot) {
+  for (py::object*& h : status_hooks) delete h;
+  status_hooks[kPoll] = new py::object(std::move(poll));
+  status_hooks[kSnapshot] = new py::object(std::move(snapshot));
+}
+void status_hook(Hook which, const Tensor& t) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return;
+  py::gil_scoped_acquire gil;
+  try {
+    (*status_hooks[which])(static_cast<int>(t.get_device()));
+  } catch (py::error_already_set& e) {
+    // As torch's own errors, which cross the autograd engine's threads.
+    const std::string what = py::str(e.value());
+    if (e.matches(PyExc_ValueError)) TORCH_CHECK_VALUE(false, what);
+    TORCH_CHECK(false, what);
+  }
+}
+
+// Where a forward on one shard writes: its statistics (4, N), or the results of a shard
+// that is the whole vocabulary.
+struct TiedOut {
+  float *stats, *logprob, *entropy, *lse;
+};
+void tied_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_t v_offset, int64_t ignore_index,
+                  const TiedOut& o, int64_t status) {
   const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
-  Tensor out = empty({whole ? 3 : 4, n}, h, at::kFloat);
   size_t bytes = 0;
   check_rc(nimble_tied_logprobs_forward_workspace_size(n, d, v, dtype_of(h), &bytes),
            "nimble_tied_logprobs_forward_workspace_size");
   const Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, h, at::kByte);
-  float* o = out.mutable_data_ptr<float>();
   check_rc(nimble_tied_logprobs_forward(h.const_data_ptr(), w.const_data_ptr(), tokens.const_data_ptr<int64_t>(), n, d,
-                                        v, v_offset, dtype_of(h), ignore_index, whole ? nullptr : o,
-                                        whole ? o : nullptr, whole ? o + n : nullptr, whole ? o + 2 * n : nullptr,
+                                        v, v_offset, dtype_of(h), ignore_index, o.stats, o.logprob, o.entropy, o.lse,
                                         ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status), stream_of(h)),
            "nimble_tied_logprobs_forward");
+}
+
+Tensor tied_shard_stats(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_t v_offset, int64_t ignore_index,
+                        int64_t status) {
+  const c10::cuda::CUDAGuard guard(h.device());
+  Tensor out = empty({4, h.size(0)}, h, at::kFloat);
+  tied_forward(h, w, tokens, v_offset, ignore_index, {out.mutable_data_ptr<float>(), nullptr, nullptr, nullptr},
+               status);
   return out;
 }
 
@@ -288,6 +321,87 @@ void tied_backward(const std::optional<Tensor>& g_logprob, const std::optional<T
                grad_weights ? dtype_of(*grad_weights) : dt, accumulate ? 1 : 0, static_cast<size_t>(slab_bytes),
                ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status), stream_of(h)),
            "nimble_tied_logprobs_backward");
+}
+
+// Contiguous and on a 16-byte boundary, as the TMA loads need it.
+Tensor for_tma(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+struct TiedRows {
+  Tensor h, w, logprob, entropy, lse;  // h, w: 16-bit, as the kernels read them
+};
+TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& tokens, int64_t ignore_index,
+                   int64_t status) {
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  TiedRows r;
+  r.w = for_tma(weights.to(hidden.scalar_type()));
+  r.h = for_tma(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)}));
+  status_hook(kPoll, r.h);
+  const auto shape = hidden.sizes().slice(0, hidden.dim() - 1);
+  r.logprob = empty(shape, hidden, at::kFloat);
+  r.entropy = empty(shape, hidden, at::kFloat);
+  r.lse = empty({r.h.size(0)}, hidden, at::kFloat);
+  tied_forward(r.h, r.w, tokens, 0, ignore_index,
+               {nullptr, r.logprob.mutable_data_ptr<float>(), r.entropy.mutable_data_ptr<float>(),
+                r.lse.mutable_data_ptr<float>()},
+               status);
+  status_hook(kSnapshot, r.h);
+  return r;
+}
+
+// On one rank with the whole vocabulary (the sharded form is the package's).
+struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weights, const Tensor& tokens,
+                               int64_t ignore_index, const std::optional<Tensor>& buffer, int64_t slab_bytes,
+                               int64_t status) {
+    TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r.h, r.w, tokens, r.lse, r.entropy});
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["slab_bytes"] = slab_bytes;
+    ctx->saved_data["status"] = status;
+    ctx->saved_data["weights"] = static_cast<int64_t>(weights.scalar_type());
+    ctx->saved_data["shape"] = hidden.sizes().vec();
+    if (buffer) ctx->saved_data["buffer"] = *buffer;
+    return {r.logprob, r.entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "the log probabilities' backward is not differentiable itself");
+    variable_list out(7);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1];
+    const c10::cuda::CUDAGuard guard(h.device());
+    std::optional<Tensor> gh, gw;
+    const auto buffer = ctx->saved_data.find("buffer");
+    const bool accumulate = buffer != ctx->saved_data.end();
+    if (ctx->needs_input_grad(0)) gh = empty(ctx->saved_data["shape"].toIntVector(), h, h.scalar_type());
+    if (accumulate) gw = buffer->second.toTensor();
+    else if (ctx->needs_input_grad(1))
+      gw = empty(w.sizes(), w, static_cast<at::ScalarType>(ctx->saved_data["weights"].toInt()));
+    status_hook(kPoll, h);
+    tied_backward(grads[0].defined() ? std::optional<Tensor>(grads[0]) : std::nullopt,
+                  grads[1].defined() ? std::optional<Tensor>(grads[1]) : std::nullopt, h, w, saved[2], saved[3],
+                  saved[4], 0, w.size(0), ctx->saved_data["ignore_index"].toInt(), gh, gw, accumulate,
+                  ctx->saved_data["slab_bytes"].toInt(), ctx->saved_data["status"].toInt());
+    status_hook(kSnapshot, h);
+    if (gh) out[0] = *gh;
+    if (gw && !accumulate) out[1] = *gw;
+    return out;
+  }
+};
+
+py::tuple tied_token_logprobs(const Tensor& hidden, const Tensor& weights, const Tensor& tokens, int64_t ignore_index,
+                              const std::optional<Tensor>& buffer, int64_t slab_bytes, int64_t status) {
+  if (at::GradMode::is_enabled() && (hidden.requires_grad() || weights.requires_grad())) {
+    const variable_list out =
+        TiedLogProbsNode::apply(hidden, weights, tokens, ignore_index, buffer, slab_bytes, status);
+    return py::make_tuple(out[0], out[1]);
+  }
+  const TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status);
+  return py::make_tuple(r.logprob, r.entropy);
 }
 
 // ------------------------------------------------------------------------- AdamW
@@ -417,7 +531,9 @@ PYBIND11_MODULE(nimbleml_b200_host, m) {
   m.doc() = "Host side of layer_norm, the token log probabilities and adamw_step_many over the C ABI";
   m.def("layer_norm", &layer_norm);
   m.def("token_logprobs", &token_logprobs);
-  m.def("tied_forward", &tied_forward);
+  m.def("set_status_hooks", &set_status_hooks);
+  m.def("tied_token_logprobs", &tied_token_logprobs);
+  m.def("tied_shard_stats", &tied_shard_stats);
   m.def("tied_backward", &tied_backward);
   m.def("adamw_step_many", &adamw_step_many);
 }

@@ -120,7 +120,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
 def shard_logprob_stats(h: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, vocab_offset: int = 0) -> torch.Tensor:
     """(4, N) statistics of one weight shard: a reference logit, sum 2^d, sum d 2^d (d = (s - reference) log2 e) and the
     token's logit (0 where the shard does not hold it)."""
-    return host.tied_forward(h, w, tokens, vocab_offset, _NO_IGNORE, False, _status_ptr(h.device))
+    return host.tied_shard_stats(h, w, tokens, vocab_offset, _NO_IGNORE, _status_ptr(h.device))
 
 
 def combine_logprob_stats(stats: torch.Tensor, tokens: torch.Tensor, vocab_size: int, ignore_index: int):
@@ -148,12 +148,22 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group):
-    """(h, w as the kernels read them, (3, n) log probability, entropy, lse)."""
+def _after_call(device: torch.device) -> None:
+    snapshot_status(device)
+    if CHECK_BOUNDS:
+        check_status(device)
+
+
+host.set_status_hooks(lambda index: poll_status(torch.device("cuda", index)),
+                      lambda index: _after_call(torch.device("cuda", index)))
+
+
+def _shard_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group):
+    """(h, w as the kernels read them, (3, n) log probability, entropy, lse) with the vocabulary in shards."""
     dev = hidden.device
     if dev.index != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
+            return _shard_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
     # 16-bit operands for the tensor cores; fp32 master weights still get an fp32 grad.
     w = _aligned(weights if weights.dtype == hidden.dtype else weights.to(hidden.dtype))
     h = _aligned(hidden if hidden.ndim == 2 else hidden.reshape(-1, hidden.shape[-1]))
@@ -161,27 +171,21 @@ def _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_siz
     watch = not torch.cuda.is_current_stream_capturing()
     if watch:
         poll_status(dev)
-    world = vocab_parallel.world_size(group)
-    if world == 1 and vocab_offset == 0 and w.shape[0] == vocab_size:
-        out = host.tied_forward(h, w, tokens, 0, ignore_index, True, _status_ptr(dev))
+    part = shard_logprob_stats(h, w, tokens, vocab_offset)
+    if vocab_parallel.world_size(group) > 1:
+        part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
     else:
-        part = shard_logprob_stats(h, w, tokens, vocab_offset)
-        if world > 1:
-            part = vocab_parallel.gather_shard_stats(part, group).transpose(0, 1).contiguous()
-        else:
-            part = part.unsqueeze(0)
-        out = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
+        part = part.unsqueeze(0)
+    out = combine_logprob_stats(part, tokens, vocab_size, ignore_index)
     if watch:
-        snapshot_status(dev)
-    if CHECK_BOUNDS:
-        check_status(dev)
+        _after_call(dev)
     return h, w, out
 
 
-class _TiedTokenLogProbs(torch.autograd.Function):
+class _ShardTokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group, grad_buffer):
-        h, w, out = _tied_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
+        h, w, out = _shard_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(h, w, tokens, out)
         ctx.meta = (ignore_index, vocab_offset, vocab_size, group, weights.dtype, hidden.shape)
@@ -215,11 +219,9 @@ class _TiedTokenLogProbs(torch.autograd.Function):
                                    vocab_offset=vocab_offset, vocab_size=vocab_size, ignore_index=ignore_index,
                                    grad_hidden=gh, grad_weights=gw, accumulate=buf is not None)
             if watch:
-                snapshot_status(dev)
+                _after_call(dev)
             if gh is not None and world > 1:
                 gh = vocab_parallel.reduce_grad_hidden(gh, group).to(h.dtype)
-        if CHECK_BOUNDS:
-            check_status(dev)
         if gh is not None and len(shape) != 2:
             gh = gh.view(shape)
         return (gh, None if buf is not None else gw, *none)
@@ -267,11 +269,14 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
     shape = hidden.shape[:-1]
     ids = _token_ids(tokens, math.prod(shape), hidden.device)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
+    if v == vocab_size and vocab_parallel.world_size(group) == 1:
+        return TokenLogProbs(*host.tied_token_logprobs(hidden, weights, ids, ign, grad_weights_buffer, SLAB_BYTES,
+                                                       _status_ptr(hidden.device)))
     args = (hidden, weights, ids, ign, int(vocab_offset), vocab_size, group)
     if (hidden.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
-        lp, ent = _TiedTokenLogProbs.apply(*args, grad_weights_buffer)
+        lp, ent = _ShardTokenLogProbs.apply(*args, grad_weights_buffer)
     else:
-        out = _tied_forward(*args)[2]
+        out = _shard_forward(*args)[2]
         lp, ent = out[0], out[1]
     if len(shape) != 1:
         lp, ent = lp.view(shape), ent.view(shape)
