@@ -366,12 +366,15 @@ NIMBLE_API int nimble_tied_logprobs_forward_workspace_size(int64_t n_tokens, int
  *     (0 where the shard does not hold it), for nimble_tied_logprobs_combine;
  *   out_logprob, out_entropy, out_lse (n_tokens; all three or none): the results,
  *     for a shard that is the whole vocabulary (v_offset 0). Ignored rows and bad
- *     tokens as in nimble_token_logprobs_forward. */
+ *     tokens as in nimble_token_logprobs_forward;
+ *   host_flag: 1 into a word of pinned host memory when the status word has a bit
+ *     at the call's end (else it is left alone), so that a host that looks at it
+ *     needs no copy. It needs status. */
 NIMBLE_API int nimble_tied_logprobs_forward(const void* hidden, const void* weights, const int64_t* tokens,
                                             int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
                                             int dtype, int64_t ignore_index, float* shard_stats, float* out_logprob,
                                             float* out_entropy, float* out_lse, void* workspace,
-                                            size_t workspace_bytes, int* status, void* stream);
+                                            size_t workspace_bytes, int* status, int* host_flag, void* stream);
 
 /* Merges the statistics of n_shards shards ([n_shards][4][n_tokens]) in order
  * into out_logprob, out_entropy and out_lse; ignored rows and bad tokens as in

@@ -106,7 +106,7 @@ SIGNATURES = {
     "nimble_tied_logprobs_forward": (
         _c_int,
         [_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp,
-         _c_size, _c_vp, _c_vp]),
+         _c_size, _c_vp, _c_vp, _c_vp]),
     "nimble_tied_logprobs_combine": (
         _c_int, [_c_vp, _c_int, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
     "nimble_tied_logprobs_backward_workspace_size": (

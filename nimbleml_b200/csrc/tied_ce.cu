@@ -1552,8 +1552,11 @@ struct LpStats {
 __global__ void __launch_bounds__(32 * kReduceGroups)
 lp_row_reduce_kernel(const float2* __restrict__ part, const float* __restrict__ part_u, int n_parts,
                      const float* __restrict__ tgt, const int64_t* __restrict__ tokens, int64_t M, int64_t v_offset,
-                     int64_t v_local, int64_t ignore_index, LpOut out, int* status) {
+                     int64_t v_local, int64_t ignore_index, LpOut out, int* status, int* host_flag) {
   __shared__ float sm[3][kReduceGroups][32];
+  // What the products before this kernel reported; bad tokens below tell the host themselves.
+  if (host_flag && blockIdx.x == 0 && threadIdx.x == 0 && *static_cast<volatile int*>(status))
+    *static_cast<volatile int*>(host_flag) = 1;
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   LpStats a;
@@ -1592,7 +1595,10 @@ lp_row_reduce_kernel(const float2* __restrict__ part, const float* __restrict__ 
       out.logp[row] = out.entropy[row] = out.lse[row] = 0.0f;
       return;
     }
-    if (!mine && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
+    if (!mine && status) {
+      atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
+      if (host_flag) *static_cast<volatile int*>(host_flag) = 1;
+    }
     const float ls = logf(a.s), ln2 = 0.6931471805599453f;
     const float rel = ls - ln2 * fmaf(a.f, kLog2e, -__fmul_rn(a.f, kLog2e));  // lse - f
     out.logp[row] = mine ? (x - a.f) - rel : __int_as_float(0x7fc00000);
@@ -1968,7 +1974,7 @@ extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weig
                                             int64_t n_tokens, int64_t d_model, int64_t v_local, int64_t v_offset,
                                             int dtype, int64_t ignore_index, float* shard_stats, float* out_logprob,
                                             float* out_entropy, float* out_lse, void* workspace,
-                                            size_t workspace_bytes, int* status, void* stream) {
+                                            size_t workspace_bytes, int* status, int* host_flag, void* stream) {
   if (int rc = check_half(dtype)) return rc;
   if (int rc = check_common(hidden, weights, tokens, n_tokens, d_model, v_local, dtype)) return rc;
   if (v_offset < 0) return fail(NIMBLE_ERR_INVALID_ARG, "v_offset must be >= 0");
@@ -1976,6 +1982,7 @@ extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weig
   if (n_tokens == 0) return NIMBLE_OK;
   if (out_logprob ? !out_entropy || !out_lse || v_offset != 0 : !shard_stats)
     return fail(NIMBLE_ERR_INVALID_ARG, "need shard_stats, or the three results of a whole vocabulary");
+  if (host_flag && !status) return fail(NIMBLE_ERR_INVALID_ARG, "host_flag needs a status word");
   const LpFwdLayout L = lp_fwd_layout(n_tokens, v_local);
   if (!workspace || workspace_bytes < L.total)
     return fail(NIMBLE_ERR_WORKSPACE, "log probability forward workspace too small");
@@ -2004,7 +2011,8 @@ extern "C" int nimble_tied_logprobs_forward(const void* hidden, const void* weig
   if (rc) return rc;
   const LpOut out{shard_stats, out_logprob, out_entropy, out_lse};
   lp_row_reduce_kernel<<<static_cast<unsigned>((n_tokens + 31) / 32), 32 * kReduceGroups, 0, s>>>(
-      ep.part, ep.part_u, n_parts, ep.tgt, tokens, n_tokens, v_offset, v_local, ignore_index, out, status);
+      ep.part, ep.part_u, n_parts, ep.tgt, tokens, n_tokens, v_offset, v_local, ignore_index, out, status,
+      host_flag);
   NIMBLE_CUDA_TRY(cudaGetLastError());
   return NIMBLE_OK;
 }

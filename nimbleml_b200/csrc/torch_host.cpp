@@ -250,9 +250,10 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t ign
 }
 
 // ------------------------------------------------------- tied log probabilities
-// The package's hooks around a tied call: `poll` raises what an earlier call's status
-// copy shows, `snapshot` queues the copy that the next one reads. A captured launch must
-// not be joined by either.
+// The package's hooks around a tied call: `poll` raises what an earlier call reported,
+// `snapshot` queues the copy of the status word that the next one reads (a forward needs
+// none: its last kernel raises the host's flag itself, where the copy and its event took
+// 7 of 38 us of a call with few tokens). A captured launch must not be joined by either.
 py::object* status_hooks[2] = {nullptr, nullptr};
 enum Hook { kPoll = 0, kSnapshot = 1 };
 void set_status_hooks(py::object poll, py::object snapshot) {
@@ -262,6 +263,7 @@ void set_status_hooks(py::object poll, py::object snapshot) {
 }
 void status_hook(Hook which, const Tensor& t) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return;
+  TORCH_CHECK(status_hooks[which], "set_status_hooks comes first");
   py::gil_scoped_acquire gil;
   try {
     (*status_hooks[which])(static_cast<int>(t.get_device()));
@@ -279,7 +281,7 @@ struct TiedOut {
   float *stats, *logprob, *entropy, *lse;
 };
 void tied_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_t v_offset, int64_t ignore_index,
-                  const TiedOut& o, int64_t status) {
+                  const TiedOut& o, int64_t status, int64_t host_flag) {
   const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
   size_t bytes = 0;
   check_rc(nimble_tied_logprobs_forward_workspace_size(n, d, v, dtype_of(h), &bytes),
@@ -287,7 +289,8 @@ void tied_forward(const Tensor& h, const Tensor& w, const Tensor& tokens, int64_
   const Tensor ws = empty({static_cast<int64_t>(std::max<size_t>(bytes, 1))}, h, at::kByte);
   check_rc(nimble_tied_logprobs_forward(h.const_data_ptr(), w.const_data_ptr(), tokens.const_data_ptr<int64_t>(), n, d,
                                         v, v_offset, dtype_of(h), ignore_index, o.stats, o.logprob, o.entropy, o.lse,
-                                        ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status), stream_of(h)),
+                                        ws.mutable_data_ptr(), bytes, reinterpret_cast<int*>(status),
+                                        reinterpret_cast<int*>(host_flag), stream_of(h)),
            "nimble_tied_logprobs_forward");
 }
 
@@ -296,7 +299,7 @@ Tensor tied_shard_stats(const Tensor& h, const Tensor& w, const Tensor& tokens, 
   const c10::cuda::CUDAGuard guard(h.device());
   Tensor out = empty({4, h.size(0)}, h, at::kFloat);
   tied_forward(h, w, tokens, v_offset, ignore_index, {out.mutable_data_ptr<float>(), nullptr, nullptr, nullptr},
-               status);
+               status, 0);
   return out;
 }
 
@@ -333,7 +336,7 @@ struct TiedRows {
   Tensor h, w, logprob, entropy, lse;  // h, w: 16-bit, as the kernels read them
 };
 TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& tokens, int64_t ignore_index,
-                   int64_t status) {
+                   int64_t status, int64_t host_flag) {
   const c10::cuda::CUDAGuard guard(hidden.device());
   TiedRows r;
   r.w = for_tma(weights.to(hidden.scalar_type()));
@@ -346,8 +349,7 @@ TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& to
   tied_forward(r.h, r.w, tokens, 0, ignore_index,
                {nullptr, r.logprob.mutable_data_ptr<float>(), r.entropy.mutable_data_ptr<float>(),
                 r.lse.mutable_data_ptr<float>()},
-               status);
-  status_hook(kSnapshot, r.h);
+               status, host_flag);
   return r;
 }
 
@@ -355,8 +357,8 @@ TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& to
 struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weights, const Tensor& tokens,
                                int64_t ignore_index, const std::optional<Tensor>& buffer, int64_t slab_bytes,
-                               int64_t status) {
-    TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status);
+                               int64_t status, int64_t host_flag) {
+    TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status, host_flag);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({r.h, r.w, tokens, r.lse, r.entropy});
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -369,7 +371,7 @@ struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the log probabilities' backward is not differentiable itself");
-    variable_list out(7);
+    variable_list out(8);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &w = saved[1];
@@ -394,13 +396,14 @@ struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
 };
 
 py::tuple tied_token_logprobs(const Tensor& hidden, const Tensor& weights, const Tensor& tokens, int64_t ignore_index,
-                              const std::optional<Tensor>& buffer, int64_t slab_bytes, int64_t status) {
+                              const std::optional<Tensor>& buffer, int64_t slab_bytes, int64_t status,
+                              int64_t host_flag) {
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weights.requires_grad())) {
     const variable_list out =
-        TiedLogProbsNode::apply(hidden, weights, tokens, ignore_index, buffer, slab_bytes, status);
+        TiedLogProbsNode::apply(hidden, weights, tokens, ignore_index, buffer, slab_bytes, status, host_flag);
     return py::make_tuple(out[0], out[1]);
   }
-  const TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status);
+  const TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status, host_flag);
   return py::make_tuple(r.logprob, r.entropy);
 }
 

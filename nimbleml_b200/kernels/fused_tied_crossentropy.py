@@ -101,7 +101,9 @@ def check_status(device: torch.device, *, clear: bool = True) -> int:
     val = int(buf.item())
     if clear and val:
         buf.zero_()
-        _monitor(device).pending = False  # an older asynchronous copy would repeat this value
+        mon = _monitor(device)
+        mon.pending = False  # an older asynchronous copy would repeat this value
+        mon.flag[0] = 0
     _raise_for(val)
     return val
 
@@ -113,6 +115,9 @@ class _StatusMonitor:
     current stream and records an event; ``poll`` looks at the copy only once
     that event has completed (``Event.query`` does not block), and raises
     (clearing the device word) when an error bit is set.
+
+    ``flag`` is a word of pinned host memory that a kernel sets when it finds the
+    status word set: a call that hands it on (``flag_ptr``) needs no copy.
     """
 
     def __init__(self, device: torch.device):
@@ -120,6 +125,9 @@ class _StatusMonitor:
         self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
         self.event = torch.cuda.Event()
         self.pending = False
+        self._flag = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.flag = self._flag.numpy()
+        self.flag_ptr = self._flag.data_ptr()
 
     def snapshot(self) -> None:
         self.host.copy_(status_word(self.device), non_blocking=True)
@@ -127,6 +135,9 @@ class _StatusMonitor:
         self.pending = True
 
     def poll(self) -> None:
+        if self.flag[0]:
+            self.flag[0] = 0
+            check_status(self.device)
         if not self.pending or not self.event.query():
             return
         self.pending = False

@@ -31,6 +31,8 @@ from nimbleml_b200.kernels.fused_tied_crossentropy import (
     _NO_IGNORE,
     CHECK_BOUNDS,
     SLAB_BYTES,
+    _monitor,
+    _monitors,
     _status_words,
     _stream_ptr,
     as_label_indices,
@@ -70,10 +72,12 @@ def _token_ids(tokens, n: int, device: torch.device) -> torch.Tensor:
 
 
 def _status_ptr(device: torch.device) -> int:
-    """Address of the device's status word, which a captured launch must find in place: made by the first
-    call on a device, it would otherwise lie in the graph's own memory."""
-    if device.index not in _status_words and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("call the operator once on this device before capturing it into a CUDA graph")
+    """Address of the device's status word, which a captured launch must find in place, as the monitor's
+    pinned memory: made by the first call on a device, it would otherwise lie in the graph's own memory."""
+    if device.index not in _status_words or device.index not in _monitors:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call the operator once on this device before capturing it into a CUDA graph")
+        _monitor(device)
     return status_word(device).data_ptr()
 
 
@@ -270,8 +274,12 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
     ids = _token_ids(tokens, math.prod(shape), hidden.device)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
     if v == vocab_size and vocab_parallel.world_size(group) == 1:
-        return TokenLogProbs(*host.tied_token_logprobs(hidden, weights, ids, ign, grad_weights_buffer, SLAB_BYTES,
-                                                       _status_ptr(hidden.device)))
+        dev = hidden.device
+        out = TokenLogProbs(*host.tied_token_logprobs(hidden, weights, ids, ign, grad_weights_buffer, SLAB_BYTES,
+                                                      _status_ptr(dev), _monitor(dev).flag_ptr))
+        if CHECK_BOUNDS:
+            check_status(dev)
+        return out
     args = (hidden, weights, ids, ign, int(vocab_offset), vocab_size, group)
     if (hidden.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         lp, ent = _ShardTokenLogProbs.apply(*args, grad_weights_buffer)

@@ -91,8 +91,8 @@ def test_native_tied_logprobs_arguments():
     assert need < 4096 * 128256 * 2 / 16  # no N x V buffer
     assert native.tied_logprobs_backward_workspace_size(4096, 4096, 128256, DTYPE_BF16) < 4096 * 128256 * 2
 
-    def fwd(d=8, dt=DTYPE_F16, ws=1 << 20, off=0, out=p, n=4, res=(None, None, None)):
-        return (p, p, p, n, d, 100, off, dt, -1, out, *res, p, ws, None, None)
+    def fwd(d=8, dt=DTYPE_F16, ws=1 << 20, off=0, out=p, n=4, res=(None, None, None), flag=None):
+        return (p, p, p, n, d, 100, off, dt, -1, out, *res, p, ws, None, flag, None)
 
     _fails(-1, "nimble_tied_logprobs_forward", *fwd(dt=DTYPE_F32))
     _fails(-1, "nimble_tied_logprobs_forward", *fwd(d=9))
@@ -100,6 +100,7 @@ def test_native_tied_logprobs_arguments():
     _fails(-1, "nimble_tied_logprobs_forward", *fwd(out=None))
     _fails(-1, "nimble_tied_logprobs_forward", *fwd(out=None, res=(p, p, None)))
     _fails(-1, "nimble_tied_logprobs_forward", *fwd(off=5, res=(p, p, p)))  # not the whole vocabulary
+    _fails(-1, "nimble_tied_logprobs_forward", *fwd(flag=p))  # nothing to tell without a status word
     _fails(-2, "nimble_tied_logprobs_forward", *fwd(ws=8))
     native.call("nimble_tied_logprobs_forward", *fwd(n=0))
 

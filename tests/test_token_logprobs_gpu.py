@@ -9,6 +9,10 @@ e_s = n u + 2^-22 + 2 u D1 relative, ln s by e_s + u |ln s|; a log probability b
 u (|x - m| + |logp|); the entropy ln s - sum(2^d d) / s by e_s + (n u + 2^-22 + e_s) D1 +
 2 u D2 and roundings of its two terms (``row_bounds``).
 """
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -531,6 +535,42 @@ def test_tied_bad_token():
     check_status(h.device)
 
 
+@pytest.mark.parametrize("grad", [False, True])
+def test_tied_errors_reach_a_later_call(grad):
+    """A bad token and a wait that ran out are raised by the next call, without a copy of the status word."""
+    from nimbleml_b200._native_loader import STATUS_WAIT_TIMEOUT
+    from nimbleml_b200.kernels import fused_tied_crossentropy as k
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    for n in (5, 40):  # both forms of the forward
+        h, w, tokens, g = make_tied(n, 64, 300, torch.bfloat16, n)
+        dev = h.device
+        k.check_status(dev)
+        k.poll_status(dev)
+        want = tied_token_logprobs(h, w, tokens).logprobs
+        bad = tokens.clone()
+        bad[2] = 300
+        hl = h.detach().requires_grad_(grad)
+        tied_token_logprobs(hl, w, bad)
+        torch.cuda.synchronize()
+        with pytest.raises(ValueError, match="out of range"):
+            tied_token_logprobs(hl, w, tokens)
+        assert tied_token_logprobs(hl, w, tokens).logprobs.equal(want)  # reported once
+        k.status_word(dev).fill_(STATUS_WAIT_TIMEOUT)  # as a product before the merge leaves it
+        tied_token_logprobs(hl, w, tokens)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="timed out"):
+            tied_token_logprobs(hl, w, tokens)
+        r = tied_token_logprobs(hl, w, tokens)
+        assert r.logprobs.equal(want) and k.check_status(dev) == 0
+        if grad:
+            r = tied_token_logprobs(hl, w, bad)
+            torch.cuda.synchronize()
+            with pytest.raises(ValueError, match="out of range"):
+                torch.autograd.grad(r.logprobs.nan_to_num().sum(), hl)
+            assert k.check_status(dev) == 0
+
+
 @pytest.mark.parametrize("tied", [False, True])
 def test_captured_and_on_another_stream(tied):
     """Forward and backward in a CUDA graph, replayed on new values, equal the eager calls bit for bit."""
@@ -569,3 +609,37 @@ def test_captured_and_on_another_stream(tied):
         if not turn:
             for x, y in zip(on_side, want):
                 assert x.equal(y)
+
+
+FIRST_CALL = """
+import torch
+from nimbleml_b200.losses import tied_token_logprobs, token_logprobs
+
+g = torch.Generator().manual_seed(1)
+h, w = torch.randn(4, 64, generator=g).cuda().half(), torch.randn(300, 64, generator=g).cuda().half()
+x, tokens = torch.randn(4, 300, generator=g).cuda(), torch.tensor([1, 2, 3, 299], device="cuda")
+side = torch.cuda.Stream()
+for call in (lambda: token_logprobs(x, tokens), lambda: tied_token_logprobs(h, w, tokens)):
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    except RuntimeError as e:
+        assert "once on this device" in str(e), e
+    else:
+        raise SystemExit("a first call was captured")
+token_logprobs(x, tokens)  # readies the device for both
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    r = tied_token_logprobs(h, w, tokens)
+graph.replay()
+want = tied_token_logprobs(h, w, tokens)
+assert r.logprobs.equal(want.logprobs) and r.entropy.equal(want.entropy)
+print("ok")
+"""
+
+
+def test_first_call_in_a_capture_is_refused():
+    run = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
