@@ -54,6 +54,12 @@ Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type).memory_format(c10::nullopt).requires_grad(false));
 }
 
+// t in a type, contiguous; t itself, without a call to torch, where it is both.
+Tensor as_type(const Tensor& t, at::ScalarType type) {
+  if (t.scalar_type() == type && t.is_contiguous()) return t;
+  return t.to(type).contiguous();
+}
+
 // (n, d) rows of x: a view where its rows are contiguous and do not overlap, else a
 // copy; and their pitch.
 Tensor rows_of(const Tensor& x, int64_t& n, int64_t& d, int64_t& pitch) {
@@ -79,8 +85,8 @@ NormArgs norm_args(const Tensor& x, const Tensor& gamma, const std::optional<Ten
   const auto own = x.scalar_type();
   const bool same = gamma.scalar_type() == own && (!beta || beta->scalar_type() == own);
   const auto type = same ? own : at::kFloat;
-  a.gamma = gamma.to(type).contiguous();
-  if (beta) a.beta = beta->to(type).contiguous();
+  a.gamma = as_type(gamma, type);
+  if (beta) a.beta = as_type(*beta, type);
   return a;
 }
 
@@ -118,7 +124,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     const c10::cuda::CUDAGuard guard(x.device());
     const int64_t n = x.size(0), d = x.size(1);
     const int64_t beta_type = ctx->saved_data["beta"].toInt();
-    const Tensor gy = grads[0].to(x.scalar_type()).contiguous();
+    const Tensor gy = as_type(grads[0], x.scalar_type());
     Tensor gx = empty(gy.sizes(), x, x.scalar_type());
     Tensor gg = empty({d}, x, at::kFloat), gb;
     if (beta_type >= 0) gb = empty({d}, x, at::kFloat);
@@ -132,8 +138,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
                                        gb.defined() ? gb.mutable_data_ptr<float>() : nullptr, ws.mutable_data_ptr(),
                                        bytes, stream_of(x)),
              "nimble_layernorm_backward");
-    gg = gg.to(static_cast<at::ScalarType>(ctx->saved_data["gamma"].toInt()));
-    if (gb.defined()) gb = gb.to(static_cast<at::ScalarType>(beta_type));
+    gg = as_type(gg, static_cast<at::ScalarType>(ctx->saved_data["gamma"].toInt()));
+    if (gb.defined()) gb = as_type(gb, static_cast<at::ScalarType>(beta_type));
     return {gx, gg, gb, Tensor()};
   }
 };
@@ -187,7 +193,7 @@ RowsOut rows_forward(const Tensor& logits, const Tensor& tokens, int64_t ignore_
   return o;
 }
 
-Tensor grad_rows(const Tensor& g) { return g.defined() ? g.to(at::kFloat).contiguous() : g; }
+Tensor grad_rows(const Tensor& g) { return g.defined() ? as_type(g, at::kFloat) : g; }
 const float* ptr_or_null(const Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 
 struct TokenLogProbsNode : torch::autograd::Function<TokenLogProbsNode> {
@@ -251,15 +257,16 @@ py::tuple token_logprobs(const Tensor& logits, const Tensor& tokens, int64_t ign
 
 // ------------------------------------------------------- tied log probabilities
 // The package's hooks around a tied call: `poll` raises what an earlier call reported,
-// `snapshot` queues the copy of the status word that the next one reads (a forward needs
-// none: its last kernel raises the host's flag itself, where the copy and its event took
-// 7 of 38 us of a call with few tokens). A captured launch must not be joined by either.
+// `check` waits for this one. No call queues a copy of the status word: a forward's last
+// kernel raises the host's flag for all that the word holds by then, a backward's errors
+// among them (a copy and its event took 7 of 38 us of a call with few tokens). A
+// captured launch must not be joined by either hook.
 py::object* status_hooks[2] = {nullptr, nullptr};
-enum Hook { kPoll = 0, kSnapshot = 1 };
-void set_status_hooks(py::object poll, py::object snapshot) {
+enum Hook { kPoll = 0, kCheck = 1 };
+void set_status_hooks(py::object poll, py::object check) {
   for (py::object*& h : status_hooks) delete h;
   status_hooks[kPoll] = new py::object(std::move(poll));
-  status_hooks[kSnapshot] = new py::object(std::move(snapshot));
+  status_hooks[kCheck] = new py::object(std::move(check));
 }
 void status_hook(Hook which, const Tensor& t) {
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return;
@@ -328,7 +335,7 @@ void tied_backward(const std::optional<Tensor>& g_logprob, const std::optional<T
 
 // Contiguous and on a 16-byte boundary, as the TMA loads need it.
 Tensor for_tma(const Tensor& t) {
-  const Tensor c = t.contiguous();
+  const Tensor c = t.is_contiguous() ? t : t.contiguous();
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
@@ -339,7 +346,7 @@ TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& to
                    int64_t status, int64_t host_flag) {
   const c10::cuda::CUDAGuard guard(hidden.device());
   TiedRows r;
-  r.w = for_tma(weights.to(hidden.scalar_type()));
+  r.w = for_tma(as_type(weights, hidden.scalar_type()));
   r.h = for_tma(hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)}));
   status_hook(kPoll, r.h);
   const auto shape = hidden.sizes().slice(0, hidden.dim() - 1);
@@ -357,13 +364,15 @@ TiedRows tied_rows(const Tensor& hidden, const Tensor& weights, const Tensor& to
 struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
   static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weights, const Tensor& tokens,
                                int64_t ignore_index, const std::optional<Tensor>& buffer, int64_t slab_bytes,
-                               int64_t status, int64_t host_flag) {
+                               int64_t status, int64_t host_flag, bool check) {
     TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status, host_flag);
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({r.h, r.w, tokens, r.lse, r.entropy});
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["slab_bytes"] = slab_bytes;
     ctx->saved_data["status"] = status;
+    ctx->saved_data["host_flag"] = host_flag;
+    ctx->saved_data["check"] = check;
     ctx->saved_data["weights"] = static_cast<int64_t>(weights.scalar_type());
     ctx->saved_data["shape"] = hidden.sizes().vec();
     if (buffer) ctx->saved_data["buffer"] = *buffer;
@@ -371,7 +380,7 @@ struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "the log probabilities' backward is not differentiable itself");
-    variable_list out(8);
+    variable_list out(9);
     if (!grads[0].defined() && !grads[1].defined()) return out;
     const auto saved = ctx->get_saved_variables();
     const Tensor &h = saved[0], &w = saved[1];
@@ -383,12 +392,12 @@ struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
     if (accumulate) gw = buffer->second.toTensor();
     else if (ctx->needs_input_grad(1))
       gw = empty(w.sizes(), w, static_cast<at::ScalarType>(ctx->saved_data["weights"].toInt()));
-    status_hook(kPoll, h);
+    if (*reinterpret_cast<volatile int*>(ctx->saved_data["host_flag"].toInt())) status_hook(kPoll, h);
     tied_backward(grads[0].defined() ? std::optional<Tensor>(grads[0]) : std::nullopt,
                   grads[1].defined() ? std::optional<Tensor>(grads[1]) : std::nullopt, h, w, saved[2], saved[3],
                   saved[4], 0, w.size(0), ctx->saved_data["ignore_index"].toInt(), gh, gw, accumulate,
                   ctx->saved_data["slab_bytes"].toInt(), ctx->saved_data["status"].toInt());
-    status_hook(kSnapshot, h);
+    if (ctx->saved_data["check"].toBool()) status_hook(kCheck, h);
     if (gh) out[0] = *gh;
     if (gw && !accumulate) out[1] = *gw;
     return out;
@@ -397,13 +406,15 @@ struct TiedLogProbsNode : torch::autograd::Function<TiedLogProbsNode> {
 
 py::tuple tied_token_logprobs(const Tensor& hidden, const Tensor& weights, const Tensor& tokens, int64_t ignore_index,
                               const std::optional<Tensor>& buffer, int64_t slab_bytes, int64_t status,
-                              int64_t host_flag) {
+                              int64_t host_flag, bool check) {
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weights.requires_grad())) {
     const variable_list out =
-        TiedLogProbsNode::apply(hidden, weights, tokens, ignore_index, buffer, slab_bytes, status, host_flag);
+        TiedLogProbsNode::apply(hidden, weights, tokens, ignore_index, buffer, slab_bytes, status, host_flag, check);
+    if (check) status_hook(kCheck, hidden);
     return py::make_tuple(out[0], out[1]);
   }
   const TiedRows r = tied_rows(hidden, weights, tokens, ignore_index, status, host_flag);
+  if (check) status_hook(kCheck, hidden);
   return py::make_tuple(r.logprob, r.entropy);
 }
 

@@ -159,7 +159,7 @@ def _after_call(device: torch.device) -> None:
 
 
 host.set_status_hooks(lambda index: poll_status(torch.device("cuda", index)),
-                      lambda index: _after_call(torch.device("cuda", index)))
+                      lambda index: check_status(torch.device("cuda", index)))
 
 
 def _shard_forward(hidden, weights, tokens, ignore_index, vocab_offset, vocab_size, group):
@@ -275,11 +275,8 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
     if v == vocab_size and vocab_parallel.world_size(group) == 1:
         dev = hidden.device
-        out = TokenLogProbs(*host.tied_token_logprobs(hidden, weights, ids, ign, grad_weights_buffer, SLAB_BYTES,
-                                                      _status_ptr(dev), _monitor(dev).flag_ptr))
-        if CHECK_BOUNDS:
-            check_status(dev)
-        return out
+        return TokenLogProbs(*host.tied_token_logprobs(hidden, weights, ids, ign, grad_weights_buffer, SLAB_BYTES,
+                                                       _status_ptr(dev), _monitor(dev).flag_ptr, CHECK_BOUNDS))
     args = (hidden, weights, ids, ign, int(vocab_offset), vocab_size, group)
     if (hidden.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
         lp, ent = _ShardTokenLogProbs.apply(*args, grad_weights_buffer)

@@ -569,6 +569,35 @@ def test_tied_errors_reach_a_later_call(grad):
             with pytest.raises(ValueError, match="out of range"):
                 torch.autograd.grad(r.logprobs.nan_to_num().sum(), hl)
             assert k.check_status(dev) == 0
+            # What a backward reports, the next forward finds.
+            r = tied_token_logprobs(hl, w, tokens)
+            torch.autograd.grad(r.logprobs.sum(), hl)
+            k.status_word(dev).fill_(STATUS_WAIT_TIMEOUT)
+            tied_token_logprobs(hl, w, tokens)
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="timed out"):
+                k.poll_status(dev)
+            assert k.check_status(dev) == 0
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tied_checked_calls(grad, monkeypatch):
+    """With bounds checks on, the call itself raises."""
+    import nimbleml_b200.losses.logprobs as mod
+
+    monkeypatch.setattr(mod, "CHECK_BOUNDS", True)
+    h, w, tokens, g = make_tied(40, 64, 300, torch.float16, 6)
+    hl = h.requires_grad_(grad)
+    r = mod.tied_token_logprobs(hl, w, tokens)
+    if grad:
+        (gh,) = torch.autograd.grad(r.entropy.sum(), hl, retain_graph=True)
+        mod.status_word(h.device).fill_(1 << 1)
+        with pytest.raises((RuntimeError, ValueError)):
+            torch.autograd.grad(r.entropy.sum(), hl)
+    tokens[1] = 300
+    with pytest.raises(ValueError, match="out of range"):
+        mod.tied_token_logprobs(hl, w, tokens)
+    mod.check_status(h.device)
 
 
 @pytest.mark.parametrize("tied", [False, True])
