@@ -252,7 +252,9 @@ struct Chunk8 {
 };
 
 // Chunks whose pointers allow vectors and whose length is whole blocks of 128: a
-// warp takes kU blocks at a time, all their loads first.
+// warp takes kU blocks at a time and loads the next ones ahead. (353 M weights: four
+// blocks at a time with none ahead 2101 us, one at a time with two or three ahead in
+// shared memory by asynchronous copies 1254 to 1400, this 1113.)
 template <typename G, typename C, bool kCopy>
 __device__ __forceinline__ void chunk_8bit_vec(const Chunk8& k, const AdamScalars& a) {
   constexpr int kU = 2;

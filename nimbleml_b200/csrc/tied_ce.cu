@@ -17,6 +17,9 @@
 //             tcgen05 GEMMs give dE rows of the slab (complete) and add the
 //             slab's share of dh, reading G, h and E in place (MN-major
 //             operands where the contraction runs along their rows).
+// The log probability and entropy of every token (instead of the mean loss) are two
+// more epilogues of the same GEMM, with a slab backward of the same shape and a kernel
+// of their own for few tokens; they follow the cross-entropy entry points below.
 // All GEMMs compute C[M x N] = A[M x K] . B[N x K]^T with operands staged by
 // TMA (128-byte swizzle) into a shared-memory ring and fp32 accumulators
 // double-buffered in TMEM.

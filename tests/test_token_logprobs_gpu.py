@@ -535,6 +535,50 @@ def test_tied_bad_token():
     check_status(h.device)
 
 
+def test_tied_odd_calls():
+    """One row without a batch, no rows, rows that repeat or lie apart, weights of other types and layouts."""
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    h, w, tokens, g = make_tied(6, 64, 300, torch.bfloat16, 12)
+    a, b = torch.randn(6, generator=g).cuda(), torch.randn(6, generator=g).cuda()
+    whole = tied_token_logprobs(h, w, tokens)
+    # One row.
+    hl = h[2].detach().requires_grad_()
+    one = tied_token_logprobs(hl, w, int(tokens[2]))
+    assert one.logprobs.shape == () and one.logprobs == whole.logprobs[2] and one.entropy == whole.entropy[2]
+    (gh,) = torch.autograd.grad(one.logprobs + one.entropy, hl)
+    assert gh.shape == (64,)
+    check_tied_grads(gh.view(1, 64), None, h[2:3], w, tokens[2:3], torch.ones(1).cuda(), torch.ones(1).cuda())
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(tied_token_logprobs(hl, w, 5).logprobs, hl, create_graph=True)
+    # No rows.
+    hl, wl = h[:0].detach().requires_grad_(), w.detach().requires_grad_()
+    none = tied_token_logprobs(hl, wl, tokens[:0])
+    assert none.logprobs.shape == (0,)
+    gh, gw = torch.autograd.grad(none.logprobs.sum() + none.entropy.sum(), (hl, wl))
+    assert gh.shape == (0, 64) and (gw == 0).all() and gw.shape == w.shape
+    # One row for every token.
+    hl = h[1].detach().requires_grad_()
+    same = tied_token_logprobs(hl.expand(6, 64), w, tokens)
+    rows = h[1:2].expand(6, 64).contiguous()
+    assert same.logprobs.equal(tied_token_logprobs(rows, w, tokens).logprobs)
+    # Rows apart, weights transposed in memory, fp32 masters: their gradient is fp32.
+    wide = torch.zeros(6, 100, dtype=h.dtype, device="cuda")
+    wide[:, 8:72] = h
+    hl, wl = wide[:, 8:72].detach().requires_grad_(), w.t().contiguous().t().float().requires_grad_()
+    assert not hl.is_contiguous() and not wl.is_contiguous()
+    r = tied_token_logprobs(hl, wl, tokens)
+    assert r.logprobs.equal(whole.logprobs) and r.entropy.equal(whole.entropy)
+    gh, gw = torch.autograd.grad((r.logprobs, r.entropy), (hl, wl), (a, b))
+    assert gw.dtype == torch.float32 and gh.dtype == h.dtype
+    check_tied_grads(gh, gw, h, w, tokens, a, b)
+    # Upstream gradients that repeat, and only one of the two results used.
+    hl = h.detach().requires_grad_()
+    r = tied_token_logprobs(hl.view(2, 3, 64), w, tokens.view(2, 3))
+    (gh,) = torch.autograd.grad(r.entropy.sum(), hl)
+    check_tied_grads(gh, None, h, w, tokens, torch.zeros(6).cuda(), torch.ones(6).cuda())
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_tied_errors_reach_a_later_call(grad):
     """A bad token and a wait that ran out are raised by the next call, without a copy of the status word."""
