@@ -253,18 +253,23 @@ __device__ __forceinline__ uint32_t key_col(uint64_t key) { return ~static_cast<
 // thread notes the maxima of up to kSegs segments of its share. The k-th best of
 // the threads' maxima, found by bisection over counts, is no better than the k-th
 // best logit; only segments that reach it are read again (from L2: k of 16 x 256
-// and a few more), and what reaches it there is sorted. Keeping a list of
+// and a few more, listed first and shared out over all threads), and what reaches it
+// there is sorted. Keeping a list of
 // candidates against a rising threshold inside the pass was measured first: its
 // rare, divergent insertions took 150 to 900 us of a 4096 x 128256 bf16 pass for
 // k = 5 to 64, which takes 150 us by itself.
 constexpr int kMaxTopK = 64;
 constexpr int kRowThreads = 256;
 constexpr int kSegs = 16;
-constexpr int kKeyCap = 2048;  // candidates a block holds
+// Candidates a block holds. Shared memory is taken from the L1 cache, through which the
+// logits come: 19 KB a block instead of 42 (2048 candidates, fp32 maxima, room for every
+// segment in the list) took k = 5 of 4096 x 128256 bf16 from 205 to 193 us, k = 64 of
+// 2048 rows from 124 to 113.
+constexpr int kKeyCap = 1024;
 // The second scan below: candidates beyond kKeyWater are cut back to the best k
-// after each of its steps, which offer at most 4 logits a thread.
-constexpr int kKeyWater = 512;
-static_assert(kKeyWater + 4 * kRowThreads <= kKeyCap, "a step of the second scan must find room");
+// after each of its steps, which offer at most kScan logits a thread.
+constexpr int kKeyWater = 512, kScan = 2;
+static_assert(kKeyWater + kScan * kRowThreads <= kKeyCap, "a step of the second scan must find room");
 
 // Sorts keys[0, n) in descending order (bitonic, whole block); keys must have
 // room for the next power of two of n. Starts and ends with a barrier.
@@ -294,9 +299,12 @@ __device__ void block_sort_desc(uint64_t* keys, int n) {
 struct TopKShared {
   uint64_t keys[kKeyCap];
   uint64_t best[kMaxTopK];  // the best k, sorted
-  float seg_max[kSegs][kRowThreads];
+  uint16_t seg_max[kSegs][kRowThreads];  // upper halves of ordered values
+  // Segments to read again (segment * kRowThreads + thread), each good for one candidate
+  // at least: more than kKeyCap of them are more candidates than that.
+  uint16_t segs[kKeyCap];
   uint64_t tau;  // keys above it are candidates
-  int count;
+  int count, n_segs;
 };
 
 // The best k of the first n candidates, sorted, to sh.best and to the front of
@@ -315,13 +323,13 @@ __device__ int topk_prune(TopKShared& sh, int n, int k) {
     }
     __syncthreads();
     if (threadIdx.x < left) sh.keys[threadIdx.x] = sh.best[threadIdx.x];
+    if (threadIdx.x == 0 && n >= k) sh.tau = sh.best[k - 1];
   } else {
     block_sort_desc(sh.keys, n);
     if (threadIdx.x < left) sh.best[threadIdx.x] = sh.keys[threadIdx.x];
+    if (threadIdx.x == 0) sh.tau = sh.keys[k - 1];  // n > kRowThreads >= k
   }
   if (threadIdx.x == 0) sh.count = left;
-  __syncthreads();
-  if (threadIdx.x == 0 && n >= k) sh.tau = sh.best[k - 1];
   __syncthreads();
   return left;
 }
@@ -330,7 +338,7 @@ __device__ int topk_prune(TopKShared& sh, int n, int k) {
 // A cluster of `parts` blocks per row, each block on one contiguous part of
 // the columns; its first block merges the parts over distributed shared memory.
 // 4096 x 128256 bf16: 149 us without alternatives (7.0 TB/s, some of the rows still in
-// L2), 183 with 5; 2048 x 32000 fp16 28 to 31 us (4.3 TB/s; the exponentials alone, 16 a
+// L2), 176 with 5; 2048 x 32000 fp16 28 to 31 us (4.3 TB/s; the exponentials alone, 16 a
 // clock and SM, are 15). Fetching the next vectors ahead in registers gained nothing.
 template <typename T, bool kTopK>
 __global__ void __launch_bounds__(kRowThreads, kTopK ? 5 : 6)
@@ -377,6 +385,9 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   const int tail0 = head + nvec * kVec;
   const uint4* r4 = reinterpret_cast<const uint4*>(r + head);
 
+  // With alternatives the token's logit comes early: their tail is latency throughout.
+  [[maybe_unused]] float x_tok = 0.0f;
+  if (kTopK && part == 0 && threadIdx.x == 0 && tok >= 0 && tok < V) x_tok = to_f<T>(x[row * ld + tok]);
   SoftStats acc;
   float tau_v = -INFINITY;
   uint64_t tau = 0;
@@ -413,7 +424,7 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
     if constexpr (kTopK) {
       seg_hi = fmaxf(seg_hi, hi);
       if (--seg_left == 0) {
-        sh.seg_max[seg++][threadIdx.x] = seg_hi;  // read by this thread only
+        sh.seg_max[seg++][threadIdx.x] = ordered(seg_hi) >> 16;  // read by this thread only
         seg_hi = -INFINITY;
         seg_left = per_seg;
       }
@@ -428,10 +439,10 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
     acc.add(ragged_v);
   }
   if constexpr (kTopK) {
-    if (seg_left != per_seg) sh.seg_max[seg++][threadIdx.x] = seg_hi;
+    if (seg_left != per_seg) sh.seg_max[seg++][threadIdx.x] = ordered(seg_hi) >> 16;
     if (threadIdx.x == 0) {
       sh.tau = 0;
-      sh.count = 0;
+      sh.count = sh.n_segs = 0;
     }
     // Largest 16-bit prefix of an ordered value that k threads' maxima reach; 0
     // where fewer than k threads have any logit.
@@ -444,22 +455,26 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
     }
     tau_v = prefix <= 0x007Fu ? -INFINITY : unordered(prefix << 16);
     if (ragged) offer(ragged_v, col0 + ragged_j);
-#pragma unroll 1
-    for (int g = 0; g < seg; ++g) {
-      if (!(sh.seg_max[g][threadIdx.x] >= tau_v)) continue;
-#pragma unroll 1
-      for (int p = g * per_seg; p < min(steps, (g + 1) * per_seg); ++p) {
-        uint4 raw[kU];
 #pragma unroll
-        for (int i = 0; i < kU; ++i) raw[i] = vec_at(p, i) < nvec ? __ldg(r4 + vec_at(p, i)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < kU; ++i) {
-          if (vec_at(p, i) >= nvec) continue;
+    for (int g = 0; g < kSegs; ++g)
+      if (g < seg && sh.seg_max[g][threadIdx.x] >= prefix) {
+        const int at = atomicAdd(&sh.n_segs, 1);
+        if (at < kKeyCap) sh.segs[at] = static_cast<uint16_t>(g * kRowThreads + threadIdx.x);
+      }
+    __syncthreads();
+    const int total = min(sh.n_segs, kKeyCap) * kU;
+    for (int q = threadIdx.x; q < total; q += kRowThreads) {
+      const int which = sh.segs[q / kU], i = q % kU;
+      const int g = which / kRowThreads, t = which % kRowThreads;
 #pragma unroll 1
-          for (uint32_t mask = vec_at_least<T>(raw[i], tau_v); mask != 0; mask &= mask - 1) {
-            const int j = __ffs(mask) - 1;
-            offer(vec_elem<T>(raw[i], j), col0 + head + vec_at(p, i) * kVec + j);
-          }
+      for (int p = g * per_seg; p < (g + 1) * per_seg; ++p) {
+        const int v = (p * kU + i) * kRowThreads + t;
+        if (v >= nvec) break;
+        const uint4 raw = __ldg(r4 + v);
+#pragma unroll 1
+        for (uint32_t mask = vec_at_least<T>(raw, tau_v); mask != 0; mask &= mask - 1) {
+          const int j = __ffs(mask) - 1;
+          offer(vec_elem<T>(raw, j), col0 + head + v * kVec + j);
         }
       }
     }
@@ -467,25 +482,26 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
   int kept = 0;
   if constexpr (kTopK) {
     __syncthreads();
-    kept = sh.count;
-    __syncthreads();
+    kept = max(sh.count, sh.n_segs);
     if (kept <= kKeyCap) {
+      kept = sh.count;
       kept = topk_prune(sh, kept, k);
     } else {
       // More candidates than room (a row that rises with its columns): scan the
       // part again, from the threshold that the candidates at hand give, and cut
       // the candidates back between steps. The candidates themselves come again.
-      topk_prune(sh, kKeyCap, k);
+      const int have = min(sh.count, kKeyCap);  // few where the listed segments are NaN
+      topk_prune(sh, have, k);
       if (threadIdx.x == 0) {
-        sh.tau = sh.best[k - 1] - 1;
+        sh.tau = have >= k ? sh.best[k - 1] - 1 : 0;
         sh.count = 0;
       }
       __syncthreads();
       take_threshold();
       kept = 0;
-      for (int j0 = 0; j0 < n; j0 += 4 * kRowThreads) {
+      for (int j0 = 0; j0 < n; j0 += kScan * kRowThreads) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kScan; ++e) {
           const int j = j0 + e * kRowThreads + threadIdx.x;
           if (j < n) offer(to_f<T>(r[j]), col0 + j);
         }
@@ -549,8 +565,8 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
     const RowResult res = row_result(all);
     const bool bad = tok < 0 || tok >= V;
     if (bad && status) atomicOr(status, NIMBLE_STATUS_BAD_LABEL);
-    out_logp[row] =
-        bad ? __int_as_float(0x7fc00000) : token_logprob(to_f<T>(x[row * ld + tok]), res.max, res.logsum);
+    if constexpr (!kTopK) x_tok = bad ? 0.0f : to_f<T>(x[row * ld + tok]);
+    out_logp[row] = bad ? __int_as_float(0x7fc00000) : token_logprob(x_tok, res.max, res.logsum);
     out_ent[row] = res.entropy;
     out_max[row] = res.max;
     out_logsum[row] = res.logsum;
@@ -577,18 +593,19 @@ logprobs_rows_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __restr
 constexpr int kShortVecs = 512;
 constexpr int kLaneVecs = kShortVecs / 32;
 constexpr int kShortWarps = 8;
-constexpr int kShortCap = 512;
+constexpr int kShortCap = 256;
 // Fewer rows take a block each: a warp alone is slower than a block where there are
 // no other rows to hide it (600 / 1200 / 8000 rows of 2000 fp16 logits: 7.0 / 8.4 / 34
 // us by blocks, 7.1 / 7.2 / 12.5 by warps; with 64 alternatives 12.4 / 17.8 / 84
 // against 16.0 / 16.7 / 43).
 constexpr int64_t kShortRows = 1024;
 constexpr int kShortWater = 128;  // of the second scan, whose steps offer at most 128 logits
+static_assert(kShortWater + 128 <= kShortCap, "a step of the second scan must find room");
 
 struct ShortTopK {
   uint64_t keys[kShortCap];
   uint64_t best[kMaxTopK];
-  float vec_max[kLaneVecs][32];
+  uint16_t vec_max[kLaneVecs][32];  // upper halves of ordered values
   int count;
 };
 
@@ -652,7 +669,7 @@ logprobs_short_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __rest
       for (int i = 0; i < kU; ++i) {
         const uint4 one[1] = {raw[i]};
         const float v = vec_max<T, 1>(one);
-        sh.vec_max[s0 + i][lane] = v;  // s0 + i < kLaneVecs: nvec <= kShortVecs, a multiple of 32 kU
+        sh.vec_max[s0 + i][lane] = ordered(v) >> 16;  // s0 + i < kLaneVecs: nvec <= kShortVecs, a multiple of 32 kU
         group_max[i] = fmaxf(group_max[i], v);
         hi = fmaxf(hi, v);
       }
@@ -721,7 +738,7 @@ logprobs_short_kernel(const T* __restrict__ x, int64_t ld, const int64_t* __rest
 #pragma unroll 1
     for (int s = 0; s < lanes_of; ++s) {
       const int q = s * 32 + lane;
-      if (q >= nvec || !(sh.vec_max[s][lane] >= tau_v)) continue;
+      if (q >= nvec || sh.vec_max[s][lane] < prefix) continue;
       const uint4 raw = __ldg(r4 + q);
 #pragma unroll 1
       for (uint32_t mask = vec_at_least<T>(raw, tau_v); mask != 0; mask &= mask - 1) {

@@ -274,6 +274,34 @@ def test_masked_row_with_a_nan(dtype):
     assert (g[0] == 0).all() and torch.isnan(g[1]).all() and (g[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1, 20, 64])
+def test_top_k_crowded(dtype, k):
+    """Rows whose alternatives are hard to tell apart, over more segments than a block lists: equal ones, rising ones
+    within a part in 300, masked ones, and NaN with few numbers among them (fewer than k in one row)."""
+    from nimbleml_b200.losses import token_logprobs
+
+    v = 70001
+    g = torch.Generator().manual_seed(k)
+    x = torch.full((7, v), 0.75)
+    x[1] = 4.0 + torch.arange(v) / v / 80
+    x[2] = -x[1]
+    x[3] = -torch.inf
+    x[4] = torch.where(torch.rand(v, generator=g) < 0.5, 0.75, -torch.inf)
+    x[5] = torch.nan
+    x[5, torch.randperm(v, generator=g)[:40]] = torch.randn(40, generator=g)
+    x[6] = torch.where(torch.rand(v, generator=g) < 0.9, torch.nan, -1.0)
+    x = x.to(dtype).cuda()
+    r = token_logprobs(x, torch.zeros(7, dtype=torch.int64, device="cuda"), top_k=k)
+    for i in range(7):
+        row = x[i].double()
+        at = (~torch.isnan(row)).nonzero().squeeze(1)
+        order = at[torch.sort(row[at], descending=True, stable=True).indices[:k]]
+        want = torch.full((k,), -1, device="cuda")
+        want[:len(order)] = order
+        assert r.top_ids[i].equal(want), i
+
+
 def test_one_row_without_a_batch():
     from nimbleml_b200.losses import token_logprobs
 
