@@ -70,7 +70,12 @@ constexpr int kSmemBytesPair = kStagesPair * (kABytes + kBBytes / 2) + kStoreByt
 // EPI_LP_FWD / EPI_LP_GRAD are the cross-entropy epilogues of the per-token log
 // probabilities: the forward also sums d 2^d (d = (s - max) log2 e) for the
 // entropy, the gradient has coefficients of its own for every row.
-enum Epi : int { EPI_CE_FWD = 0, EPI_CE_GRAD = 1, EPI_STORE = 2, EPI_LP_FWD = 3, EPI_LP_GRAD = 4 };
+// EPI_LP_STORE is EPI_STORE for a result in the compute type that nothing is added to,
+// written like G by TMA stores: a thread's 16-byte stores into its own row took the
+// backward of 16 / 320 / 2048 x 768 x 50257 103 / 131 / 388 us, 83 / 116 / 383 so.
+enum Epi : int { EPI_CE_FWD = 0, EPI_CE_GRAD = 1, EPI_STORE = 2, EPI_LP_FWD = 3, EPI_LP_GRAD = 4, EPI_LP_STORE = 5 };
+// Epilogues whose tiles leave through the staging buffers and the tensor map of the result.
+__host__ __device__ constexpr bool tma_out(int epi) { return epi == EPI_CE_GRAD || epi == EPI_LP_GRAD || epi == EPI_LP_STORE; }
 // Lower limit of d where it multiplies 2^d (zero long before).
 constexpr float kMinD = -1.0e4f;
 
@@ -376,7 +381,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
     constexpr int kChunks32 = kBN / 32 / kColHalves;  // 32-column chunks per warp
     const int c_begin = ch * kChunks32, c_end = c_begin + kChunks32;
     float alpha = 1.0f;
-    if constexpr (EPI == EPI_STORE) {
+    if constexpr (EPI == EPI_STORE || EPI == EPI_LP_STORE) {
       const float num = ep.alpha_num ? *ep.alpha_num : 1.0f;
       const float den = ep.alpha_den ? *ep.alpha_den : 1.0f;
       alpha = (den != 0.0f) ? num / den * ep.alpha_mult : 0.0f;
@@ -476,8 +481,8 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           // Only the warp whose column half holds the label writes the target.
           if (tcol >= c_begin * 32 && tcol < c_end * 32) ep.tgt[row] = tval;
         }
-      } else if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
-        const int64_t lab = row_ok ? ep.labels[row] : ep.ignore_index;
+      } else if constexpr (tma_out(EPI)) {
+        const int64_t lab = EPI != EPI_LP_STORE && row_ok ? ep.labels[row] : ep.ignore_index;
         const bool live = row_ok && lab != ep.ignore_index;
         const int64_t rel = live ? lab - ep.col_origin - col0_tile : -1;
         const int tcol = (rel >= 0 && rel < ncols) ? static_cast<int>(rel) : -1;
@@ -514,6 +519,10 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
           float v[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
+            if constexpr (EPI == EPI_LP_STORE) {
+              v[j] = __uint_as_float(r[j]) * alpha;
+              continue;
+            }
             const float d = fmaf(__uint_as_float(r[j]), kLog2e, -lse_l2);
             float p = ptx::ex2(d);
             if constexpr (EPI == EPI_LP_GRAD) {
@@ -633,7 +642,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       release(acc);
     }
     // Every G store must have landed before the CTA exits.
-    if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
+    if constexpr (tma_out(EPI)) {
       if (lane == 0) ptx::bulk_wait<0>();
       __syncwarp();
     }
@@ -843,12 +852,12 @@ constexpr int kSmemBytesWide = kStagesWide * (2 * kABytes + kBBytes) + kStoreByt
 // 4096 x 2048 x 32000 383 / 410 / 431 against 379 / 421 / 430. At most 128 rows fill
 // half a wide tile and take the small ones too.
 constexpr int64_t kShortK = 2048;
-// Of these short ones CTA pairs take the recompute from 512 tokens and dE from 1024 on
-// (2048 x 768 x 50257: 134 -> 124 us and 133 -> 115). With fewer a pair has too little
-// to do between two tiles: the backward of 320 x 768 x 50257 takes 131 us, 140 with the
-// recompute in pairs, 139 with dE; that of 1024 tokens 233, 231 and 228. The forward
-// gains nothing (119 against 120).
-constexpr int64_t kPairTokensGrad = 512, kPairTokensDe = 1024;
+// Of these short ones CTA pairs take the recompute and dE from 512 tokens on (2048 x 768 x
+// 50257: 134 -> 124 us and 133 -> 115). With fewer a pair has too little to do between
+// two tiles: the backward of 300 x 768 x 50257 takes 116 us, 124 with the recompute in
+// pairs, 117 with dE; that of 600 tokens 166, of 1000 tokens 224 with dE in single CTAs
+// against 161 and 216. The forward gains nothing (119 against 120).
+constexpr int64_t kPairTokens = 512;
 template <int EPI, bool kAMN>
 constexpr int gemm_kind_bit() {
   return (EPI == EPI_CE_FWD || EPI == EPI_LP_FWD) ? 1 : (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) ? 2 : kAMN ? 4 : 8;
@@ -916,14 +925,15 @@ int launch_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t 
   if (max_ctas > 0 && max_ctas < di.sms) di.sms = max_ctas;
   CUtensorMap ma, mb, mc;
   if (int rc = make_operand_map(&ma, A, dtype, kAMN, K, M, lda, kBM)) return rc;
-  if constexpr (EPI == EPI_CE_GRAD || EPI == EPI_LP_GRAD) {
+  if constexpr (tma_out(EPI)) {
     if (int rc = make_store_map(&mc, ep.g, dtype, N, M, ep.ldg)) return rc;
   } else {
     mc = ma;  // unused by the other epilogues
   }
   const bool lp_short = ep.log_probs && K <= kShortK;
-  const bool lp_pairs = lp_short && (EPI == EPI_LP_GRAD ? M >= kPairTokensGrad
-                                                        : EPI == EPI_STORE && kAMN && K >= kPairTokensDe);
+  // The tokens are the recompute's rows and dE's contraction.
+  constexpr bool kDe = (EPI == EPI_STORE || EPI == EPI_LP_STORE) && kAMN;
+  const bool lp_pairs = lp_short && (EPI == EPI_LP_GRAD ? M >= kPairTokens : kDe && K >= kPairTokens);
   const bool pairs = (g_cta_pairs & gemm_kind_bit<EPI, kAMN>()) != 0 || lp_pairs;
   if (int rc = make_operand_map(&mb, B, dtype, kBMN, K, N, ldb, pairs ? kBN / 2 : kBN)) return rc;
   const int group_m = g_group_m;
@@ -979,7 +989,7 @@ int gemm_dispatch(int dtype, const void* A, int64_t lda, const void* B, int64_t 
       return launch_gemm<__nv_bfloat16, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
     case NIMBLE_DTYPE_F32:
       // The log-probability epilogues serve 16-bit operands only.
-      if constexpr (EPI != EPI_LP_FWD && EPI != EPI_LP_GRAD)
+      if constexpr (EPI != EPI_LP_FWD && EPI != EPI_LP_GRAD && EPI != EPI_LP_STORE)
         return launch_gemm<float, EPI, kAMN, kBMN>(A, lda, B, ldb, M, N, K, dtype, ep, s, max_ctas);
   }
   return fail(NIMBLE_ERR_INVALID_ARG, "unknown dtype");
@@ -1022,7 +1032,8 @@ int launch_split(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t
 // 1000 / cols of the product's own tiles / 74 (bytes at 6.5 TB/s against operations at
 // 1.6 PFLOP/s); without a split a tile stays with one SM, at half the pair's speed. A run
 // has 512 columns or more. The whole backward of 64 / 512 / 2048 tokens (d 768, 1024, 768;
-// V 50257, 32000, 50257): 543 / 399 / 795 us with one run, 104 / 128 / 395 with these.
+// V 50257, 32000, 50257): 543 / 399 / 795 us with one run, 104 / 128 / 395 with these
+// (dE's tiles still written by single threads).
 int dh_splits(int64_t n_tokens, int64_t d_model, int64_t cols) {
   constexpr int kPairs = 74, kMaxRuns = 32;
   const int64_t tiles = std::max<int64_t>(1, (n_tokens + 255) / 256 * ((d_model + 255) / 256));
@@ -1266,6 +1277,12 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
       ee.accum_out = accumulate_grad_weights ? 1 : 0;
       ee.status = status;
       ee.log_probs = eg_base.log_probs;
+      if (EPI == EPI_LP_GRAD && grad_weights_dtype == dtype && !accumulate_grad_weights) {
+        ee.g = ee.out;
+        ee.ldg = d_model;
+        return gemm_dispatch<EPI_LP_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
+                                                       r1 - r0, d_model, n_tokens, ee, s, max_ctas);
+      }
       return gemm_dispatch<EPI_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
                                                   r1 - r0, d_model, n_tokens, ee, s, max_ctas);
     };
@@ -1856,11 +1873,15 @@ __global__ void split_sum_kernel(const float* __restrict__ partial, int runs, in
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     float v[8];
     load8<float>(partial + 8 * i, v);
-    for (int r = 1; r < runs; ++r) {
-      float w[8];
-      load8<float>(partial + r * stride + 8 * i, w);
+    constexpr int kU = 4;  // runs in flight; those behind the last are read again and not added
+    for (int r0 = 1; r0 < runs; r0 += kU) {
+      float w[kU][8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += w[k];
+      for (int u = 0; u < kU; ++u) load8<float>(partial + min(r0 + u, runs - 1) * stride + 8 * i, w[u]);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += r0 + u < runs ? w[u][k] : 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] *= a;
