@@ -449,28 +449,19 @@ void check_quantized(const Tensor& codes, const Tensor& scales) {
 
 void adamw_step_many(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_,
                      const py::object& copies_, int64_t step, double lr, double beta1, double beta2, double eps,
-                     double wd) {
+                     double wd, bool own_steps) {
   const Items params(params_), grads(grads_), ms(m_), vs(v_);
   std::optional<Items> copies;
   if (!copies_.is_none()) copies.emplace(copies_);
   TORCH_CHECK_VALUE(grads.n == params.n && ms.n == params.n && vs.n == params.n && (!copies || copies->n == params.n),
                     "params, grads, exp_avgs, exp_avg_sqs and copies must have one entry per tensor");
   TORCH_CHECK_VALUE(step >= 1, "step counts from 1, got ", step);
-  std::vector<nimble_adamw_tensor> rows;
-  rows.reserve(params.n);
-  std::unordered_set<const void*> seen;
-  std::vector<Tensor> keep;  // contiguous copies of gradients, until the launch is queued
+  std::vector<nimble_adamw_tensor> all;
+  all.reserve(params.n);
+  std::vector<Tensor> keep;  // contiguous copies of gradients, until the launches are queued
   std::optional<at::Device> dev;
   bool eight = false;
-  auto launch = [&] {
-    if (rows.empty()) return;
-    const c10::cuda::CUDAGuard guard(*dev);
-    check_rc(nimble_adamw_step_many(rows.data(), static_cast<int>(rows.size()), eight ? 8 : 32, lr, beta1, beta2,
-                                    1.0 - std::pow(beta1, static_cast<double>(step)),
-                                    1.0 - std::pow(beta2, static_cast<double>(step)), eps, wd,
-                                    c10::cuda::getCurrentCUDAStream(dev->index()).stream()),
-             "nimble_adamw_step_many");
-  };
+  // Every tensor is checked before the first launch: a refused step leaves all of them as they were.
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     if (grads.at[i] == Py_None) continue;
     const Tensor& p = tensor_in(params.at[i], "a parameter");
@@ -528,13 +519,45 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
     r.grad = g->data_ptr();
     r.n = n;
     r.grad_dtype = gdt;
-    if (!seen.insert(r.weights).second) {  // listed twice: its second update follows the first
-      launch();
-      rows.clear();
-      seen.clear();
-      seen.insert(r.weights);
+    all.push_back(r);
+  }
+  if (all.empty()) return;
+  const c10::cuda::CUDAGuard guard(*dev);
+  void* stream = c10::cuda::getCurrentCUDAStream(dev->index()).stream();
+  const double bc1 = 1.0 - std::pow(beta1, static_cast<double>(step));
+  const double bc2 = 1.0 - std::pow(beta2, static_cast<double>(step));
+  std::vector<nimble_adamw_tensor> rows;
+  rows.reserve(all.size());
+  std::unordered_set<const void*> seen;
+  auto launch = [&] {
+    if (!rows.empty())
+      check_rc(nimble_adamw_step_many(rows.data(), static_cast<int>(rows.size()), eight ? 8 : 32, lr, beta1, beta2,
+                                      bc1, bc2, eps, wd, stream),
+               "nimble_adamw_step_many");
+    rows.clear();
+    seen.clear();
+  };
+  auto whole = [](const nimble_adamw_tensor& t) {  // what the single step's vector kernel takes
+    uintptr_t bits = 0;
+    for (const void* p : {static_cast<const void*>(t.weights), t.grad, static_cast<const void*>(t.exp_avg),
+                          static_cast<const void*>(t.exp_avg_sq), static_cast<const void*>(t.weights_copy)})
+      bits |= reinterpret_cast<uintptr_t>(p);
+    return t.n % 8 == 0 && (bits & 15) == 0;
+  };
+  for (const nimble_adamw_tensor& t : all) {
+    const bool alone = own_steps && !eight && !whole(t);
+    if (seen.count(t.weights)) launch();  // listed twice: its second update follows the first
+    if (alone) {
+      check_rc(nimble_adamw_step(t.weights, t.grad, t.grad_dtype, static_cast<float*>(t.exp_avg),
+                                 static_cast<float*>(t.exp_avg_sq), t.n, static_cast<float>(lr),
+                                 static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(bc1),
+                                 static_cast<float>(bc2), static_cast<float>(eps), static_cast<float>(wd),
+                                 t.weights_copy, t.weights_copy_dtype, stream),
+               "nimble_adamw_step");
+      continue;
     }
-    rows.push_back(r);
+    seen.insert(t.weights);
+    rows.push_back(t);
   }
   launch();
 }

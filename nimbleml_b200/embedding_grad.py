@@ -122,10 +122,11 @@ def adamw_step_many(params: Sequence[torch.Tensor], grads: Sequence[Optional[tor
     With 8-bit moments the weights are updated from the new moments before
     these are rounded. A gradient that is not finite spoils its own weight and,
     with 8-bit moments, the block of 128 it lies in. A captured step keeps the
-    scalars it was captured with.
+    scalars it was captured with. All tensors are checked first: a step that is
+    refused changes none of them.
     """
     host.adamw_step_many(params, grads, exp_avgs, exp_avg_sqs, copies, int(step), float(learning_rate), float(beta1),
-                         float(beta2), float(epsilon), float(weight_decay))
+                         float(beta2), float(epsilon), float(weight_decay), False)
 
 
 class AdamW:
@@ -149,6 +150,8 @@ class AdamW:
             raise ValueError("state_bits must be 32 or 8")
         self.state_bits = int(state_bits)
         self.copies = list(copies) if copies is not None else [None] * len(self.params)
+        if len(self.copies) != len(self.params):
+            raise ValueError(f"copies must have one entry per tensor: {len(self.copies)} for {len(self.params)}")
         self.lr, self.beta1, self.beta2 = float(learning_rate), float(beta1), float(beta2)
         self.epsilon, self.weight_decay = float(epsilon), float(weight_decay)
         self.m = [self._zero_moment(p) for p in self.params]
@@ -169,32 +172,15 @@ class AdamW:
 
     @torch.no_grad()
     def step(self):
+        """One step over all tensors with a gradient; a refused one changes neither them nor ``t``.
+
+        With fp32 moments, tensors that are not whole eights on 16-byte
+        boundaries keep a launch of their own (``nimble_adamw_step``), whose
+        scalar kernel rounds in another order than the list's.
+        """
+        host.adamw_step_many(self.params, [p.grad for p in self.params], self.m, self.v, self.copies, self.t + 1,
+                             self.lr, self.beta1, self.beta2, self.epsilon, self.weight_decay, True)
         self.t += 1
-        grads = [p.grad for p in self.params]
-        if self.state_bits == 32:
-            # Tensors that are not whole eights on 16-byte boundaries keep a
-            # step of their own, whose scalar kernel rounds in another order.
-            for i, (p, g) in enumerate(zip(self.params, grads)):
-                if g is not None and not self._whole(p, g, self.m[i], self.v[i], self.copies[i]):
-                    self._step_alone(i, g.contiguous())
-                    grads[i] = None
-        adamw_step_many(self.params, grads, self.m, self.v, step=self.t, learning_rate=self.lr, beta1=self.beta1,
-                        beta2=self.beta2, epsilon=self.epsilon, weight_decay=self.weight_decay, copies=self.copies)
-
-    @staticmethod
-    def _whole(p, *others) -> bool:
-        return p.numel() % 8 == 0 and not any(t is not None and t.data_ptr() & 15 for t in (p, *others))
-
-    def _step_alone(self, i: int, g: torch.Tensor) -> None:
-        p, m, v, c = self.params[i], self.m[i], self.v[i], self.copies[i]
-        if not p.is_cuda or any(t is not None and t.device != p.device for t in (g, m, v, c)):
-            raise ValueError("AdamW needs its weights, gradients, moments and copies on one CUDA device")
-        with _on(p.device):
-            native.call("nimble_adamw_step", p.data_ptr(), g.data_ptr(), _TORCH_TO_NIMBLE[g.dtype], m.data_ptr(),
-                        v.data_ptr(), p.numel(), self.lr, self.beta1, self.beta2, 1.0 - self.beta1 ** self.t,
-                        1.0 - self.beta2 ** self.t, self.epsilon, self.weight_decay,
-                        c.data_ptr() if c is not None else None, _TORCH_TO_NIMBLE[c.dtype] if c is not None else 0,
-                        _stream_ptr(p.device))
 
     def zero_grad(self, set_to_none: bool = True):
         for p in self.params:

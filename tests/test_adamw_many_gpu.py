@@ -316,3 +316,46 @@ def test_gradients_with_strides():
         adamw_step_many([w], [g[:3]], [one[1]], [one[2]], step=1)
     with pytest.raises(ValueError, match="moments"):
         adamw_step_many([w], [g], [one[1]], [one[2][:3]], step=1)
+
+
+@pytest.mark.parametrize("size", [5, 301, 16])
+@pytest.mark.parametrize("fault", ["short", "long", "strided", "type", "moment", "late"])
+def test_a_refused_step_changes_nothing(size, fault):
+    """Copies and moments that do not fit, whatever the weights' sizes: ValueError before anything is launched."""
+    from nimbleml_b200.embedding_grad import AdamW
+
+    ps = [torch.full((7,), 2.0, device="cuda"), torch.full((size,), 1.0, device="cuda"), torch.full((24,), 3.0, device="cuda")]
+    for p in ps:
+        p.grad = torch.full_like(p, 0.5)
+    bad = {"short": torch.zeros(size - 1, device="cuda"), "long": torch.zeros(size + 1, device="cuda"),
+           "strided": torch.zeros(2 * size, device="cuda")[::2], "type": torch.zeros(size, dtype=torch.float64, device="cuda")}
+    opt = AdamW(ps, copies=[None, bad.get(fault), None])
+    if fault == "moment":
+        opt.v[1] = torch.zeros(size + 8, device="cuda")
+    elif fault == "late":  # the last of three, behind one that steps alone
+        opt.copies[2] = torch.zeros(23, device="cuda")
+    with pytest.raises(ValueError, match="moments must have" if fault == "moment" else "a copy must be"):
+        opt.step()
+    torch.cuda.synchronize()
+    assert opt.t == 0 and all((p == x).all() for p, x in zip(ps, (2.0, 1.0, 3.0)))
+    assert all((m == 0).all() for m in opt.m) and all((v == 0).all() for v in opt.v)
+    if fault != "moment":
+        assert all(c is None or (c == 0).all() for c in opt.copies)
+        opt.copies = [None] * 3
+        opt.step()
+        assert opt.t == 1 and all((p < x).all() for p, x in zip(ps, (2.0, 1.0, 3.0)))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_list_changes_nothing(bits):
+    """A tensor that is listed twice makes two launches: the second one's checks come before the first one too."""
+    from nimbleml_b200.embedding_grad import adamw_step_many, quantize_moment
+
+    p = torch.ones(130, device="cuda")
+    z = torch.zeros(130, device="cuda")
+    m = [quantize_moment(z) if bits == 8 else z.clone() for _ in range(6)]
+    g = torch.full((130,), 0.5, device="cuda")
+    with pytest.raises(ValueError, match="elements"):
+        adamw_step_many([p, p, p], [g, g, g[:100]], m[:3], m[3:], step=1)
+    torch.cuda.synchronize()
+    assert (p == 1).all()

@@ -166,3 +166,15 @@ def test_native_adamw_many_arguments():
     _fails(-1, "nimble_adamw_dequantize", None, p, 4, 0, p, None)
     _fails(-1, "nimble_adamw_quantize", p, -1, 0, p, p, None)
     native.call("nimble_adamw_dequantize", None, None, 0, 0, None, None)
+
+
+def test_adamw_copies_match_the_weights():
+    with pytest.raises(ValueError, match="one entry per tensor: 1 for 2"):
+        AdamW([torch.zeros(3), torch.zeros(8)], copies=[None])
+    # A refused step (these weights are on the CPU) does not count.
+    opt = AdamW([torch.zeros(3), torch.zeros(16)], copies=[None, None])
+    for p in opt.params:
+        p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="CUDA"):
+        opt.step()
+    assert opt.t == 0
