@@ -7,11 +7,14 @@
 // needs. Errors are Python's: ValueError for arguments, RuntimeError with the
 // library's message for a failing call.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -52,6 +55,24 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_
 
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) {
   return at::empty(shape, like.options().dtype(type).memory_format(c10::nullopt).requires_grad(false));
+}
+
+// These operators write through raw pointers, which neither a trace nor a tangent
+// follows: a trace would keep the allocation of the results and none of the kernels,
+// and a dual tensor (which does not require grad) would come out without its tangent.
+void refuse_recording(const char* name) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+              name, " cannot be traced: the trace would not hold its kernels");
+}
+void refuse_tangent(const char* name, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
+                              " has no forward-mode derivative, and an input has a tangent");
+}
+void refuse_transforms(const std::string& name, const Tensor& a, const std::optional<Tensor>& b) {
+  refuse_recording(name.c_str());
+  refuse_tangent(name.c_str(), a);
+  if (b) refuse_tangent(name.c_str(), *b);
 }
 
 // t in a type, contiguous; t itself, without a call to torch, where it is both.
@@ -145,6 +166,10 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 };
 
 Tensor layer_norm(const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta, double eps) {
+  refuse_recording("layer_norm");
+  refuse_tangent("layer_norm", x);
+  refuse_tangent("layer_norm", gamma);
+  if (beta) refuse_tangent("layer_norm", *beta);
   TORCH_CHECK(x.is_cuda(), "layer_norm on B200 needs CUDA tensors; there is no CPU path");
   dtype_of(x);
   const int64_t d = x.dim() ? x.size(-1) : 0;
@@ -450,6 +475,7 @@ void check_quantized(const Tensor& codes, const Tensor& scales) {
 void adamw_step_many(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_,
                      const py::object& copies_, int64_t step, double lr, double beta1, double beta2, double eps,
                      double wd, bool own_steps) {
+  refuse_recording("adamw_step_many");
   const Items params(params_), grads(grads_), ms(m_), vs(v_);
   std::optional<Items> copies;
   if (!copies_.is_none()) copies.emplace(copies_);
@@ -466,6 +492,8 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
     if (grads.at[i] == Py_None) continue;
     const Tensor& p = tensor_in(params.at[i], "a parameter");
     const Tensor* g = &tensor_in(grads.at[i], "a gradient");
+    refuse_tangent("adamw_step_many", p);
+    refuse_tangent("adamw_step_many", *g);
     if (!dev) {
       dev = p.device();
       TORCH_CHECK_VALUE(p.is_cuda(), "adamw_step_many needs CUDA tensors; there is no CPU path");
@@ -566,6 +594,7 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
 
 PYBIND11_MODULE(nimbleml_b200_host, m) {
   m.doc() = "Host side of layer_norm, the token log probabilities and adamw_step_many over the C ABI";
+  m.def("refuse_transforms", &refuse_transforms, py::arg("name"), py::arg("a"), py::arg("b") = std::nullopt);
   m.def("layer_norm", &layer_norm);
   m.def("token_logprobs", &token_logprobs);
   m.def("set_status_hooks", &set_status_hooks);

@@ -16,6 +16,7 @@ terms of every token instead:
 
 Both are differentiable in the log probabilities and in the entropies:
 d/dx_j (a logp_t + b H) = a [j = t] - p_j (a + b (H + log p_j)).
+Reverse mode only, once; inputs with a tangent and calls under a tracer raise.
 """
 from __future__ import annotations
 
@@ -102,6 +103,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     A token outside the classes gives a NaN log probability and sets the
     status word's bad-label bit.
     """
+    host.refuse_transforms("token_logprobs", logits)
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs on B200 needs CUDA tensors; there is no CPU path")
     compute_dtype_of(logits)
@@ -250,6 +252,7 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
     The gradient of the logits is formed in the compute dtype, so gradients
     carry one 16-bit rounding more than their own.
     """
+    host.refuse_transforms("tied_token_logprobs", hidden, weights)
     if not hidden.is_cuda:
         raise RuntimeError("tied_token_logprobs on B200 needs CUDA tensors; there is no CPU path")
     if hidden.dtype not in (torch.float16, torch.bfloat16):

@@ -95,7 +95,8 @@ def layer_norm(x: torch.Tensor, gamma: torch.Tensor, beta=None, eps: float = 1e-
     ``x`` is float32, float16 or bfloat16; ``gamma`` and ``beta`` (None: no
     bias) have the last dimension's size and any of these dtypes. Statistics
     are fp32, the variance is the biased one of centred values. The gradients
-    of ``gamma`` and ``beta`` are summed in a fixed order.
+    of ``gamma`` and ``beta`` are summed in a fixed order. Reverse mode only,
+    once; inputs with a tangent and calls under a tracer raise.
     """
     return host.layer_norm(x, gamma, beta, float(eps))
 

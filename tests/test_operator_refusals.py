@@ -178,3 +178,57 @@ def test_adamw_copies_match_the_weights():
     with pytest.raises(ValueError, match="CUDA"):
         opt.step()
     assert opt.t == 0
+
+
+def test_tracing_and_forward_mode_are_refused():
+    """The kernels write through raw pointers: a trace would hold none of them, and a tangent would be lost."""
+    refuse_tracing_and_forward_mode("cpu")
+
+
+def refuse_tracing_and_forward_mode(device):
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def t(*shape, dtype=torch.float32):
+        return torch.ones(shape, dtype=dtype, device=device)
+
+    ids = torch.zeros(2, dtype=torch.int64, device=device)
+    w = t(5, 16, dtype=torch.float16)
+    codes = torch.zeros(16, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+
+    def step(p):
+        adamw_step_many([p], [t(2, 16)], [t(2, 16)], [t(2, 16)], step=1)
+        return p
+
+    def step_grad(g):
+        adamw_step_many([t(2, 16)], [g], [t(2, 16)], [t(2, 16)], step=1)
+        return g
+
+    calls = {
+        "layer_norm": (lambda x: layer_norm(x, t(16)), t(2, 16)),
+        "layer_norm ": (lambda g: layer_norm(t(2, 16), g), t(16)),
+        "layer_norm  ": (lambda b: layer_norm(t(2, 16), t(16), b), t(16)),
+        "layer_norm   ": (LayerNorm(16, device=device), t(2, 16)),
+        "token_logprobs": (lambda x: token_logprobs(x, ids).logprobs, t(2, 16)),
+        "tied_token_logprobs": (lambda h: tied_token_logprobs(h, w, ids).logprobs, t(2, 16, dtype=torch.float16)),
+        "tied_token_logprobs ": (lambda e: tied_token_logprobs(t(2, 16, dtype=torch.float16), e, ids).entropy, w),
+        "tied_token_logprobs  ": (lambda h: tied_token_logprobs(h, w, ids, vocab_size=9).logprobs,
+                                  t(2, 16, dtype=torch.float16)),
+        "adamw_step_many": (step, t(2, 16)),
+        "adamw_step_many ": (step_grad, t(2, 16)),
+        "quantize_moment": (lambda x: quantize_moment(x).scales, t(16)),
+        "dequantize_moment": (lambda s: dequantize_moment(codes, s), t(1)),
+    }
+    for name, (call, x) in calls.items():
+        name = name.strip()
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(RuntimeError, match=f"{name} cannot be traced"):
+            make_fx(call)(x)
+        with fw.dual_level():
+            dual = fw.make_dual(x, torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match=f"{name} has no forward-mode derivative"):
+                call(dual)
+            if not name.startswith("adamw"):  # the same where a node would be built
+                with pytest.raises(NotImplementedError, match=f"{name} has no forward-mode derivative"):
+                    call(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)))

@@ -79,3 +79,22 @@ def test_policy_step(dtype):
         top = token_logprobs(logits, tokens[:, 0], top_k=5)
     want_ids = torch.sort(logits.double(), dim=1, descending=True, stable=True).indices[:, :5]
     assert top.top_ids.equal(want_ids)
+
+
+def test_tracing_and_forward_mode_are_refused_on_the_gpu():
+    from test_operator_refusals import refuse_tracing_and_forward_mode
+
+    refuse_tracing_and_forward_mode("cuda")
+    # A level without tangents, and tangents that are switched off, refuse nothing.
+    import torch.autograd.forward_ad as fw
+
+    from nimbleml_b200.norm import layer_norm
+
+    x, g = torch.randn(3, 64, device="cuda"), torch.ones(64, device="cuda")
+    want = layer_norm(x, g)
+    with fw.dual_level():
+        assert layer_norm(x, g).equal(want)
+        dual = fw.make_dual(x, torch.ones_like(x))
+        with fw._set_fwd_grad_enabled(False):
+            assert layer_norm(dual, g).equal(want)
+        assert layer_norm(fw.unpack_dual(dual).primal, g).equal(want)
