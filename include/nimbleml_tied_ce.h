@@ -392,11 +392,12 @@ NIMBLE_API int nimble_tied_logprobs_backward_workspace_size(int64_t n_tokens, in
 
 /* Backward on one vocab shard: recomputes the logits slab by slab, forms the
  * gradient of nimble_token_logprobs_backward in the compute dtype (fp16: times
- * a power of two chosen from the largest row coefficient, undone in fp32) and
+ * a power of two chosen from the largest row coefficient, and one more for rows
+ * far below it, undone in the results) and
  * computes grad_hidden (this shard's partial) and grad_weights as
  * nimble_tied_ce_backward does. A null grad_hidden or grad_weights is not
  * computed. hidden rows of ignored tokens must be finite: they are multiplied
- * by zero gradients. */
+ * by zero gradients. hidden and the workspace start on 16-byte boundaries. */
 NIMBLE_API int nimble_tied_logprobs_backward(const float* grad_logprob, const float* grad_entropy,
                                              const void* hidden, const void* weights, const int64_t* tokens,
                                              const float* lse, const float* entropy, int64_t n_tokens,

@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -105,6 +106,7 @@ struct EpiParams {
   const float* alpha_num;  // device scalar or null (1)
   const float* alpha_den;  // device scalar or null (1); alpha = 0 when *den == 0
   float alpha_mult;
+  const float* row_mult;   // [M] factors of the result's rows beside alpha, or null (1)
   int accum_out;
   int* status;
   // Split contraction (kSplit): the tiles' K blocks are cut into k_splits runs,
@@ -555,6 +557,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       } else {  // EPI_STORE (split: fp32 out)
         const int64_t split_at = kSplit ? t / plane * ep.split_stride : 0;
         const bool no_run = kSplit && k_begin(t) == k_end(t);  // nothing was accumulated
+        const float alpha_row = ep.row_mult && row_ok ? alpha * ep.row_mult[row] : alpha;
 #pragma unroll 1
         for (int c = c_begin; c < c_end; ++c) {
           if (c * 32 >= ncols) break;
@@ -579,7 +582,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
               }
             }
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] *= alpha;
+            for (int j = 0; j < 32; ++j) v[j] *= alpha_row;
             if (ep.out_dtype == NIMBLE_DTYPE_F32) {
               float4* o4 = reinterpret_cast<float4*>(static_cast<float*>(ep.out) + split_at + row * ep.ld_out + col);
 #pragma unroll
@@ -630,7 +633,7 @@ tc_gemm_tn_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
               if (j >= nv) break;
               float x = v[j];
               if (ep.src) x += ep.src[split_at + row * ep.ld_src + col + j];
-              x *= alpha;
+              x *= alpha_row;
               const int64_t oi = split_at + row * ep.ld_out + col + j;
               if (ep.accum_out) x += load_out_elem(ep.out, oi, ep.out_dtype);
               store_out_elem(ep.out, oi, ep.out_dtype, x);
@@ -1240,14 +1243,17 @@ namespace {
 // (base parameters `eg`) recomputes a slab's logits and writes its G, then two
 // GEMMs add the slab's share of grad_hidden and write its grad_weights rows, both
 // times alpha = alpha_num / alpha_den * alpha_mult (device scalars, null = 1).
-// A null grad_hidden or grad_weights leaves that GEMM out.
+// A null grad_hidden or grad_weights leaves that GEMM out. Where G's rows have factors
+// of their own, `row_mult` takes them back from grad_hidden's rows, and `h_de`, the
+// hidden rows times the same, stands for h in the product that sums over rows.
 template <int EPI>
 int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, const float* alpha_num,
                   const float* alpha_den, float alpha_mult, const void* h, const void* E, int64_t n_tokens,
                   int64_t d_model, int64_t v_local, int64_t v_offset, int dtype, void* grad_hidden,
                   int grad_hidden_dtype, void* grad_weights, int grad_weights_dtype, int accumulate_grad_weights,
                   int* status, cudaStream_t s, void* dh_done_event, int last_de_max_ctas, float capped_fraction,
-                  int splits = 1) {
+                  int splits = 1, const float* row_mult = nullptr, const void* h_de = nullptr) {
+  if (!h_de) h_de = h;
   const int64_t es = elem_size(dtype);
   void* g = ws + L.g;
   float* dh_acc = L.n_slabs > 1 || splits > 1 ? reinterpret_cast<float*>(ws + L.dh) : nullptr;
@@ -1280,10 +1286,10 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
       if (EPI == EPI_LP_GRAD && grad_weights_dtype == dtype && !accumulate_grad_weights) {
         ee.g = ee.out;
         ee.ldg = d_model;
-        return gemm_dispatch<EPI_LP_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
+        return gemm_dispatch<EPI_LP_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h_de, d_model,
                                                        r1 - r0, d_model, n_tokens, ee, s, max_ctas);
       }
-      return gemm_dispatch<EPI_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h, d_model,
+      return gemm_dispatch<EPI_STORE, true, true>(dtype, static_cast<uint8_t*>(g) + es * r0, L.slab, h_de, d_model,
                                                   r1 - r0, d_model, n_tokens, ee, s, max_ctas);
     };
     // 3) dh (+)= G E[c0:c0+vc]: A = G K-major, B = E slab read MN-major
@@ -1311,6 +1317,7 @@ int slab_backward(const BwdLayout& L, uint8_t* ws, const EpiParams& eg_base, con
         eh.alpha_num = alpha_num;
         eh.alpha_den = alpha_den;
         eh.alpha_mult = alpha_mult;
+        eh.row_mult = row_mult;
       } else {
         eh.out = dh_acc;
         eh.out_dtype = NIMBLE_DTYPE_F32;
@@ -1864,13 +1871,16 @@ int launch_decode(const void* hidden, const void* weights, const int64_t* tokens
   return NIMBLE_OK;
 }
 
-// out = alpha * (sum over runs of partial[run]), eight elements a thread.
+// out = alpha * row_mult (null: 1) * (sum over runs of partial[run]), eight elements a
+// thread, d8 eights a row.
 template <typename O>
-__global__ void split_sum_kernel(const float* __restrict__ partial, int runs, int64_t stride, int64_t n8,
-                                 const float* __restrict__ alpha, O* __restrict__ out) {
-  const float a = *alpha;
+__global__ void split_sum_kernel(const float* __restrict__ partial, int runs, int64_t stride, int64_t n8, int64_t d8,
+                                 const float* __restrict__ alpha, const float* __restrict__ row_mult,
+                                 O* __restrict__ out) {
+  const float alpha1 = *alpha;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < n8;
        i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const float a = row_mult ? alpha1 * row_mult[i / d8] : alpha1;
     float v[8];
     load8<float>(partial + 8 * i, v);
     constexpr int kU = 4;  // runs in flight; those behind the last are read again and not added
@@ -1889,49 +1899,97 @@ __global__ void split_sum_kernel(const float* __restrict__ partial, int runs, in
   }
 }
 
-// Row coefficients of the gradient epilogue, scaled by a power of two that
-// fp16 G needs: |G_ij| <= |a_i| + |b_i| (H_i + 1/e), and the largest such bound
-// is brought to (2^14, 2^15], so that probabilities of order 1/V stay normal
-// numbers whatever the upstream gradients' size. bf16 has fp32's exponents and
-// is not scaled. scale[0] = 1 / factor goes to the dE / dh epilogues. One block.
+// Row coefficients of the gradient epilogue, (lse log2 e, a, a + b H, b ln 2) with a and b
+// times a power of two that fp16 G needs; bf16 has fp32's exponents and takes them as they
+// are. With the bound |G_ij| <= B_i = |a_i| + |b_i| (H_i + 1/e), one factor 2^f brings the
+// largest finite bound to (2^14, 2^15], so that probabilities of order 1/V stay normal
+// numbers whatever the upstream gradients' size. A row whose bound is more than 2^8 below
+// the largest is raised to that distance by a factor 2^k of its own: by 2^f alone an upstream
+// gradient 10^6 times the others' left those rows' softmax parts in fp16's last subnormal
+// steps (grad_hidden off by 70% of that part; now by its roundings). scale[0] = 2^-f goes to
+// the dE / dh epilogues. 2^-k goes to grad_hidden's rows (row_mult) and, for dE, which sums
+// over rows, to a copy of the hidden rows (h_de): exact until hidden 2^-k is subnormal,
+// which elements of order one become 2^22 below the largest row. Rows within 2^8, as
+// nearly all are in training, have k = 0 and the bits that one factor gives them. The block
+// of a row takes the largest bound of all rows itself, which is little beside a launch more.
 constexpr int kPrepThreads = 1024;
+constexpr int kNearTop = 8;                     // log2 of a bound's distance that needs no factor of its own
+// Limits of f and f + k, and of k: normal numbers, with normal reciprocals.
+constexpr int kMinFactor = -113, kMaxFactor = 120, kMaxRaise = 126;
+template <bool kScaled>
 __global__ void __launch_bounds__(kPrepThreads)
 lp_row_prep_kernel(const float* __restrict__ g_logp, const float* __restrict__ g_ent, const float* __restrict__ lse,
                    const float* __restrict__ entropy, const int64_t* __restrict__ tokens, int64_t M, int64_t V,
-                   int64_t ignore_index, bool scaled, float4* __restrict__ rowp, float* __restrict__ scale) {
+                   int64_t ignore_index, int64_t rows_per_block, const __half* __restrict__ h, int64_t d,
+                   float4* __restrict__ rowp, float* __restrict__ scale, float* __restrict__ row_mult,
+                   __half* __restrict__ h_de) {
   __shared__ float red[kPrepThreads / 32];
   auto is_live = [&](int64_t i) {
     const int64_t t = tokens[i];
     return t != ignore_index && t >= 0 && t < V;
   };
-  float factor = 1.0f;
-  if (scaled) {
+  auto bound = [&](int64_t i) {
+    return (g_logp ? fabsf(g_logp[i]) : 0.0f) + (g_ent ? fabsf(g_ent[i]) * (entropy[i] + 0.37f) : 0.0f);
+  };
+  int f = 0, e_top = 0;
+  if constexpr (kScaled) {
     float top = 0.0f;
     for (int64_t i = threadIdx.x; i < M; i += kPrepThreads)
-      if (is_live(i))
-        top = fmaxf(top, (g_logp ? fabsf(g_logp[i]) : 0.0f) + (g_ent ? fabsf(g_ent[i]) * (entropy[i] + 0.37f) : 0.0f));
+      if (is_live(i)) {
+        const float b = bound(i);
+        if (b <= FLT_MAX) top = fmaxf(top, b);  // infinite and NaN rows are spoilt, the others not
+      }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
     __syncthreads();
     for (int w = 0; w < kPrepThreads / 32; ++w) top = fmaxf(top, red[w]);
-    // 2^-100 < top < 2^100, else (all zero, infinite, NaN) no scale.
-    if (top > 7.9e-31f && top < 1.2e30f) {
-      int e;
-      frexpf(top, &e);  // top in [2^(e-1), 2^e)
-      factor = ldexpf(1.0f, 15 - e);
+    if (top > 0.0f) {
+      frexpf(top, &e_top);  // top in [2^(e-1), 2^e)
+      f = max(kMinFactor, min(kMaxFactor, 15 - e_top));
     }
   }
-  if (threadIdx.x == 0) scale[0] = 1.0f / factor;
-  for (int64_t i = threadIdx.x; i < M; i += kPrepThreads) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = ldexpf(1.0f, -f);
+  const int64_t lo = blockIdx.x * rows_per_block, hi = min(M, lo + rows_per_block);
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kPrepThreads) {
     float4 p = make_float4(1.0e30f, 0.0f, 0.0f, 0.0f);  // p = 2^-1e30 = 0
+    int k = 0;
     if (is_live(i)) {
+      if constexpr (kScaled) {
+        const float own = bound(i);
+        if (own > 0.0f && own <= FLT_MAX) {
+          int e;
+          frexpf(own, &e);
+          k = max(0, min(min(e_top - e - kNearTop, kMaxRaise), kMaxFactor - f));
+        }
+      }
+      const float factor = ldexpf(1.0f, f + k);
       const float a = g_logp ? g_logp[i] * factor : 0.0f;
       const float b = g_ent ? g_ent[i] * factor : 0.0f;
       p = make_float4(lse[i] * kLog2e, a, fmaf(b, entropy[i], a), b * 0.6931471805599453f);
     }
     rowp[i] = p;
+    if constexpr (kScaled) row_mult[i] = ldexpf(1.0f, -k);
   }
+  if constexpr (kScaled) {
+    if (!h_de) return;
+    __syncthreads();  // this block's factors
+    const int64_t d8 = d / 8;  // d is a multiple of 8, the rows start on 16-byte boundaries
+    for (int64_t q = lo * d8 + threadIdx.x; q < hi * d8; q += kPrepThreads) {
+      const float r = row_mult[q / d8];
+      float v[8];
+      load8<__half>(h + 8 * q, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= r;
+      store8<__half>(h_de + 8 * q, v);
+    }
+  }
+}
+// Blocks for the rows: one where there is nothing but their coefficients to write (or few
+// hidden elements), else a row or more and 16 K elements each.
+int64_t prep_rows_per_block(int64_t M, int64_t d, bool copies) {
+  if (!copies) return M;
+  return std::max<int64_t>((M + 147) / 148, (16384 + d - 1) / d);
 }
 
 int check_half(int dtype) {
@@ -1963,7 +2021,7 @@ constexpr int64_t kOneSlabBytes = 256 << 20;
 struct LpBwdLayout {
   BwdLayout slabs;
   int splits = 1;
-  size_t rowp = 0, scale = 0, total = 0;
+  size_t rowp = 0, scale = 0, row_mult = 0, h_de = 0, total = 0;
 };
 LpBwdLayout lp_bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t slab_bytes) {
   LpBwdLayout L;
@@ -1978,6 +2036,10 @@ LpBwdLayout lp_bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t sla
   }
   L.rowp = off; off = align_up(off + sizeof(float4) * N);
   L.scale = off; off = align_up(off + sizeof(float));
+  if (dtype == NIMBLE_DTYPE_F16) {  // rows with factors of their own
+    L.row_mult = off; off = align_up(off + sizeof(float) * N);
+    L.h_de = off; off = align_up(off + sizeof(__half) * N * d);
+  }
   L.total = off;
   return L;
 }
@@ -2067,6 +2129,9 @@ extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const fl
     return fail(NIMBLE_ERR_INVALID_ARG, "gradient outputs must be 16-byte aligned");
   if ((d_model * elem_size(grad_hidden_dtype)) % 16 || (d_model * elem_size(grad_weights_dtype)) % 16)
     return fail(NIMBLE_ERR_INVALID_ARG, "d_model * output element size must be a multiple of 16 bytes");
+  // The row kernels read and write 16 bytes at a time before a tensor map is encoded.
+  if ((reinterpret_cast<uintptr_t>(hidden) & 15) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(NIMBLE_ERR_INVALID_ARG, "hidden and the workspace must be 16-byte aligned");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (n_tokens == 0) {
     if (grad_weights && !accumulate_grad_weights)
@@ -2080,8 +2145,14 @@ extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const fl
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   float4* rowp = reinterpret_cast<float4*>(ws + L.rowp);
   float* scale = reinterpret_cast<float*>(ws + L.scale);
-  lp_row_prep_kernel<<<1, kPrepThreads, 0, s>>>(grad_logprob, grad_entropy, lse, entropy, tokens, n_tokens, vocab_size,
-                                                ignore_index, dtype == NIMBLE_DTYPE_F16, rowp, scale);
+  const bool scaled = dtype == NIMBLE_DTYPE_F16;
+  float* row_mult = scaled ? reinterpret_cast<float*>(ws + L.row_mult) : nullptr;
+  __half* h_de = scaled && grad_weights ? reinterpret_cast<__half*>(ws + L.h_de) : nullptr;
+  const int64_t per = prep_rows_per_block(n_tokens, d_model, h_de != nullptr);
+  auto prep = scaled ? lp_row_prep_kernel<true> : lp_row_prep_kernel<false>;
+  prep<<<static_cast<unsigned>((n_tokens + per - 1) / per), kPrepThreads, 0, s>>>(
+      grad_logprob, grad_entropy, lse, entropy, tokens, n_tokens, vocab_size, ignore_index, per,
+      static_cast<const __half*>(hidden), d_model, rowp, scale, row_mult, h_de);
   NIMBLE_CUDA_TRY(cudaGetLastError());
   EpiParams eg{};
   eg.labels = tokens;
@@ -2092,14 +2163,14 @@ extern "C" int nimble_tied_logprobs_backward(const float* grad_logprob, const fl
   if (int rc = slab_backward<EPI_LP_GRAD>(L.slabs, ws, eg, scale, nullptr, 1.0f, hidden, weights, n_tokens, d_model,
                                           v_local, v_offset, dtype, grad_hidden, grad_hidden_dtype, grad_weights,
                                           grad_weights_dtype, accumulate_grad_weights, status, s, nullptr, 0, 1.0f,
-                                          L.splits))
+                                          L.splits, row_mult, h_de))
     return rc;
   if (grad_hidden && L.splits > 1) {
     const float* partial = reinterpret_cast<const float*>(ws + L.slabs.dh);
     const int64_t n = n_tokens * d_model, n8 = n / 8;  // d_model is a multiple of 8
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n8 + 255) / 256, 148 * 8));
     NIMBLE_DISPATCH(grad_hidden_dtype, O,
-                    split_sum_kernel<O><<<grid, 256, 0, s>>>(partial, L.splits, n, n8, scale,
+                    split_sum_kernel<O><<<grid, 256, 0, s>>>(partial, L.splits, n, n8, d_model / 8, scale, row_mult,
                                                              static_cast<O*>(grad_hidden)));
     NIMBLE_CUDA_TRY(cudaGetLastError());
   }

@@ -232,3 +232,11 @@ def refuse_tracing_and_forward_mode(device):
             if not name.startswith("adamw"):  # the same where a node would be built
                 with pytest.raises(NotImplementedError, match=f"{name} has no forward-mode derivative"):
                     call(fw.make_dual(x.clone().requires_grad_(), torch.ones_like(x)))
+
+
+def test_native_tied_logprobs_backward_alignment():
+    """The row kernels use 16-byte accesses: what does not allow them is refused before any launch."""
+    p = 1 << 20
+    for h, ws in ((p + 2, p), (p + 8, p), (p, p + 8)):
+        _fails(-1, "nimble_tied_logprobs_backward", p, p, h, p, p, p, p, 4, 8, 100, 0, 100, -1, DTYPE_F16, p, DTYPE_F16, p,
+               DTYPE_F16, 0, 0, ws, 1 << 30, None, None)

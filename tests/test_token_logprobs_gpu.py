@@ -744,3 +744,99 @@ def test_first_call_in_a_capture_is_refused():
     run = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parents[1])
     assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
+
+
+def check_each_row(gh, gw, h, w, tokens, a, b):
+    """As check_tied_grads, but every row of grad_hidden against its own size: whatever the other rows' upstream
+    gradients are, a row's bound B_i = |a| + |b| (H + 1/e) is brought to 2^6 or more in fp16, whose smallest half step is 2^-25:
+    2^-31 B_i an element of G. In dE a row that was raised by 2^k meets hidden 2^-k, off by half a smallest step, 2^-25."""
+    x = h.double() @ w.double().t()
+    _, ent, p, logq, d = exact_rows(x, tokens)
+    live = (tokens != IGN).unsqueeze(1)
+    a, b = a.double().unsqueeze(1), b.double().unsqueeze(1)
+    zero = torch.zeros_like(p)
+    onehot = zero.scatter(1, tokens.clamp(min=0).unsqueeze(1), 1.0)
+    t_ls, t_h = (t.unsqueeze(1) for t in row_bounds(p, d, ent))
+    ent = ent.unsqueeze(1)
+    big_g = torch.where(live, a * onehot - p * (a + b * (ent + logq)), zero)
+    mag = logit_error(h, w).unsqueeze(1) + 2.0**-22 * x.abs().amax(1, keepdim=True)
+    e_lp = t_ls + 4 * mag + 2.0**-22 * (d.abs() + logq.abs())
+    spread = (p * (logq.abs() + ent)).sum(1, keepdim=True)
+    slack = p * ((a.abs() + b.abs() * (ent + logq.abs())) * (e_lp + 2.0**-21) + b.abs() * (t_h + 2 * mag * (1 + spread) + e_lp))
+    bound = torch.where(live, a.abs() + b.abs() * (ent + 0.37), zero[:, :1])
+    under = 2.0**-31 * bound * (1 + 2.0**-10) if h.dtype == torch.float16 else 0.0
+    err = torch.where(live, half_step(h.dtype) * big_g.abs() + (1 + 2.0**-6) * slack + under + 2.0**-22 * a.abs() * onehot, zero)
+    top = float(bound.max())
+    raised = torch.where(bound > 0, (top / bound.clamp(min=2.0**-140)).clamp(min=1.0) * 2.0**-7, zero[:, :1])  # 2^k at most
+    e_h = 2.0**-25 * torch.where(raised > 1, raised, zero[:, :1]) if h.dtype == torch.float16 else zero[:, :1]
+    for got, want, tol in (
+            (gh, big_g @ w.double(), err @ w.double().abs() + (p.shape[1] + 16) * 2.0**-23 * (big_g.abs() @ w.double().abs())),
+            (gw, big_g.t() @ h.double(), err.t() @ h.double().abs() + (big_g.abs() + err).t() @ e_h.expand(h.shape) +
+             (h.shape[0] + 16) * 2.0**-23 * (big_g.t().abs() @ h.double().abs()))):
+        fin = torch.finfo(got.dtype)
+        tol = tol + half_step(got.dtype) * want.abs()
+        off = (got.double() - want).abs()
+        assert (off <= tol * (1 + 2.0**-6) + fin.smallest_normal * fin.eps).all(), float((off / (tol + 1e-300)).max())
+
+
+# (tokens, d, vocabulary): the split grad_hidden product, one run of it, several slabs, ragged edges.
+UNEVEN = [(64, 64, 20011), (5, 72, 300), (40, 64, 1500), (260, 320, 6000)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape", UNEVEN)
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e9, 1e30])
+def test_tied_rows_beside_a_large_one(dtype, shape, ratio, monkeypatch):
+    """One upstream gradient far above the others leaves the others' gradients their precision."""
+    import nimbleml_b200.losses.logprobs as mod
+
+    n, d, v = shape
+    if n == 40:
+        monkeypatch.setattr(mod, "SLAB_BYTES", 1)  # 256 columns a slab
+    h, w, tokens, g = make_tied(n, d, v, dtype, n + d)
+    a, b = torch.randn(n, generator=g).cuda(), 0.1 * torch.randn(n, generator=g).cuda()
+    # Sizes from the largest down; the results are fp32 or scaled so that fp16 holds them.
+    size = 1.0 / ratio if dtype == torch.float16 else 1.0
+    a, b = a * size, b * size
+    a[n // 2] = size * ratio
+    if ratio == 1e6:  # every size between
+        a = a * torch.logspace(0, 6, n, device="cuda")
+        a[n // 2] = size * ratio
+    tokens[1] = IGN
+    h32 = h.float().to(dtype).requires_grad_()
+    w32 = w.float().requires_grad_()
+    r = mod.tied_token_logprobs(h32, w32, tokens, IGN)
+    gh, gw = torch.autograd.grad((r.logprobs, r.entropy), (h32, w32), (a, b))
+    gh32 = torch.empty(n, d, device="cuda")  # the same in fp32, as the shards' partial sums are kept
+    gw32 = torch.empty(v, d, device="cuda")
+    lse = torch.logsumexp(h.double() @ w.double().t(), 1).float()
+    mod.shard_logprob_backward(a, b, h, w, tokens, lse, r.entropy.detach(), ignore_index=IGN, grad_hidden=gh32,
+                               grad_weights=gw32)
+    check_each_row(gh, gw, h, w, tokens, a, b)
+    check_each_row(gh32, gw32, h, w, tokens, a, b)
+    assert (gh[1] == 0).all() and (gh32[1] == 0).all()
+
+
+@pytest.mark.parametrize("spoilt", [float("inf"), float("nan")])
+def test_tied_rows_beside_a_spoilt_one(spoilt):
+    """An infinite or NaN upstream gradient spoils its own row of grad_hidden; the others keep their precision."""
+    from nimbleml_b200.losses import tied_token_logprobs
+
+    h, w, tokens, g = make_tied(50, 64, 9000, torch.float16, 4)
+    a, b = 1e-3 * torch.randn(50, generator=g).cuda(), 1e-4 * torch.randn(50, generator=g).cuda()
+    keep = torch.arange(50, device="cuda") != 7
+    for x in (a, b):
+        bad = x.clone()
+        bad[7] = spoilt
+        up = (bad, b) if x is a else (a, bad)
+        hl = h.detach().requires_grad_()
+        r = tied_token_logprobs(hl, w, tokens)
+        (gh,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), up)
+        assert not torch.isfinite(gh[7]).all() and torch.isfinite(gh[keep]).all()
+        # The others as without it, in bits (their largest row sets the factor).
+        none = tokens.clone()
+        none[7] = IGN
+        hl = h.detach().requires_grad_()
+        r = tied_token_logprobs(hl, w, none, IGN)
+        (want,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), (a, b))
+        assert gh[keep].equal(want[keep])
