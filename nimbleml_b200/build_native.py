@@ -8,8 +8,9 @@ loads on hosts without a GPU. Run ``python -m nimbleml_b200.build_native``.
 The same step builds ``_lib/nimbleml_tied_ce_native*.so``, the pybind11
 module with the reference-style ``*_device`` entry points
 (``csrc/tied_ce_pybind.cpp``), linked against the library with an
-``$ORIGIN`` run path, and ``_lib/nimbleml_b200_host*.so``, the torch host side of
-the operators whose calls are short (``csrc/torch_host.cpp``).
+``$ORIGIN`` run path, and ``_lib/nimbleml_b200_host.torch-<version>*.so``, the
+torch host side of the operators whose calls are short (``csrc/torch_host.cpp``),
+one file for each torch version.
 """
 from __future__ import annotations
 
@@ -53,8 +54,12 @@ def pybind_module_path() -> Path:
 
 
 def host_module_path() -> Path:
+    """The host module of the installed torch: it is compiled against torch's headers, so one that was built
+    with another version is not this one (it is neither loaded nor taken for up to date)."""
+    import torch
+
     ext = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
-    return LIB_DIR / f"nimbleml_b200_host{ext}"
+    return LIB_DIR / f"nimbleml_b200_host.torch-{torch.__version__}{ext}"
 
 
 def _stale(target: Path, deps) -> bool:
@@ -83,7 +88,8 @@ def build_pybind(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the torch host module (g++ against the installed torch) if it is older than its source or the library."""
+    """Compile the torch host module (g++ against the installed torch) if there is none for this torch, or one older
+    than its source or the library."""
     out = host_module_path()
     if not force and not _stale(out, [HOST_SOURCE, LIB_PATH, HEADERS[-1]]):
         return out

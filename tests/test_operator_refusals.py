@@ -240,3 +240,17 @@ def test_native_tied_logprobs_backward_alignment():
     for h, ws in ((p + 2, p), (p + 8, p), (p, p + 8)):
         _fails(-1, "nimble_tied_logprobs_backward", p, p, h, p, p, p, p, 4, 8, 100, 0, 100, -1, DTYPE_F16, p, DTYPE_F16, p,
                DTYPE_F16, 0, 0, ws, 1 << 30, None, None)
+
+
+def test_host_module_of_another_torch(monkeypatch):
+    """After a torch upgrade the module that the old one was built with is neither loaded nor up to date."""
+    from nimbleml_b200 import build_native
+    from nimbleml_b200._host import load_host
+
+    here = build_native.host_module_path()
+    assert here.exists() and not build_native._stale(here, [build_native.HOST_SOURCE, build_native.LIB_PATH])
+    monkeypatch.setattr(torch, "__version__", "99.0.0+cu999")
+    other = build_native.host_module_path()
+    assert other != here and build_native._stale(other, [build_native.HOST_SOURCE])
+    with pytest.raises(ImportError, match="build_native"):
+        load_host()
