@@ -118,7 +118,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     ids = _token_ids(tokens, math.prod(shape[:-1]), dev)
     ign = _NO_IGNORE if ignore_index is None else int(ignore_index)
     out = TokenLogProbs(*host.token_logprobs(logits, ids, ign, top_k, _status_ptr(dev)))
-    if CHECK_BOUNDS:
+    if CHECK_BOUNDS and not torch.cuda.is_current_stream_capturing():
         check_status(dev)
     return out
 

@@ -840,3 +840,21 @@ def test_tied_rows_beside_a_spoilt_one(spoilt):
         r = tied_token_logprobs(hl, w, none, IGN)
         (want,) = torch.autograd.grad((r.logprobs, r.entropy), (hl,), (a, b))
         assert gh[keep].equal(want[keep])
+
+
+def test_checked_calls_over_logits(monkeypatch):
+    """With bounds checks on, an eager call raises by itself; a captured one, which cannot wait, is recorded."""
+    import nimbleml_b200.losses.logprobs as mod
+
+    monkeypatch.setattr(mod, "CHECK_BOUNDS", True)
+    x, tokens, _ = make_logits(6, 700, torch.float16, 5)
+    want = mod.token_logprobs(x, tokens, top_k=3)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = mod.token_logprobs(x, tokens, top_k=3)
+    graph.replay()
+    assert all(a.equal(b) for a, b in zip(got, want))
+    tokens[2] = 700
+    with pytest.raises(ValueError, match="out of range"):
+        mod.token_logprobs(x, tokens)
+    mod.check_status(x.device)
