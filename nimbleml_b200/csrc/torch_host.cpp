@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -66,7 +67,7 @@ void refuse_recording(const char* name) {
               name, " cannot be traced: the trace would not hold its kernels");
 }
 void refuse_tangent(const char* name, const Tensor& t) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name,
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), name,
                               " has no forward-mode derivative, and an input has a tangent");
 }
 void refuse_transforms(const std::string& name, const Tensor& a, const std::optional<Tensor>& b) {
@@ -487,13 +488,16 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
   std::vector<Tensor> keep;  // contiguous copies of gradients, until the launches are queued
   std::optional<at::Device> dev;
   bool eight = false;
+  const bool duals = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // none outside a level
   // Every tensor is checked before the first launch: a refused step leaves all of them as they were.
   for (Py_ssize_t i = 0; i < params.n; ++i) {
     if (grads.at[i] == Py_None) continue;
     const Tensor& p = tensor_in(params.at[i], "a parameter");
     const Tensor* g = &tensor_in(grads.at[i], "a gradient");
-    refuse_tangent("adamw_step_many", p);
-    refuse_tangent("adamw_step_many", *g);
+    if (duals) {
+      refuse_tangent("adamw_step_many", p);
+      refuse_tangent("adamw_step_many", *g);
+    }
     if (!dev) {
       dev = p.device();
       TORCH_CHECK_VALUE(p.is_cuda(), "adamw_step_many needs CUDA tensors; there is no CPU path");
@@ -554,15 +558,15 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
   void* stream = c10::cuda::getCurrentCUDAStream(dev->index()).stream();
   const double bc1 = 1.0 - std::pow(beta1, static_cast<double>(step));
   const double bc2 = 1.0 - std::pow(beta2, static_cast<double>(step));
-  std::vector<nimble_adamw_tensor> rows;
-  rows.reserve(all.size());
+  size_t start = 0, end = 0;  // of the next list: all[start, end), moved up over those that step alone
   std::unordered_set<const void*> seen;
+  seen.reserve(all.size());
   auto launch = [&] {
-    if (!rows.empty())
-      check_rc(nimble_adamw_step_many(rows.data(), static_cast<int>(rows.size()), eight ? 8 : 32, lr, beta1, beta2,
-                                      bc1, bc2, eps, wd, stream),
+    if (end > start)
+      check_rc(nimble_adamw_step_many(all.data() + start, static_cast<int>(end - start), eight ? 8 : 32, lr, beta1,
+                                      beta2, bc1, bc2, eps, wd, stream),
                "nimble_adamw_step_many");
-    rows.clear();
+    start = end;
     seen.clear();
   };
   auto whole = [](const nimble_adamw_tensor& t) {  // what the single step's vector kernel takes
@@ -572,10 +576,11 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
       bits |= reinterpret_cast<uintptr_t>(p);
     return t.n % 8 == 0 && (bits & 15) == 0;
   };
-  for (const nimble_adamw_tensor& t : all) {
-    const bool alone = own_steps && !eight && !whole(t);
-    if (seen.count(t.weights)) launch();  // listed twice: its second update follows the first
-    if (alone) {
+  for (size_t i = 0; i < all.size(); ++i) {
+    const nimble_adamw_tensor t = all[i];
+    // Weights that are listed twice: the second update follows the first.
+    if (own_steps && !eight && !whole(t)) {
+      if (seen.count(t.weights)) launch();
       check_rc(nimble_adamw_step(t.weights, t.grad, t.grad_dtype, static_cast<float*>(t.exp_avg),
                                  static_cast<float*>(t.exp_avg_sq), t.n, static_cast<float>(lr),
                                  static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(bc1),
@@ -584,8 +589,11 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
                "nimble_adamw_step");
       continue;
     }
-    seen.insert(t.weights);
-    rows.push_back(t);
+    if (!seen.insert(t.weights).second) {
+      launch();
+      seen.insert(t.weights);
+    }
+    all[end++] = t;
   }
   launch();
 }
