@@ -359,3 +359,63 @@ def test_a_refused_list_changes_nothing(bits):
         adamw_step_many([p, p, p], [g, g, g[:100]], m[:3], m[3:], step=1)
     torch.cuda.synchronize()
     assert (p == 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_state(bits):
+    """Weights, moments (codes and scales) and copies of a replayed step, bit for bit as eager ones."""
+    from nimbleml_b200.embedding_grad import adamw_step_many, quantize_moment
+
+    sizes = [1, 300, 16, 9000, 129]
+    ps, gs, cs, _, _, _ = make(sizes, torch.bfloat16, torch.float16, 1, 19)
+
+    def state():
+        p = [x.clone() for x in ps]
+        z = [torch.zeros_like(x) for x in ps]
+        if bits == 8:
+            return p, [quantize_moment(x) for x in z], [quantize_moment(x) for x in z], [x.clone() for x in cs]
+        return p, z, [x.clone() for x in z], [x.clone() for x in cs]
+
+    a, b = state(), state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        adamw_step_many(b[0], gs, b[1], b[2], step=3, copies=b[3], **HYPER)
+    side = torch.cuda.Stream()
+    for turn in range(3):
+        adamw_step_many(a[0], gs, a[1], a[2], step=3, copies=a[3], **HYPER)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side if turn == 1 else torch.cuda.current_stream()):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(side)
+        for one, two in zip(a, b):
+            for x, y in zip(one, two):
+                for u, v in zip(x, y) if isinstance(x, tuple) else ((x, y),):
+                    assert u.view(torch.uint8).equal(v.view(torch.uint8))
+        for g in gs:
+            g.mul_(0.5)
+
+
+@pytest.mark.parametrize("beta2", [0.9, 0.999, 0.9999])
+def test_32_bit_moments_against_64_bits(beta2):
+    """The step's betas are fp32 numbers and its 1 - beta is theirs, exactly: with these, v is off by three roundings a
+    step (all its terms are positive), m by three of the sum of magnitudes. Against the betas as given, off by e <= 2^-25,
+    a term (1 - beta2) beta2^k g^2 moves by e / (1 - beta2) + k e / beta2 of itself."""
+    from nimbleml_b200.embedding_grad import adamw_step_many
+
+    g = torch.Generator().manual_seed(7)
+    n, steps, u = 1027, 25, 2.0**-24
+    p, m, v = torch.randn(n, generator=g).cuda(), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    b1f, b2f = float(np.float32(0.9)), float(np.float32(beta2))
+    m64, v64, big, given = (torch.zeros(n, dtype=torch.float64, device="cuda") for _ in range(4))
+    for t in range(1, steps + 1):
+        gr = torch.randn(n, generator=g).cuda()
+        adamw_step_many([p], [gr], [m], [v], step=t, beta1=0.9, beta2=beta2)
+        g64 = gr.double()
+        m64 = b1f * m64 + (1 - b1f) * g64
+        big = b1f * big + (1 - b1f) * g64.abs()
+        v64 = b2f * v64 + (1 - b2f) * g64 * g64
+        given = beta2 * given + (1 - beta2) * g64 * g64
+        assert ((m.double() - m64).abs() <= 1.01 * 3 * t * u * big).all()
+        assert ((v.double() - v64).abs() <= 1.01 * 3 * t * u * v64).all()
+        e = 2.0**-25
+        assert ((v.double() - given).abs() <= (1.01 * 3 * t * u + e / (1 - beta2) + t * e / beta2) * 1.01 * given).all()

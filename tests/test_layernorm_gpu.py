@@ -213,3 +213,38 @@ def test_captured_and_on_another_stream():
     graph.replay()
     for a, b in zip(got, run(x, gamma, beta, gy)):
         assert a.equal(b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,d,off", [(1, 520, 0), (7, 520, 0), (13, 33, 0), (7, 520, 1), (15, 4104, 0), (33, 8191, 0), (3, 2048, 0)])
+def test_nothing_behind_the_outputs_is_written(dtype, n, d, off):
+    """Rows go in pairs and eights: odd counts and widths, with vectors and (off the 16-byte grid) without."""
+    from nimbleml_b200._native_loader import native
+    from nimbleml_b200.embedding_grad import _TORCH_TO_NIMBLE, _stream_ptr
+
+    x, gamma, beta, gy = make(n, d, dtype, torch.float32, n + d)
+    want = run(x, gamma, beta, gy)
+
+    def room(size, dt):  # `size` elements behind `off`, with a sentinel on both sides
+        buf = torch.full((off + size + 64 * 1024,), 7.0, device="cuda").to(dt)
+        return buf, buf[off:off + size]
+
+    bufs = {k: room(size, dt) for k, size, dt in (("y", n * d, dtype), ("mean", n, torch.float32), ("rstd", n, torch.float32),
+                                                  ("gx", n * d, dtype), ("gg", d, torch.float32), ("gb", d, torch.float32))}
+    at = {k: part.data_ptr() for k, (_, part) in bufs.items()}
+    need = native.layernorm_backward_workspace_size(n, d)
+    ws = torch.full((need + 4096,), 7, dtype=torch.uint8, device="cuda")
+    t, s = _TORCH_TO_NIMBLE[dtype], _stream_ptr(x.device)
+    f32 = _TORCH_TO_NIMBLE[torch.float32]
+    native.call("nimble_layernorm_forward", x.data_ptr(), d, gamma.data_ptr(), beta.data_ptr(), n, d, 1e-5, t, f32, at["y"],
+                at["mean"], at["rstd"], s)
+    native.call("nimble_layernorm_backward", gy.data_ptr(), x.data_ptr(), d, gamma.data_ptr(), at["mean"], at["rstd"], n, d, t, f32,
+                at["gx"], at["gg"], at["gb"], ws.data_ptr(), need, s)
+    y, gx, gg, gb = (bufs[k][1] for k in ("y", "gx", "gg", "gb"))
+    if off == 0:
+        assert y.equal(want[0].view(-1)) and gx.equal(want[1].view(-1)) and gg.equal(want[2]) and gb.equal(want[3])
+    else:  # element by element: sums in another order
+        check(x, gamma, beta, 1e-5, gy, y.view(n, d), gx.view(n, d), gg, gb)
+    for buf, part in bufs.values():
+        assert (buf[:off] == 7).all() and (buf[off + part.numel():] == 7).all()
+    assert (ws[need:] == 7).all()

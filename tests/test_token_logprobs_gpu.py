@@ -858,3 +858,45 @@ def test_checked_calls_over_logits(monkeypatch):
     with pytest.raises(ValueError, match="out of range"):
         mod.token_logprobs(x, tokens)
     mod.check_status(x.device)
+
+
+# (tokens, d, vocabulary, columns a slab (0: the library's), slabs, runs of grad_hidden's product in each).
+SLABS_AND_RUNS = [(300, 72, 5003, 2048, 3, 4), (300, 72, 4196, 2048, 3, 4), (70, 264, 3000, 1024, 3, 2), (513, 520, 4100, 1536, 3, 3),
+                  (300, 72, 4097, 4096, 2, 8), (2700, 64, 50000, 0, 2, 6)]
+
+
+def slab_workspace(n, d, cols, slabs, runs, dtype):
+    """Bytes that the backward asks for with this many slabs and runs: G, the runs' sums, the row coefficients, the
+    scale, and for fp16 the rows' factors and hidden copy, each from a multiple of 256."""
+    up = lambda x: -(-x // 256) * 256  # noqa: E731
+    total = up(2 * n * cols) + (up(4 * n * d * runs) if slabs > 1 or runs > 1 else 0) + up(16 * n) + up(4)
+    return total + (up(4 * n) + up(2 * n * d) if dtype == torch.float16 else 0)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("shape", SLABS_AND_RUNS)
+@pytest.mark.parametrize("buffer", [False, True])
+def test_tied_several_slabs_in_several_runs(dtype, shape, buffer, monkeypatch):
+    """The runs' partial grad_hidden goes from slab to slab; a last slab of 100 columns (two 64-column blocks) or one leaves
+    runs without any."""
+    import nimbleml_b200.losses.logprobs as mod
+    from nimbleml_b200.embedding_grad import _TORCH_TO_NIMBLE
+
+    n, d, v, cols, slabs, runs = shape
+    slab_bytes = 2 * n * cols
+    cols = cols or 25088  # half of 50000 columns in whole tiles
+    assert -(-v // cols) == slabs
+    assert mod.native.tied_logprobs_backward_workspace_size(n, d, v, _TORCH_TO_NIMBLE[dtype], slab_bytes) == slab_workspace(
+        n, d, cols, slabs, runs, dtype)
+    monkeypatch.setattr(mod, "SLAB_BYTES", slab_bytes)
+    h, w, tokens, g = make_tied(n, d, v, dtype, n + v)
+    tokens[::7] = IGN
+    tokens[1] = v - 1  # in the last slab
+    a, b = torch.randn(n, generator=g).cuda(), torch.randn(n, generator=g).cuda()
+    base = torch.randn(v, d, generator=g).cuda() if buffer else None
+    buf = base.clone() if buffer else None
+    hl, wl = h.detach().requires_grad_(), w.detach().requires_grad_(not buffer)
+    r = mod.tied_token_logprobs(hl, wl, tokens, IGN, grad_weights_buffer=buf)
+    grads = torch.autograd.grad((r.logprobs, r.entropy), (hl,) if buffer else (hl, wl), (a, b))
+    check_tied_grads(grads[0], buf if buffer else grads[1], h, w, tokens, a, b, base)
+    assert (grads[0][tokens == IGN] == 0).all()
