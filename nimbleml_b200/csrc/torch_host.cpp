@@ -18,10 +18,11 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdint>
 #include <optional>
 #include <string>
-#include <unordered_set>
 #include <vector>
 
 #include "nimbleml_tied_ce.h"
@@ -473,6 +474,33 @@ void check_quantized(const Tensor& codes, const Tensor& scales) {
   TORCH_CHECK_VALUE(codes.is_cuda() && scales.device() == codes.device(), "8-bit moments live on one CUDA device");
 }
 
+// A set of at most n pointers, none of them null, in one allocation.
+class PointerSet {
+ public:
+  explicit PointerSet(size_t n) {
+    size_t size = 2;
+    while (size < 2 * n) size *= 2;
+    slots_.assign(size, nullptr);
+  }
+  bool has(const void* p) const { return slots_[find(p)] != nullptr; }
+  bool insert(const void* p) {  // false where it was there
+    const size_t at = find(p);
+    if (slots_[at]) return false;
+    slots_[at] = p;
+    return true;
+  }
+  void clear() { std::fill(slots_.begin(), slots_.end(), nullptr); }
+
+ private:
+  size_t find(const void* p) const {  // its place, or the free one that it would take
+    const uint64_t h = (reinterpret_cast<uintptr_t>(p) >> 2) * 0x9E3779B97F4A7C15ull;
+    size_t at = (h >> 32) & (slots_.size() - 1);
+    while (slots_[at] && slots_[at] != p) at = (at + 1) & (slots_.size() - 1);
+    return at;
+  }
+  std::vector<const void*> slots_;
+};
+
 void adamw_step_many(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_,
                      const py::object& copies_, int64_t step, double lr, double beta1, double beta2, double eps,
                      double wd, bool own_steps) {
@@ -486,6 +514,9 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
   std::vector<nimble_adamw_tensor> all;
   all.reserve(params.n);
   std::vector<Tensor> keep;  // contiguous copies of gradients, until the launches are queued
+  std::vector<c10::TensorImpl*> written;
+  written.reserve(6 * params.n);
+  auto writes = [&](const Tensor& t) { written.push_back(t.unsafeGetTensorImpl()); };
   std::optional<at::Device> dev;
   bool eight = false;
   const bool duals = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;  // none outside a level
@@ -527,6 +558,8 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
                           "moments must have the sizes and the device of their weights");
         values = codes.data_ptr();
         scales = static_cast<float*>(s.data_ptr());
+        writes(codes);
+        writes(s);
       } else {
         TORCH_CHECK_VALUE(THPVariable_Check(o), "moments are all fp32 tensors or all (codes, scales) pairs");
         const Tensor& t = THPVariable_Unpack(o);
@@ -535,6 +568,7 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
         TORCH_CHECK_VALUE(t.numel() == n && t.device() == *dev,
                           "moments must have the sizes and the device of their weights");
         values = t.data_ptr();
+        writes(t);
       }
     };
     moment(ms.at[i], r.exp_avg, r.exp_avg_scale);
@@ -545,8 +579,10 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
       TORCH_CHECK_VALUE(r.weights_copy_dtype >= 0 && c.numel() == n && c.is_contiguous() && c.device() == *dev,
                         "a copy must be contiguous, on the device and of the size of its weights");
       r.weights_copy = c.data_ptr();
+      writes(c);
     }
     if (n == 0) continue;
+    writes(p);
     r.weights = static_cast<float*>(p.data_ptr());
     r.grad = g->data_ptr();
     r.n = n;
@@ -559,8 +595,7 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
   const double bc1 = 1.0 - std::pow(beta1, static_cast<double>(step));
   const double bc2 = 1.0 - std::pow(beta2, static_cast<double>(step));
   size_t start = 0, end = 0;  // of the next list: all[start, end), moved up over those that step alone
-  std::unordered_set<const void*> seen;
-  seen.reserve(all.size());
+  PointerSet seen(all.size());
   auto launch = [&] {
     if (end > start)
       check_rc(nimble_adamw_step_many(all.data() + start, static_cast<int>(end - start), eight ? 8 : 32, lr, beta1,
@@ -580,7 +615,7 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
     const nimble_adamw_tensor t = all[i];
     // Weights that are listed twice: the second update follows the first.
     if (own_steps && !eight && !whole(t)) {
-      if (seen.count(t.weights)) launch();
+      if (seen.has(t.weights)) launch();
       check_rc(nimble_adamw_step(t.weights, t.grad, t.grad_dtype, static_cast<float*>(t.exp_avg),
                                  static_cast<float*>(t.exp_avg_sq), t.n, static_cast<float>(lr),
                                  static_cast<float>(beta1), static_cast<float>(beta2), static_cast<float>(bc1),
@@ -589,13 +624,16 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
                "nimble_adamw_step");
       continue;
     }
-    if (!seen.insert(t.weights).second) {
+    if (!seen.insert(t.weights)) {
       launch();
       seen.insert(t.weights);
     }
     all[end++] = t;
   }
   launch();
+  // As torch's own in-place updates: a backward pass that still needs an old value raises.
+  for (c10::TensorImpl* t : written)
+    if (!t->is_inference()) t->bump_version();
 }
 
 }  // namespace

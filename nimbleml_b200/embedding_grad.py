@@ -125,7 +125,8 @@ def adamw_step_many(params: Sequence[torch.Tensor], grads: Sequence[Optional[tor
     these are rounded. A gradient that is not finite spoils its own weight and,
     with 8-bit moments, the block of 128 it lies in. A captured step keeps the
     scalars it was captured with. All tensors are checked first: a step that is
-    refused changes none of them.
+    refused changes none of them. It counts as an in-place write: a backward
+    pass that has kept an updated tensor raises.
     """
     host.adamw_step_many(params, grads, exp_avgs, exp_avg_sqs, copies, int(step), float(learning_rate), float(beta1),
                          float(beta2), float(epsilon), float(weight_decay), False)

@@ -419,3 +419,36 @@ def test_32_bit_moments_against_64_bits(beta2):
         assert ((v.double() - v64).abs() <= 1.01 * 3 * t * u * v64).all()
         e = 2.0**-25
         assert ((v.double() - given).abs() <= (1.01 * 3 * t * u + e / (1 - beta2) + t * e / beta2) * 1.01 * given).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_counts_as_a_write(bits):
+    """A backward pass over what a step has overwritten since the forward is refused, not taken from the new values."""
+    from nimbleml_b200.embedding_grad import AdamW
+    from nimbleml_b200.losses import tied_token_logprobs
+    from nimbleml_b200.norm import layer_norm
+
+    gamma = torch.ones(64, device="cuda", requires_grad=True)
+    master = torch.randn(300, 64, device="cuda")
+    weight = master.half().requires_grad_()
+    x = torch.randn(5, 64, device="cuda").half().requires_grad_()
+    opt = AdamW([gamma, master], copies=[None, weight.detach()], state_bits=bits, learning_rate=0.1)
+    gamma.grad, master.grad = torch.ones_like(gamma), torch.ones_like(master)
+    y = layer_norm(x.float(), gamma)
+    r = tied_token_logprobs(x, weight, torch.arange(5, device="cuda"))
+    before = [t._version for t in (gamma, master, weight)]
+    opt.step()
+    assert all(t._version > v for t, v in zip((gamma, master, weight), before))
+    assert all(m._version > 0 for q in (*opt.m, *opt.v) for m in (q if bits == 8 else (q,)))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logprobs.sum().backward()
+    # Afresh all is well; inference tensors, which count nothing, are stepped too.
+    (layer_norm(x.float(), gamma).sum() + tied_token_logprobs(x, weight, torch.arange(5, device="cuda")).logprobs.sum()).backward()
+    with torch.inference_mode():
+        p = torch.ones(40, device="cuda")
+        p.grad = torch.ones(40, device="cuda")
+        inside = AdamW([p], state_bits=bits)
+        inside.step()
+        assert (p < 1).all()
