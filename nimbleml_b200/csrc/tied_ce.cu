@@ -6,7 +6,7 @@
 //             lse = m + log s; loss = mean_i (lse_i - S_i,y_i)
 //   backward: G = (exp(S - m) / s - onehot(y)) * grad_scale / N
 //             dh = G E ; dE = G^T h
-// Here nothing N x V is ever stored:
+// Here the logits are never stored, and of G one vocabulary slab at a time:
 //   forward : one persistent tcgen05 GEMM over (token block x vocab tile)
 //             tiles whose epilogue reduces each TMEM accumulator row to a
 //             (max, sum-exp) pair and gathers the target logit; a row reduce
@@ -18,8 +18,9 @@
 //             slab's share of dh, reading G, h and E in place (MN-major
 //             operands where the contraction runs along their rows).
 // The log probability and entropy of every token (instead of the mean loss) are two
-// more epilogues of the same GEMM, with a slab backward of the same shape and a kernel
-// of their own for few tokens; they follow the cross-entropy entry points below.
+// more epilogues of the same GEMM, with a slab backward of the same shape (one slab, all
+// of G, up to 256 MiB) and a kernel of their own for few tokens; they follow the
+// cross-entropy entry points below.
 // All GEMMs compute C[M x N] = A[M x K] . B[N x K]^T with operands staged by
 // TMA (128-byte swizzle) into a shared-memory ring and fp32 accumulators
 // double-buffered in TMEM.
@@ -1092,12 +1093,12 @@ struct BwdLayout {
   int64_t slab = 0, n_slabs = 0;
   size_t g = 0, dh = 0, hr = 0, er = 0, total = 0;
 };
-// `whole_vocab`: the shard may be the entire vocabulary (one GPU), so the
-// backward walks it in at least two slabs and no G buffer ever holds more
-// than half of the N x V logits. A shard of a vocabulary split over P >= 2
-// ranks is at most half of it already; its slabs follow the byte budget
-// alone, so a shard whose G fits the budget is one slab and needs no fp32
-// grad_hidden accumulator.
+// `whole_vocab` (the caller's choice): at least two slabs, so that no G buffer ever
+// holds more than half of the shard's N x V_local. Without it the slabs follow the byte
+// budget alone, and a shard whose G fits the budget is one slab and needs no fp32
+// grad_hidden accumulator. Cross-entropy asks for it where the shard may be the entire
+// vocabulary (one GPU; a shard of a vocabulary split over P >= 2 ranks is at most half
+// of it already), the log probabilities where G is larger than 256 MiB.
 BwdLayout bwd_layout(int64_t N, int64_t d, int64_t V, int dtype, size_t slab_bytes, bool whole_vocab = true) {
   BwdLayout L;
   const int64_t es = elem_size(dtype);
@@ -1545,7 +1546,15 @@ extern "C" int nimble_tied_logits_backward(const void* grad_logits, int64_t grad
 // the hidden states and the tied matrix: the forward GEMM with an epilogue that
 // also sums d 2^d, and the slab backward with a gradient of its own per row,
 //   G_ij = a_i [j = t_i] - p_ij (a_i + b_i H_i + b_i log p_ij),
-// a = d loss / d logp, b = d loss / d H. No N x V buffer exists in either pass.
+// a = d loss / d logp, b = d loss / d H. The forward keeps nothing N x V; the backward
+// holds at most half of G in the compute type, or all of it up to 256 MiB.
+//
+// G is rounded to the 16 bits that the tensor cores multiply at full rate, once, as in
+// the cross-entropy path: each element off by half a step of its own. In grad_hidden
+// and in dE of many tokens these errors average out (gradients 1.4 times as far from the
+// exact ones as from a G in fp32); dE of a handful of tokens is a sum of a handful of
+// such terms, off by up to half a step of each. A G in two 16-bit parts would double
+// both products.
 
 namespace nimble {
 namespace {

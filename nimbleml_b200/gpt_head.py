@@ -174,7 +174,8 @@ class TiedEmbedding:
 
     def token_logprobs(self, hidden: torch.Tensor, tokens, ignore_index: Optional[int] = None) -> TokenLogProbs:
         """Log probability of every token and entropy of every row of the tied head
-        over ``hidden`` (..., d), 16-bit; the head's dE is added into ``grad``."""
+        over ``hidden`` (..., d), 16-bit (a float32 ``compute_dtype`` raises
+        ValueError); the head's dE is added into ``grad``."""
         return tied_token_logprobs(hidden, self.weight, tokens, ignore_index, vocab_offset=self.vocab_offset,
                                    vocab_size=self.vocab_size, group=self.group if self.world > 1 else None,
                                    grad_weights_buffer=self.grad)

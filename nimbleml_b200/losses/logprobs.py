@@ -250,7 +250,9 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
             adds the weight grad into; autograd then gets none for ``weights``.
 
     The gradient of the logits is formed in the compute dtype, so gradients
-    carry one 16-bit rounding more than their own.
+    carry one 16-bit rounding more than their own. It averages out over many
+    tokens; with a handful of them each term of the weight grad has it whole.
+    Upstream gradients may have any size, and any sizes beside each other.
     """
     host.refuse_transforms("tied_token_logprobs", hidden, weights)
     if not hidden.is_cuda:
