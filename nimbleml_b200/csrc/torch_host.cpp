@@ -71,10 +71,9 @@ void refuse_tangent(const char* name, const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), name,
                               " has no forward-mode derivative, and an input has a tangent");
 }
-void refuse_transforms(const std::string& name, const Tensor& a, const std::optional<Tensor>& b) {
-  refuse_recording(name.c_str());
-  refuse_tangent(name.c_str(), a);
-  if (b) refuse_tangent(name.c_str(), *b);
+void refuse_transforms(const char* name, const Tensor& t) {
+  refuse_recording(name);
+  refuse_tangent(name, t);
 }
 
 // t in a type, contiguous; t itself, without a call to torch, where it is both.
@@ -168,8 +167,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
 };
 
 Tensor layer_norm(const Tensor& x, const Tensor& gamma, const std::optional<Tensor>& beta, double eps) {
-  refuse_recording("layer_norm");
-  refuse_tangent("layer_norm", x);
+  refuse_transforms("layer_norm", x);
   refuse_tangent("layer_norm", gamma);
   if (beta) refuse_tangent("layer_norm", *beta);
   TORCH_CHECK(x.is_cuda(), "layer_norm on B200 needs CUDA tensors; there is no CPU path");
@@ -640,7 +638,17 @@ void adamw_step_many(const py::object& params_, const py::object& grads_, const 
 
 PYBIND11_MODULE(nimbleml_b200_host, m) {
   m.doc() = "Host side of layer_norm, the token log probabilities and adamw_step_many over the C ABI";
-  m.def("refuse_transforms", &refuse_transforms, py::arg("name"), py::arg("a"), py::arg("b") = std::nullopt);
+  // What the package's functions begin with where their own checks come before the host's.
+  m.def("begin_token_logprobs", [](const Tensor& x) { refuse_transforms("token_logprobs", x); });
+  m.def("begin_tied_token_logprobs", [](const Tensor& h, const Tensor& w) {
+    refuse_transforms("tied_token_logprobs", h);
+    refuse_tangent("tied_token_logprobs", w);
+  });
+  m.def("begin_quantize", [](const Tensor& x) { refuse_transforms("quantize_moment", x); });
+  m.def("begin_dequantize", [](const Tensor& codes, const Tensor& scales) {
+    refuse_transforms("dequantize_moment", codes);
+    refuse_tangent("dequantize_moment", scales);
+  });
   m.def("layer_norm", &layer_norm);
   m.def("token_logprobs", &token_logprobs);
   m.def("set_status_hooks", &set_status_hooks);

@@ -78,7 +78,7 @@ def _check_quantized(codes: torch.Tensor, scales: torch.Tensor) -> None:
 
 def quantize_moment(x: torch.Tensor, *, root: bool = False) -> QuantizedMoment:
     """An fp32 moment in 8 bits; ``root`` for the second moment, which is held as its root."""
-    host.refuse_transforms("quantize_moment", x)
+    host.begin_quantize(x)
     if x.dtype != torch.float32 or not x.is_cuda:
         raise ValueError("moments are float32 CUDA tensors")
     x = x.contiguous()
@@ -92,7 +92,7 @@ def quantize_moment(x: torch.Tensor, *, root: bool = False) -> QuantizedMoment:
 
 def dequantize_moment(codes: torch.Tensor, scales: torch.Tensor, *, root: bool = False) -> torch.Tensor:
     """The fp32 values that 8-bit codes stand for (``root``: their squares, the second moment)."""
-    host.refuse_transforms("dequantize_moment", codes, scales)
+    host.begin_dequantize(codes, scales)
     _check_quantized(codes, scales)
     out = torch.empty(codes.shape, dtype=torch.float32, device=codes.device)
     with _on(codes.device):

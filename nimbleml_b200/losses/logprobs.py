@@ -103,7 +103,7 @@ def token_logprobs(logits: torch.Tensor, tokens, ignore_index: Optional[int] = N
     A token outside the classes gives a NaN log probability and sets the
     status word's bad-label bit.
     """
-    host.refuse_transforms("token_logprobs", logits)
+    host.begin_token_logprobs(logits)
     if not logits.is_cuda:
         raise RuntimeError("token_logprobs on B200 needs CUDA tensors; there is no CPU path")
     compute_dtype_of(logits)
@@ -254,7 +254,7 @@ def tied_token_logprobs(hidden: torch.Tensor, weights: torch.Tensor, tokens, ign
     tokens; with a handful of them each term of the weight grad has it whole.
     Upstream gradients may have any size, and any sizes beside each other.
     """
-    host.refuse_transforms("tied_token_logprobs", hidden, weights)
+    host.begin_tied_token_logprobs(hidden, weights)
     if not hidden.is_cuda:
         raise RuntimeError("tied_token_logprobs on B200 needs CUDA tensors; there is no CPU path")
     if hidden.dtype not in (torch.float16, torch.bfloat16):
