@@ -186,7 +186,8 @@ class TiedEmbedding:
     @torch.no_grad()
     def step(self) -> None:
         """One AdamW step over the shard's master rows; the compute copy is
-        rewritten in the same kernel pass."""
+        rewritten in the same kernel pass. It counts as an in-place write: the
+        backward of an earlier :meth:`token_logprobs` raises."""
         self.t += 1
         bc1 = 1.0 - self.beta1 ** self.t
         bc2 = 1.0 - self.beta2 ** self.t
@@ -194,6 +195,9 @@ class TiedEmbedding:
                     self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), self.master.numel(), self.lr, self.beta1,
                     self.beta2, bc1, bc2, self.epsilon, self.weight_decay, self.weight.data_ptr(),
                     _TORCH_TO_NIMBLE[self.weight.dtype], _stream_ptr(self.master.device))
+        for t in (self.master, self.exp_avg, self.exp_avg_sq, self.weight):
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
 
 __all__ = ["norm_tied_cross_entropy", "TiedEmbedding"]

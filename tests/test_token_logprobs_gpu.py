@@ -900,3 +900,23 @@ def test_tied_several_slabs_in_several_runs(dtype, shape, buffer, monkeypatch):
     grads = torch.autograd.grad((r.logprobs, r.entropy), (hl,) if buffer else (hl, wl), (a, b))
     check_tied_grads(grads[0], buf if buffer else grads[1], h, w, tokens, a, b, base)
     assert (grads[0][tokens == IGN] == 0).all()
+
+
+def test_a_step_of_the_tied_matrix_counts_as_a_write():
+    """The backward recomputes the logits from the tied matrix: after a step it is refused, not taken from the new one."""
+    from nimbleml_b200.gpt_head import TiedEmbedding
+
+    h, w, tokens, g = make_tied(9, 64, 300, torch.float16, 5)
+    emb = TiedEmbedding(w.float(), 300)
+    hl = h.requires_grad_()
+    r = emb.token_logprobs(hl, tokens)
+    emb.grad.fill_(1.0)
+    emb.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.logprobs.sum().backward()
+    emb.token_logprobs(hl, tokens).logprobs.sum().backward()
+    with torch.inference_mode():
+        inside = TiedEmbedding(w.float(), 300)
+        inside.grad.fill_(1.0)
+        inside.step()
+        assert (inside.master < w.float()).any()
