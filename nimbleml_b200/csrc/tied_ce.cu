@@ -1921,6 +1921,8 @@ __global__ void split_sum_kernel(const float* __restrict__ partial, int runs, in
 // which elements of order one become 2^22 below the largest row. Rows within 2^8, as
 // nearly all are in training, have k = 0 and the bits that one factor gives them. The block
 // of a row takes the largest bound of all rows itself, which is little beside a launch more.
+// Factors and copy add 2 to 3 us to the backward of 64 / 320 / 2048 x 768 x 50257 fp16
+// (82 -> 84, 119 -> 121, 373 -> 375), nothing to that of 16 tokens (80).
 constexpr int kPrepThreads = 1024;
 constexpr int kNearTop = 8;                     // log2 of a bound's distance that needs no factor of its own
 // Limits of f and f + k, and of k: normal numbers, with normal reciprocals.
